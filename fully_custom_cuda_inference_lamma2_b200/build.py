@@ -27,8 +27,9 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 LIB = os.path.join(PKG, "libfcci_decode.so")
-LIB_SOURCES = ["decode_attn.cu", "capi.cu", "compat.cu", "noalloc.cu", "prefill_attn.cu", "gemv.cu", "step.cu", "exchange.cu"]
-LIB_HEADERS = ["ptx.cuh", "tcgen05.cuh", "fcci_internal.h"]
+LIB_SOURCES = ["decode_attn.cu", "capi.cu", "compat.cu", "noalloc.cu", "prefill_attn.cu", "gemv.cu", "step.cu", "exchange.cu",
+               "paged_append.cu", "paged_attn.cu"]
+LIB_HEADERS = ["ptx.cuh", "tcgen05.cuh", "fcci_internal.h", "paged.cuh"]
 MODULES = {
     "attn_varlen": "attn_varlen_module.cpp",
     "capture_decode_step": "capture_decode_step_module.cpp",
@@ -56,7 +57,8 @@ def _run(cmd: list[str], cwd: str | None = None) -> None:
 
 
 def _common_headers() -> list[str]:
-    return [os.path.join(INCLUDE, h) for h in ("fcci_decode.h", "fcci_compat.h", "fcci_prefill.h", "fcci_exchange.h")]
+    return [os.path.join(INCLUDE, h) for h in ("fcci_decode.h", "fcci_compat.h", "fcci_prefill.h", "fcci_exchange.h",
+                                                 "fcci_paged.h")]
 
 
 def build_library(force: bool = False) -> str:
@@ -81,7 +83,7 @@ def build_library(force: bool = False) -> str:
 def build_module(name: str, force: bool = False) -> str:
     src = os.path.join(CSRC, MODULES[name])
     out = module_path(name)
-    deps = [src, os.path.join(CSRC, "binding_common.h"), LIB] + _common_headers()
+    deps = [src, os.path.join(CSRC, "binding_common.h"), os.path.join(CSRC, "paged_binding.h"), LIB] + _common_headers()
     if not force and _newer(out, deps):
         return out
     import torch

@@ -10,6 +10,7 @@
 #include "binding_common.h"
 #include "fcci_exchange.h"
 #include "fcci_prefill.h"
+#include "paged_binding.h"
 
 using namespace fcci_py;
 
@@ -474,6 +475,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             return (int64_t)flags;
         },
         py::arg("workspace"), py::arg("clear") = true);
+    def_paged(m);
     m.def("launch_count", []() { return (int64_t)fcci_launch_count(); });
     // ctx exchange plumbing (fcci_exchange.h): IPC buffers and the bounded flag wait
     m.def(

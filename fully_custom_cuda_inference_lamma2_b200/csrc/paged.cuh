@@ -1,0 +1,152 @@
+// What the kernels of the paged KV cache share: the launch parameters, a sequence's ranges,
+// the e4m3 / power-of-two scale arithmetic and the position rotation.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "fcci_internal.h"
+#include "fcci_paged.h"
+#include "ptx.cuh"
+
+namespace fcci {
+namespace pg {
+
+constexpr int kMaxRot = 256;
+constexpr int kScaleMin = -15, kScaleMax = 8;  // exponents of a page's scale
+
+struct Params {
+    int32_t B, Hq, Hkv, G, D;
+    int32_t total_q, max_q;
+    const int32_t* cu_q;
+    const __half* q;
+    int64_t q_st, q_sh;
+    const __half* k_new;
+    int64_t kn_st, kn_sh;
+    const __half* v_new;
+    int64_t vn_st, vn_sh;
+    int32_t page, page_log2, num_pages, max_pages;
+    uint8_t* k_pages;  // strides in bytes
+    int64_t k_sp, k_sh, k_st;
+    uint8_t* v_pages;
+    int64_t v_sp, v_sh, v_st;
+    uint8_t* k_scales;
+    int64_t ks_sp, ks_sh;
+    uint8_t* v_scales;
+    int64_t vs_sp, vs_sh;
+    const int32_t* table;
+    int64_t table_st;
+    int32_t* seq_lens;
+    __half* out;
+    int64_t o_st, o_sh;
+    __half* q_rot;  // [total_q, Hq, D] contiguous
+    float scale_log2;
+    int32_t rot;
+    int32_t advance;
+    int32_t append;
+    uint32_t* err;
+    uint32_t* done_cnt;
+};
+
+// Frequencies theta^(-2i/rot) / 2 pi in turns per position, as 64-bit fixed-point fractions:
+// pos * freq wraps modulo one turn by itself, so the angle of a far position loses nothing.
+struct Freqs {
+    uint64_t turn[kMaxRot / 2];
+};
+
+struct Seq {
+    int T, n, tok0;  // cached rows, new tokens, first row of the new tokens
+    bool ok;
+};
+
+__device__ __forceinline__ Seq seq_of(const Params& p, int b) {
+    Seq s;
+    s.T = p.seq_lens[b];
+    s.tok0 = p.cu_q ? p.cu_q[b] : b;
+    s.n = p.cu_q ? p.cu_q[b + 1] - s.tok0 : 1;
+    const long long cap = (long long)p.max_pages << p.page_log2;
+    s.ok = s.T >= 0 && s.n >= 0 && s.n <= p.max_q && s.tok0 >= 0 && (long long)s.tok0 + s.n <= p.total_q &&
+           (long long)s.T + (p.append ? s.n : 0) <= cap;
+    return s;
+}
+
+__device__ __forceinline__ void set_error(const Params& p, uint32_t bit) { atomicOr(p.err, bit); }
+
+// Page of row t of sequence b; -1 (and the error bit) when the table names none of the pool.
+__device__ __forceinline__ int page_of(const Params& p, int b, int t) {
+    const int id = p.table[(int64_t)b * p.table_st + (t >> p.page_log2)];
+    if ((unsigned)id < (unsigned)p.num_pages) return id;
+    set_error(p, FCCI_DEV_ERR_PAGE);
+    return -1;
+}
+
+// Smallest e in [kScaleMin, kScaleMax] with amax <= 448 * 2^e: 448 = 1.75 * 2^8, so with
+// amax = m * 2^E it is E - 8, one more when m > 1.75 (mantissa bits above 0x600000).
+__device__ __forceinline__ int scale_exponent(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return max(kScaleMin, min(kScaleMax, e));
+}
+
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Two values to e4m3 codes (round to nearest even, saturating; the first in the low byte).
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
+// Two e4m3 codes to fp16 (exact).
+__device__ __forceinline__ uint32_t half2_of_e4m3x2(uint32_t codes) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)codes));
+    return h;
+}
+
+// cos and sin of pos * freq: the top 32 bits of the wrapped product are the angle in units of
+// 2^-32 turns, taken as a signed fraction of half a turn.
+__device__ __forceinline__ float2 rope_cs(uint64_t turn, int pos) {
+    const int32_t hi = (int32_t)(((uint64_t)(uint32_t)pos * turn) >> 32);
+    float2 cs;
+    sincospif((float)hi * 4.656612873077393e-10f, &cs.y, &cs.x);
+    return cs;
+}
+
+// x1' = x1 cos - x2 sin, x2' = x2 cos + x1 sin
+__device__ __forceinline__ float rotated(float x, float partner, float2 cs, bool first_half) {
+    return first_half ? fmaf(x, cs.x, -(partner * cs.y)) : fmaf(x, cs.x, partner * cs.y);
+}
+
+// The last CTA of the grid moves seq_lens: every CTA has read them by then. Called by all
+// threads at the kernel's end; `flag` is a shared word.
+__device__ __forceinline__ void advance_lengths(const Params& p, int* flag) {
+    if (!p.advance) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        const unsigned total = gridDim.x * gridDim.y * gridDim.z;
+        *flag = atomicAdd(p.done_cnt, 1u) == total - 1;
+    }
+    __syncthreads();
+    if (!*flag) return;
+    __threadfence();
+    for (int b = threadIdx.x; b < p.B; b += blockDim.x) {
+        const Seq s = seq_of(p, b);
+        if (s.ok) p.seq_lens[b] = s.T + (p.append ? s.n : 0);
+    }
+    if (threadIdx.x == 0) atomicExch(p.done_cnt, 0u);
+}
+
+// Workspace: a fixed head (error word, counters that are zero between calls) and per-call
+// regions behind it, so that one workspace serves calls of different shapes.
+constexpr int kMaxGrid = 1024;  // CTAs of the split attention launch, at most
+constexpr size_t kHeadBytes = 256 + kMaxGrid * 4;
+constexpr int kMaxCols = 16;  // query rows of one attention unit
+struct WsLayout {
+    size_t part_lse, part_o, q_rot, total;
+};
+WsLayout ws_layout(int Hq, int Hkv, int D, int total_q, int max_q, int max_kv, int grid);
+
+int launch_append(const Params& p, const Freqs& f, bool e4m3, cudaStream_t st);
+
+}  // namespace pg
+}  // namespace fcci

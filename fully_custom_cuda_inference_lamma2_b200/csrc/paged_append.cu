@@ -1,0 +1,320 @@
+// Append of new keys and values to the paged cache, with the position rotation on the way.
+//
+// What a call must move: k_new, v_new and q in (fp16), q rotated out (fp16), the rows out
+// (fp16, or one byte and a scale per page): it is bound by memory, or by launch and load
+// latency when there are few tokens. Each value is rounded once, from the fp32 rotation.
+//
+// An e4m3 page has one scale 2^e for each kv head. Powers of two make the product with 2^-e
+// exact, and an e that grows later re-rounds only the codes that become subnormal.
+#include <mutex>
+
+#include "paged.cuh"
+
+namespace fcci {
+namespace pg {
+
+constexpr int kTokenThreads = 256;
+
+// One token per sequence. A warp takes one row (a query head, or the key or value of a kv
+// head): few rows in all, so the rows spread over as many warps as there are, and the chain
+// length -> page -> scale is what the time goes into.
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(kTokenThreads) paged_append_token_kernel(const __grid_constant__ Params p,
+                                                                         const __grid_constant__ Freqs f) {
+    constexpr int E = D / 32;  // elements of a row per lane
+    __shared__ int flag;
+    griddep_launch_dependents();
+    griddep_wait();
+    const int b = blockIdx.x;
+    const int lane = threadIdx.x & 31;
+    const int task = blockIdx.y * (kTokenThreads / 32) + (threadIdx.x >> 5);
+    const int nkv = p.append ? 2 * p.Hkv : 0;
+    const Seq s = seq_of(p, b);
+    if (!s.ok) {
+        if (task == 0 && lane == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
+    } else if (task < nkv + (p.q ? p.Hq : 0)) {
+        const bool is_q = task >= nkv, is_v = !is_q && task >= p.Hkv;
+        const int h = is_q ? task - nkv : (is_v ? task - p.Hkv : task);
+        const __half* src = is_q ? p.q + b * p.q_st + h * p.q_sh
+                                 : (is_v ? p.v_new + b * p.vn_st + h * p.vn_sh : p.k_new + b * p.kn_st + h * p.kn_sh);
+        const int d0 = lane * E, half = p.rot >> 1;
+        float x[E];
+        __align__(16) __half raw[E], other[E];
+        auto load = [](__half(&dst)[E], const __half* a) {
+            if constexpr (E == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(a);
+            else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(a);
+            else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(a);
+        };
+        load(raw, src + d0);
+        const bool turn = !is_v && d0 < p.rot, first = d0 < half;
+        if (turn) load(other, src + (first ? d0 + half : d0 - half));
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x[e] = __half2float(raw[e]);
+            if (turn) {
+                const float2 cs = rope_cs(f.turn[(first ? d0 : d0 - half) + e], s.T);
+                x[e] = rotated(x[e], __half2float(other[e]), cs, first);
+            }
+        }
+        auto store16 = [&](__half* dst) {
+#pragma unroll
+            for (int e = 0; e < E; e += 2)
+                *reinterpret_cast<uint32_t*>(dst + d0 + e) = pack_half2(x[e], x[e + 1]);
+        };
+        if (is_q) {
+            store16(p.q_rot + ((int64_t)b * p.Hq + h) * D);
+        } else {
+            const int id = page_of(p, b, s.T);
+            if (id >= 0) {
+                const int off = s.T & (p.page - 1);
+                uint8_t* page = is_v ? p.v_pages + id * p.v_sp + h * p.v_sh : p.k_pages + id * p.k_sp + h * p.k_sh;
+                const int64_t st = is_v ? p.v_st : p.k_st;
+                if constexpr (!E4M3) {
+                    store16(reinterpret_cast<__half*>(page + off * st));
+                } else {
+                    uint8_t* sp = is_v ? p.v_scales + id * p.vs_sp + h * p.vs_sh : p.k_scales + id * p.ks_sp + h * p.ks_sh;
+                    const int had = off ? (int)*sp - 127 : -1000;  // a fresh page has no scale yet
+                    float amax = 0.f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[e]));
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                    int ex = scale_exponent(amax);
+                    if (off && ex > had) {
+                        // the rows before this one take the larger scale (rare: the page's largest value grew past a power of two)
+                        const float down = exp2_int(max(had, -126) - ex);
+                        for (int i = lane; i < off * (D / 4); i += 32) {
+                            uint32_t* w = reinterpret_cast<uint32_t*>(page + (i / (D / 4)) * st + (i % (D / 4)) * 4);
+                            const uint32_t c = *w;
+                            const uint32_t lo = half2_of_e4m3x2(c & 0xffffu), hi = half2_of_e4m3x2(c >> 16);
+                            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+                            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                            *w = e4m3x2(a.x * down, a.y * down) | (e4m3x2(g.x * down, g.y * down) << 16);
+                        }
+                    }
+                    ex = max(ex, had);
+                    const float up = exp2_int(-ex);
+                    if constexpr (E == 2) {
+                        *reinterpret_cast<uint16_t*>(page + off * st + d0) = (uint16_t)e4m3x2(x[0] * up, x[1] * up);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < E; e += 4)
+                            *reinterpret_cast<uint32_t*>(page + off * st + d0 + e) =
+                                e4m3x2(x[e] * up, x[e + 1] * up) | (e4m3x2(x[e + 2] * up, x[e + 3] * up) << 16);
+                    }
+                    if (lane == 0) *sp = (uint8_t)(ex + 127);
+                }
+            }
+        }
+    }
+    advance_lengths(p, &flag);
+}
+
+// Many tokens per sequence. A CTA takes one page's worth of positions of one sequence (page
+// blockIdx.x behind the first page that the call touches) and a share of the heads: it
+// builds the cos/sin table of its positions once in shared memory, and its warps then run over the
+// heads. A warp holds R = 2048 / D rows of one head in registers (64 values a lane, as 4
+// rows of two 8-element chunks, a chunk of the first half and the one it is rotated with),
+// so a page is 1 to 8 warps, which agree on the largest value through shared memory
+// before they round.
+constexpr int kRowsThreads = 256;
+
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(const __grid_constant__ Params p,
+                                                                         const __grid_constant__ Freqs f) {
+    constexpr int R = 2048 / D;      // rows per warp
+    constexpr int PL = D / 16;       // lanes per row
+    constexpr int RP = 32 / PL;      // rows per pass
+    constexpr int kWarps = kRowsThreads / 32;
+    extern __shared__ float2 cs_table[];  // [page][rot / 2]
+    __shared__ int flag;
+    __shared__ float amax_sm[2][kWarps];
+    griddep_launch_dependents();
+    griddep_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int b = blockIdx.y;
+    const Seq s = seq_of(p, b);
+    const int pj = (s.T >> p.page_log2) + blockIdx.x;
+    const int p0 = pj << p.page_log2;  // first position of the page
+    if (!s.ok) {
+        if (blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
+    } else if (s.n > 0 && p0 < s.T + s.n) {
+        const int half = p.rot >> 1;
+        for (int i = tid; i < p.page * half; i += kRowsThreads) {
+            const int r = i / half, k = i - r * half;
+            if (p0 + r >= s.T && p0 + r < s.T + s.n) cs_table[i] = rope_cs(f.turn[k], p0 + r);
+        }
+        const int id = page_of(p, b, p0);
+        __syncthreads();
+        const int W = max(1, p.page / R);      // warps of one page
+        const int groups = kWarps / W;         // heads in flight
+        const int grp = warp / W, part = warp % W;
+        const int row0 = part * R + lane / PL;  // row of pass 0; pass i: + i * RP
+        const int j = lane % PL;
+        // chunk pair j: two 8-element chunks rotated with one another, then the plain ones
+        const bool turn_j = j < (p.rot >> 4);
+        const int dlo = turn_j ? 8 * j : p.rot + 16 * (j - (p.rot >> 4));
+        const int dhi = turn_j ? dlo + half : dlo + 8;
+        const int heads = (p.q ? p.Hq : 0) + 2 * p.Hkv;
+        const int per = (heads + gridDim.z - 1) / gridDim.z;
+        const int h_end = min(heads, (int)(blockIdx.z + 1) * per);
+        int buf = 0;
+        for (int hb = blockIdx.z * per; hb < h_end; hb += groups, buf ^= 1) {
+            const int item = hb + grp;
+            const bool live = item < h_end;
+            const bool is_k = item < p.Hkv, is_v = !is_k && item < 2 * p.Hkv, is_q = !is_k && !is_v;
+            const int h = is_k ? item : (is_v ? item - p.Hkv : item - 2 * p.Hkv);
+            const __half* src = is_q ? p.q + h * p.q_sh : (is_v ? p.v_new + h * p.vn_sh : p.k_new + h * p.kn_sh);
+            const int64_t sst = is_q ? p.q_st : (is_v ? p.vn_st : p.kn_st);
+            uint8_t* page = nullptr;
+            uint8_t* sp = nullptr;
+            const int64_t st = is_v ? p.v_st : p.k_st;
+            if (live && !is_q && id >= 0) {
+                page = is_v ? p.v_pages + id * p.v_sp + h * p.v_sh : p.k_pages + id * p.k_sp + h * p.k_sh;
+                if constexpr (E4M3)
+                    sp = is_v ? p.v_scales + id * p.vs_sp + h * p.vs_sh : p.k_scales + id * p.ks_sp + h * p.ks_sh;
+            }
+            const bool work = live && (is_q || page);
+            float x[4][16];
+            float amax = 0.f;
+            uint4 lo[4], hi[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int pos = p0 + row0 + i * RP;
+                lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
+                if (work && row0 + i * RP < p.page && pos >= s.T && pos < s.T + s.n) {
+                    const __half* a = src + (int64_t)(s.tok0 + pos - s.T) * sst;
+                    lo[i] = *reinterpret_cast<const uint4*>(a + dlo);
+                    hi[i] = *reinterpret_cast<const uint4*>(a + dhi);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __half* a = reinterpret_cast<const __half*>(&lo[i]);
+                const __half* c = reinterpret_cast<const __half*>(&hi[i]);
+                const int r = row0 + i * RP, pos = p0 + r;
+                const bool fresh = r < p.page && pos >= s.T && pos < s.T + s.n;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float u = __half2float(a[e]), w = __half2float(c[e]);
+                    if (turn_j && !is_v && fresh) {
+                        const float2 cs = cs_table[r * half + dlo + e];
+                        const float t = rotated(u, w, cs, true);
+                        w = rotated(w, u, cs, false);
+                        u = t;
+                    }
+                    x[i][e] = u;
+                    x[i][8 + e] = w;
+                    amax = fmaxf(amax, fmaxf(fabsf(u), fabsf(w)));
+                }
+            }
+            auto store16 = [&](__half* row, int i) {
+                uint4 u, w;
+                u.x = pack_half2(x[i][0], x[i][1]), u.y = pack_half2(x[i][2], x[i][3]);
+                u.z = pack_half2(x[i][4], x[i][5]), u.w = pack_half2(x[i][6], x[i][7]);
+                w.x = pack_half2(x[i][8], x[i][9]), w.y = pack_half2(x[i][10], x[i][11]);
+                w.z = pack_half2(x[i][12], x[i][13]), w.w = pack_half2(x[i][14], x[i][15]);
+                *reinterpret_cast<uint4*>(row + dlo) = u;
+                *reinterpret_cast<uint4*>(row + dhi) = w;
+            };
+            if constexpr (E4M3) {
+#pragma unroll
+                for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                // old rows of the call's first page keep (or grow) the page's scale
+                const bool old = p0 < s.T;
+                const int had = old && sp ? (int)*sp - 127 : -1000;
+                if (W > 1) {
+                    // every warp of the page has read the old scale before this barrier;
+                    // two buffers: a warp may be one head ahead of another's reads
+                    if (lane == 0) amax_sm[buf][warp] = amax;
+                    __syncthreads();
+                    for (int w = 0; w < W; ++w) amax = fmaxf(amax, amax_sm[buf][grp * W + w]);
+                }
+                if (work && !is_q) {
+                    int ex = scale_exponent(amax);
+                    const bool grows = old && ex > had;
+                    ex = max(ex, had);
+                    const float up = exp2_int(-ex), down = grows ? exp2_int(max(had, -126) - ex) : 1.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = row0 + i * RP, pos = p0 + r;
+                        if (r >= p.page || pos >= s.T + s.n) continue;
+                        uint8_t* row = page + r * st;
+                        if (pos >= s.T) {
+                            uint2 u, w;
+                            u.x = e4m3x2(x[i][0] * up, x[i][1] * up) | (e4m3x2(x[i][2] * up, x[i][3] * up) << 16);
+                            u.y = e4m3x2(x[i][4] * up, x[i][5] * up) | (e4m3x2(x[i][6] * up, x[i][7] * up) << 16);
+                            w.x = e4m3x2(x[i][8] * up, x[i][9] * up) | (e4m3x2(x[i][10] * up, x[i][11] * up) << 16);
+                            w.y = e4m3x2(x[i][12] * up, x[i][13] * up) | (e4m3x2(x[i][14] * up, x[i][15] * up) << 16);
+                            *reinterpret_cast<uint2*>(row + dlo) = u;
+                            *reinterpret_cast<uint2*>(row + dhi) = w;
+                        } else if (grows) {
+                            for (int k = 0; k < 4; ++k) {
+                                uint32_t* w = reinterpret_cast<uint32_t*>(row + (k < 2 ? dlo : dhi) + (k & 1) * 4);
+                                const uint32_t c = *w;
+                                const uint32_t c0 = half2_of_e4m3x2(c & 0xffffu), c1 = half2_of_e4m3x2(c >> 16);
+                                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&c0));
+                                const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&c1));
+                                *w = e4m3x2(a.x * down, a.y * down) | (e4m3x2(g.x * down, g.y * down) << 16);
+                            }
+                        }
+                    }
+                    if (part == 0 && lane == 0) *sp = (uint8_t)(ex + 127);
+                }
+            }
+            if (work && (is_q || !E4M3)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = row0 + i * RP, pos = p0 + r;
+                    if (r >= p.page || pos < s.T || pos >= s.T + s.n) continue;
+                    __half* row = is_q ? p.q_rot + ((int64_t)(s.tok0 + pos - s.T) * p.Hq + h) * D
+                                       : reinterpret_cast<__half*>(page + r * st);
+                    store16(row, i);
+                }
+            }
+        }
+    }
+    advance_lengths(p, &flag);
+}
+
+template <int D, bool E4M3>
+static int launch_append_t(const Params& p, const Freqs& f, cudaStream_t st) {
+    const int heads = (p.q ? p.Hq : 0) + (p.append ? 2 * p.Hkv : 0);
+    if (!p.cu_q) {
+        const int per = kTokenThreads / 32;
+        return launch_pdl(paged_append_token_kernel<D, E4M3>, dim3(p.B, (heads + per - 1) / per), dim3(kTokenThreads), 0,
+                          st, p, f);
+    }
+    // pages that the longest run of new tokens can touch, and a head split that fills the GPU
+    // when there are few pages
+    const int64_t slots = ((int64_t)p.max_q + p.page - 2) / p.page + 1;
+    const int64_t pages = (int64_t)p.total_q / p.page + p.B;
+    int64_t z = (8 * 148 + pages - 1) / pages;
+    const int64_t most = (heads + 7) / 8;
+    if (z > most) z = most;
+    if (z < 1) z = 1;
+    const size_t smem = (size_t)p.page * (p.rot / 2) * sizeof(float2);
+    static std::once_flag once[128];
+    static cudaError_t attr[128];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return set_cuda_status(cudaGetLastError());
+    std::call_once(once[dev], [&]() {
+        attr[dev] = cudaFuncSetAttribute(paged_append_rows_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         64 * 1024);
+    });
+    if (attr[dev] != cudaSuccess) return set_cuda_status(attr[dev]);
+    return launch_pdl(paged_append_rows_kernel<D, E4M3>, dim3((unsigned)slots, p.B, (unsigned)z), dim3(kRowsThreads), smem,
+                      st, p, f);
+}
+
+int launch_append(const Params& p, const Freqs& f, bool e4m3, cudaStream_t st) {
+    switch (p.D) {
+        case 64: return e4m3 ? launch_append_t<64, true>(p, f, st) : launch_append_t<64, false>(p, f, st);
+        case 128: return e4m3 ? launch_append_t<128, true>(p, f, st) : launch_append_t<128, false>(p, f, st);
+        case 256: return e4m3 ? launch_append_t<256, true>(p, f, st) : launch_append_t<256, false>(p, f, st);
+        default: return set_status(FCCI_EUNSUPPORTED, "paged append: unsupported head_dim");
+    }
+}
+
+}  // namespace pg
+}  // namespace fcci
