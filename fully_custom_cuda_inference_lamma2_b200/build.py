@@ -28,7 +28,7 @@ GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 LIB = os.path.join(PKG, "libfcci_decode.so")
 LIB_SOURCES = ["decode_attn.cu", "capi.cu", "compat.cu", "noalloc.cu", "prefill_attn.cu", "gemv.cu", "step.cu", "exchange.cu",
-               "paged_append.cu", "paged_attn.cu"]
+               "paged_append.cu", "paged_split.cu", "paged_step.cu"]
 LIB_HEADERS = ["ptx.cuh", "tcgen05.cuh", "fcci_internal.h", "paged.cuh"]
 MODULES = {
     "attn_varlen": "attn_varlen_module.cpp",

@@ -1087,17 +1087,17 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// fp16 tensor map with 128-byte swizzle. dims[0] is the contiguous dimension;
-// stride_bytes[i] is the byte stride of dims[i + 1]. A stride of an extent-1
+// Tensor map of fp16 (or, with `bytes`, 8-bit) elements, swizzled over 128 bytes (64 with `sw64`). dims[0] is the
+// contiguous dimension; stride_bytes[i] is the byte stride of dims[i + 1]. A stride of an extent-1
 // dimension is never used by a load; it is replaced by the packed value so the
 // encoder's alignment checks pass.
-int encode_f16_sw128(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const int64_t* stride_bytes,
-                     const uint32_t* box) {
+int encode_tiled(CUtensorMap* map, bool bytes, bool sw64, const void* base, int rank, const uint64_t* dims,
+                 const int64_t* stride_bytes, const uint32_t* box) {
     auto fn = encode_fn();
     if (!fn || rank < 1 || rank > 5) return FCCI_ETMAP;
     cuuint64_t d[5], st[4];
     cuuint32_t bx[5], estr[5];
-    int64_t prev = 2;  // bytes per element: the stride of dimension 0
+    int64_t prev = bytes ? 1 : 2;  // bytes per element: the stride of dimension 0
     for (int i = 0; i < rank; ++i) {
         d[i] = (cuuint64_t)dims[i];
         bx[i] = box[i];
@@ -1109,10 +1109,16 @@ int encode_f16_sw128(CUtensorMap* map, const void* base, int rank, const uint64_
             prev = sb;
         }
     }
-    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), d, st, bx, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    CUresult r = fn(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                    const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    sw64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? FCCI_OK : FCCI_ETMAP;
+}
+
+int encode_f16_sw128(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const int64_t* stride_bytes,
+                     const uint32_t* box) {
+    return encode_tiled(map, false, false, base, rank, dims, stride_bytes, box);
 }
 
 // 4-D map (head_dim, token, kv head, sequence) over an fp16 arena; 64-column boxes of

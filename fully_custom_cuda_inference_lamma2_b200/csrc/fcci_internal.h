@@ -32,6 +32,9 @@ int max_grid(int dev);
 int device_sm_count(int dev);
 
 int set_status(int code, const char* msg);
+// TMA descriptor of fp16 or 8-bit elements with 128- or 64-byte swizzle (dims[0] contiguous, byte strides of dims[1..]).
+int encode_tiled(CUtensorMap* map, bool bytes, bool sw64, const void* base, int rank, const uint64_t* dims,
+                 const int64_t* stride_bytes, const uint32_t* box);
 // fp16 TMA descriptor with 128-byte swizzle (dims[0] contiguous, byte strides of dims[1..]).
 int encode_f16_sw128(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const int64_t* stride_bytes,
                      const uint32_t* box);

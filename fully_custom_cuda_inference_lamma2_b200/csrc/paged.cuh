@@ -102,13 +102,18 @@ __device__ __forceinline__ uint32_t half2_of_e4m3x2(uint32_t codes) {
     return h;
 }
 
-// cos and sin of pos * freq: the top 32 bits of the wrapped product are the angle in units of
-// 2^-32 turns, taken as a signed fraction of half a turn.
+// cos and sin of pos * freq. The top 32 bits of the wrapped product are the angle in units of
+// 2^-32 turns; the nearest quarter turn is taken off as an integer, so what is rounded to fp32 is at
+// most an eighth of a turn (angle off by 2^-25 at most), and put back as a swap and signs.
 __device__ __forceinline__ float2 rope_cs(uint64_t turn, int pos) {
-    const int32_t hi = (int32_t)(((uint64_t)(uint32_t)pos * turn) >> 32);
-    float2 cs;
-    sincospif((float)hi * 4.656612873077393e-10f, &cs.y, &cs.x);
-    return cs;
+    const uint32_t a = (uint32_t)(((uint64_t)(uint32_t)pos * turn) >> 32);
+    const uint32_t quarter = (a + 0x20000000u) >> 30;
+    float s, c;
+    sincospif((float)(int32_t)(a - (quarter << 30)) * 4.656612873077393e-10f, &s, &c);
+    const bool odd = quarter & 1;
+    const float x = odd ? s : c, y = odd ? c : s;
+    // quarter 0: (c, s), 1: (-s, c), 2: (-c, -s), 3: (s, -c)
+    return make_float2(((quarter + 1) & 2) ? -x : x, (quarter & 2) ? -y : y);
 }
 
 // x1' = x1 cos - x2 sin, x2' = x2 cos + x1 sin
@@ -147,6 +152,8 @@ struct WsLayout {
 WsLayout ws_layout(int Hq, int Hkv, int D, int total_q, int max_q, int max_kv, int grid);
 
 int launch_append(const Params& p, const Freqs& f, bool e4m3, cudaStream_t st);
+// Split-KV attention; `fused`: the launch appends the one new row of each sequence itself.
+int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, uint8_t* ws, const WsLayout& L, cudaStream_t st);
 
 }  // namespace pg
 }  // namespace fcci

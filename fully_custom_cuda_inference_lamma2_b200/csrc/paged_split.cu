@@ -1,0 +1,856 @@
+// Split-KV attention over the paged cache: one new token per sequence (decode, with its append
+// fused in), or a few of them (a short chunk whose rows an append has written already).
+//
+// Work. A unit is (sequence b, kv head h, column group c): up to 8 * NB query rows of the group,
+// rows being (token, query head) pairs, so a cached key is read once for all of them. A unit's
+// keys are cut into tiles of KEYS rows; all tiles of all units form one line, of which every CTA of a
+// persistent grid takes an equal stretch, whatever the lengths are. A unit that lies in one
+// stretch is finished there; of a cut one, every CTA leaves its part (o, log-sum-exp) in the
+// workspace and the last to arrive joins them. No CTA waits for another.
+//
+// Inside a CTA warp 4 fetches and warps 0..3 compute. A stage holds the K and the V tile, in
+// rows of 128 bytes (64 for e4m3 with head_dim 64) in the tensor-map swizzle; the pages of a tile
+// are fetched side by side, one lane and one box each, the page that ends a sequence in boxes
+// of 16 rows. The page table is read one tile ahead and the scales arrive behind the tile
+// that they belong to, so neither latency is on the path. Warp w owns keys [16 MT w, 16 MT (w+1)):
+//   S^T = K Q^T      A = 16 keys, B = 8 query rows (mma m16n8k16, fp32 sums)
+//   O^T += V^T P^T   A = 16 dims, B = P^T by movmatrix
+// e4m3 codes become fp16 in registers, exactly, and the power-of-two scales go onto S and onto
+// the product of each 16 keys, in fp32, so no scale can leave fp16's range. The queries are
+// rotated here in fp32 and split in two fp16 parts (hi + lo): one rounding of them to fp16 would
+// be the largest error of the whole step. P is rounded to fp16 (relative 2^-11, weights in [0, 1]).
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <mutex>
+
+#include "paged.cuh"
+
+namespace fcci {
+namespace pg {
+
+constexpr int kConsumerWarps = 4, kConsumers = kConsumerWarps * 32, kThreads = kConsumers + 32;
+constexpr int kMaxStages = 6;
+constexpr uint64_t kWaitLimitNs = 4000000000ull;  // 4 s: far beyond any healthy wait
+constexpr uint64_t kDrainLimitNs = 500000000ull;
+constexpr int kBar = 1;
+
+struct SplitParams {
+    Params p;
+    int32_t fused;   // the kernel appends row T itself (decode)
+    int32_t stages;
+    float* part_lse;  // [2 * grid][kMaxCols]
+    float* part_o;    // [2 * grid][kMaxCols][D]
+    uint32_t* cut_cnt;  // [grid], zero between calls
+};
+
+template <int D, int NB, bool E4M3>
+struct Cfg {
+    static constexpr int ROWB = E4M3 ? D : 2 * D;             // bytes of a row
+    // keys of a tile; an e4m3 page always lies in one tile (page * D <= 16384), because an append
+    // that grows its scale rewrites the page's rows where the tile holds them
+    static constexpr int KEYS = ROWB <= 128 && (E4M3 || NB == 1) ? 128 : 64;
+    static constexpr int MT = KEYS / 64;                      // 16-key groups of a warp
+    static constexpr int PITCH = ROWB < 128 ? ROWB : 128;     // bytes of a row in one block
+    static constexpr int BLOCKS = ROWB / PITCH;               // blocks side by side
+    static constexpr int TILE = KEYS * ROWB;
+    static constexpr int COLS = 8 * NB;
+    static constexpr int RP = D + 4;                          // fp32 pitch of the joining rows
+    static constexpr int QP = D + 16;                         // fp16 pitch of the query rows
+    // query fragments in registers where they fit beside two CTAs' accumulators, else in shared memory
+    static constexpr bool QREG = NB == 1 && D <= 128;
+    static constexpr int RED = 2 * COLS * RP * 4;             // bytes; with QREG the query rows pass through it
+    static constexpr int QB = QREG ? 0 : 2 * COLS * QP * 2;   // bytes of their own buffer
+    static_assert(!QREG || 2 * COLS * QP * 2 <= RED, "queries in the joining buffer");
+    static size_t smem(int stages, int B, int rope_rows, int rot) {
+        return 1024 + (size_t)stages * 2 * TILE + RED + QB + (size_t)rope_rows * (rot / 2) * 8 + 2 * kConsumerWarps * COLS * 4 +
+               kMaxStages * (2 * 8 * 4 + 16) + 64 + (size_t)(3 * B + 2) * 4;
+    }
+};
+
+struct Line {  // a place on the line of tiles
+    int b, h, c, j;     // sequence, kv head, column group, tile
+    int tiles, groups;  // of sequence b
+};
+
+template <int D, int NB, bool E4M3>
+__global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_constant__ CUtensorMap mk,
+                                                            const __grid_constant__ CUtensorMap mv,
+                                                            const __grid_constant__ CUtensorMap mk16,
+                                                            const __grid_constant__ CUtensorMap mv16,
+                                                            const __grid_constant__ SplitParams sp,
+                                                            const __grid_constant__ Freqs f) {
+    using C = Cfg<D, NB, E4M3>;
+    constexpr int KEYS = C::KEYS, MT = C::MT, PITCH = C::PITCH, COLS = C::COLS, RP = C::RP, QP = C::QP;
+    constexpr int KSTEPS = D / 16, CHUNKS = PITCH / 16;
+    const Params& p = sp.p;
+    extern __shared__ uint8_t raw[];
+    uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const int S = sp.stages, B = p.B, Hkv = p.Hkv, G = p.G;
+    uint8_t* tiles_sm = sm;
+    float* red = reinterpret_cast<float*>(sm + (size_t)S * 2 * C::TILE);
+    __half* q_hi = reinterpret_cast<__half*>(C::QREG ? red : red + C::RED / 4);
+    __half* q_lo = q_hi + COLS * QP;
+    float* red_ml = red + (C::RED + C::QB) / 4;              // [4 warps][COLS][2]
+    uint64_t* full = reinterpret_cast<uint64_t*>(red_ml + 2 * kConsumerWarps * COLS);
+    uint64_t* empty = full + kMaxStages;
+    float* scale_sm = reinterpret_cast<float*>(empty + kMaxStages);  // [stage][K, V][8 page boxes]; K -1: no such page
+    int* misc = reinterpret_cast<int*>(scale_sm + kMaxStages * 16);
+    volatile int* abort_flag = misc;
+    int* base = misc + 16;  // [B + 1] tiles before sequence b
+    int* seqT = base + B + 1;
+    int* seqN = seqT + B;
+    float2* cs = reinterpret_cast<float2*>(seqN + B + ((B + 1) & 1));
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&full[s], 2);  // the fetched bytes, and the scales
+            mbar_init(&empty[s], kConsumerWarps);
+        }
+        misc[0] = 0;
+        fence_mbar_init();
+    }
+    if (tid == kConsumers) {
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
+        prefetch_tmap(&mk16);
+        prefetch_tmap(&mv16);
+    }
+    griddep_launch_dependents();
+    griddep_wait();
+
+    // ---- the line of tiles: lengths and the prefix of the tile counts
+    auto keys_of = [&](int T, int n) { return T + (sp.fused || p.cu_q ? n : 0); };
+    auto groups_of = [&](int n) { return (n * G + COLS - 1) / COLS; };
+    auto tiles_of = [&](int T, int n) { return max(1, (keys_of(T, n) + KEYS - 1) / KEYS); };
+    bool uniform = true;
+    {
+        const int chunk = (B + kThreads - 1) / kThreads, lo = tid * chunk, hi = min(B, lo + chunk);
+        int local = 0, first = -1;
+        for (int b = lo; b < hi; ++b) {
+            const Seq s = seq_of(p, b);
+            if (!s.ok && blockIdx.x == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
+            // a sequence that is not served: its one row gets zeros in decode, none are touched otherwise
+            const int T = s.ok ? s.T : 0, n = s.ok ? s.n : (p.cu_q ? 0 : 1);
+            seqT[b] = s.ok ? s.T : -1;
+            seqN[b] = n;
+            const int cnt = (s.ok ? tiles_of(T, n) : 1) * Hkv * groups_of(n);
+            base[b + 1] = cnt;
+            local += cnt;
+            if (first < 0) first = cnt;
+            if (cnt != first) uniform = false;
+        }
+        int incl = local;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        int* scratch = reinterpret_cast<int*>(red_ml);
+        if (lane == 31) scratch[warp] = incl;
+        if (tid == 0) base[0] = 0, scratch[8] = first;
+        __syncthreads();
+        if (first >= 0 && first != scratch[8]) uniform = false;
+        int run = incl - local;
+        for (int w = 0; w < warp; ++w) run += scratch[w];
+        for (int b = lo; b < hi; ++b) base[b + 1] = run += base[b + 1];
+        uniform = __syncthreads_and(uniform) != 0;
+    }
+    // ---- this CTA's stretch
+    const long long N = base[B];
+    long long CT = N < (long long)gridDim.x ? N : (long long)gridDim.x;
+    if (uniform && N > 0) {
+        // equal units: a number of CTAs that is a multiple of the units keeps every cut at the same
+        // places of each, unless that leaves more than 15 % of the grid idle
+        const long long units = (long long)B * Hkv * groups_of(seqN[0]);
+        if (units <= (long long)gridDim.x) {
+            const long long k = min((long long)gridDim.x / units, N / units);
+            if (20 * units * k >= 17 * CT) CT = units * k;
+        }
+    }
+    long long t0 = 0, t1 = 0;
+    if ((long long)blockIdx.x < CT) {
+        t0 = (long long)blockIdx.x * N / CT;
+        t1 = ((long long)blockIdx.x + 1) * N / CT;
+    }
+    const int ntiles = (int)(t1 - t0);
+    auto enter = [&](Line& x) {
+        x.groups = groups_of(seqN[x.b]);
+        x.tiles = seqT[x.b] < 0 ? 1 : tiles_of(seqT[x.b], seqN[x.b]);
+    };
+    Line at = {0, 0, 0, 0, 1, 1};
+    if (ntiles > 0) {
+        int lo = 0, hi = B - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (base[mid] <= t0) lo = mid;
+            else hi = mid - 1;
+        }
+        at.b = lo;
+        enter(at);
+        int rem = (int)(t0 - base[lo]);
+        at.j = rem % at.tiles;
+        rem /= at.tiles;
+        at.c = rem % at.groups;
+        at.h = rem / at.groups;
+    }
+    auto step = [&](Line& x) {
+        if (++x.j < x.tiles) return;
+        x.j = 0;
+        if (++x.c < x.groups) return;
+        x.c = 0;
+        if (++x.h < Hkv) return;
+        x.h = 0;
+        do ++x.b;
+        while (x.b < B && base[x.b + 1] == base[x.b]);
+        if (x.b < B) enter(x);
+    };
+    auto keys_at = [&](const Line& x) { return seqT[x.b] < 0 ? 0 : keys_of(seqT[x.b], seqN[x.b]); };
+
+    const int box = min(p.page, KEYS);  // rows of one page in a tile
+    const int boxes = KEYS / box;
+    if (warp == kConsumerWarps) {
+        // ============================================================ fetching warp
+        const uint64_t pol = l2_policy_evict_first();
+        const bool is_v = lane >= 16;
+        const int slot = lane & 15;  // page box of this lane, of K (lanes 0..) or V (lanes 16..)
+        auto rows_at = [&](const Line& x) {
+            return slot < boxes ? max(0, min(box, keys_at(x) - x.j * KEYS - slot * box)) : 0;
+        };
+        auto page_at = [&](const Line& x) {
+            if (rows_at(x) == 0) return -1;
+            return p.table[(int64_t)x.b * p.table_st + ((x.j * KEYS + slot * box) >> p.page_log2)];
+        };
+        int pid = ntiles > 0 ? page_at(at) : -1;
+        float sc = 0.f;
+        int it = 0;
+        auto publish = [&](int i, float v) {  // scales of tile i, then its second arrival
+            if (slot < boxes) scale_sm[(i % S) * 16 + (is_v ? 8 : 0) + slot] = v;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[i % S]);
+        };
+        for (; it < ntiles; ++it) {
+            const int s = it % S;
+            const int rows = rows_at(at), h = at.h;
+            const int row0 = (at.j * KEYS + slot * box) & (p.page - 1);
+            const bool there = rows > 0 && (unsigned)pid < (unsigned)p.num_pages;
+            if (rows > 0 && !there) set_error(p, FCCI_DEV_ERR_PAGE);
+            const int id = there ? pid : 0;
+            step(at);
+            const int pid_next = it + 1 < ntiles ? page_at(at) : -1;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ((uint32_t)(it / S) & 1u) ^ 1u, abort_flag, kWaitLimitNs))) {
+                if (lane == 0) {
+                    *abort_flag = 1;
+                    set_error(p, FCCI_DEV_ERR_TIMEOUT);
+                }
+                break;
+            }
+            const int fetched = !there ? 0 : rows == box ? box : (rows + 15) & ~15;
+            const uint32_t bytes = __reduce_add_sync(0xffffffffu, (unsigned)(fetched * C::ROWB));
+            if (lane == 0) mbar_arrive_expect_tx(&full[s], bytes);
+            __syncwarp();
+            if (there) {
+                uint8_t* dst = tiles_sm + (size_t)s * 2 * C::TILE + (is_v ? C::TILE : 0) + slot * box * PITCH;
+                const CUtensorMap* m = is_v ? &mv : &mk;
+                const CUtensorMap* m16 = is_v ? &mv16 : &mk16;
+#pragma unroll
+                for (int k = 0; k < C::BLOCKS; ++k) {
+                    const int col = k * PITCH / (E4M3 ? 1 : 2);
+                    if (rows == box) {
+                        tma_load_4d(dst + k * KEYS * PITCH, m, col, row0, h, id, &full[s], pol);
+                    } else {
+                        for (int r = 0; r < fetched; r += 16)
+                            tma_load_4d(dst + k * KEYS * PITCH + r * PITCH, m16, col, row0 + r, h, id, &full[s], pol);
+                    }
+                }
+            }
+            float next = there ? 1.f : -1.f;
+            if (E4M3 && there) {
+                const uint8_t* a = is_v ? p.v_scales + id * p.vs_sp + h * p.vs_sh : p.k_scales + id * p.ks_sp + h * p.ks_sh;
+                next = exp2_int((int)*a - 127);
+            }
+            if (it > 0) publish(it - 1, sc);
+            sc = next;
+            pid = pid_next;
+        }
+        if (it > 0) publish(it - 1, sc);
+        if (*abort_flag) {
+            // let copies still in flight land before the CTA can exit
+            volatile int never = 0;
+            for (int i = max(0, it - S); i < it; ++i)
+                mbar_wait_bounded(&full[i % S], (uint32_t)(i / S) & 1u, &never, kDrainLimitNs);
+        }
+    } else {
+        // ============================================================ computing warps
+        const int w = warp, g = lane >> 2, t4 = lane & 3;
+        const int rot = p.rot, half = rot >> 1;
+        float m[NB][2], l[NB][2];
+        float2 acc[NB][KSTEPS][2];
+        uint32_t qreg[2][NB][C::QREG ? KSTEPS : 1][2] = {};  // hi, lo
+        int lim[NB][2];
+        int cs_b = -1, cs_c = -1;
+        bool fresh = true;
+        int first_tile = at.j;
+        // address of 16-byte chunk ch of row r in a K or V tile
+        auto cell = [&](uint32_t tile, int r, int ch) {
+            const int blk = ch / CHUNKS, c = ch % CHUNKS;
+            const int sw = PITCH == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
+            return tile + blk * KEYS * PITCH + r * PITCH + sw * 16;
+        };
+
+        // B fragment of k step kk: e4m3 lanes hold 4 neighbouring dims of a chunk, and k follows them
+        auto q_fragment = [&](int part, int nb, int kk, uint32_t(&r)[2]) {
+            const __half* q = (part ? q_lo : q_hi) + (nb * 8 + g) * QP + 16 * kk + (E4M3 ? 4 * t4 : 2 * t4);
+            if constexpr (E4M3) {
+                const uint2 v = *reinterpret_cast<const uint2*>(q);
+                r[0] = v.x, r[1] = v.y;
+            } else {
+                r[0] = *reinterpret_cast<const uint32_t*>(q);
+                r[1] = *reinterpret_cast<const uint32_t*>(q + 8);
+            }
+        };
+
+        auto q_of = [&](int part, int nb, int kk, uint32_t(&r)[2]) {
+            if constexpr (C::QREG) r[0] = qreg[part][nb][kk][0], r[1] = qreg[part][nb][kk][1];
+            else q_fragment(part, nb, kk, r);
+        };
+
+        for (int it = 0; it < ntiles; ++it) {
+            const int T = seqT[at.b], n = seqN[at.b], L = keys_at(at);
+            const int r0 = at.c * COLS, rows = min(COLS, n * G - r0);  // query rows of this unit
+            if (fresh) {
+                fresh = false;
+                first_tile = at.j;
+                const int i0 = r0 / G;  // first token of the unit
+                if (rot > 0 && (cs_b != at.b || cs_c != at.c)) {
+                    const int ntok = (r0 + rows - 1) / G - i0 + 1;
+                    for (int x = tid; x < ntok * half; x += kConsumers)
+                        cs[x] = rope_cs(f.turn[x % half], max(T, 0) + i0 + x / half);
+                    cs_b = at.b, cs_c = at.c;
+                    named_bar_sync(kBar, kConsumers);
+                }
+                // rotated queries, fp32, as hi + lo
+                const int64_t tok0 = p.cu_q ? p.cu_q[at.b] : at.b;
+#pragma unroll 4
+                for (int e = tid * 2; e < COLS * D; e += 2 * kConsumers) {
+                    const int c = e / D, d = e - c * D;
+                    float x0 = 0.f, x1 = 0.f;
+                    if (c < rows) {
+                        const int i = (r0 + c) / G, hq = at.h * G + (r0 + c) - i * G;
+                        const __half* q = p.q + (tok0 + i) * p.q_st + hq * p.q_sh;
+                        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(q + d));
+                        x0 = x.x, x1 = x.y;
+                        if (d < rot) {
+                            const bool lowhalf = d < half;
+                            const int k = lowhalf ? d : d - half;
+                            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(q + (lowhalf ? d + half : k)));
+                            x0 = rotated(x0, y.x, cs[(i - i0) * half + k], lowhalf);
+                            x1 = rotated(x1, y.y, cs[(i - i0) * half + k + 1], lowhalf);
+                        }
+                        if (p.q_rot && at.j == 0)
+                            *reinterpret_cast<uint32_t*>(p.q_rot + ((tok0 + i) * p.Hq + hq) * D + d) = pack_half2(x0, x1);
+                    }
+                    const __half2 hi = __floats2half2_rn(x0, x1);
+                    const float2 back = __half22float2(hi);
+                    *reinterpret_cast<__half2*>(q_hi + c * QP + d) = hi;
+                    *reinterpret_cast<__half2*>(q_lo + c * QP + d) = __floats2half2_rn(x0 - back.x, x1 - back.y);
+                }
+                named_bar_sync(kBar, kConsumers);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int kk = 0; kk < KSTEPS; ++kk) {
+                        if constexpr (C::QREG) {
+                            q_fragment(0, nb, kk, qreg[0][nb][kk]);
+                            q_fragment(1, nb, kk, qreg[1][nb][kk]);
+                        }
+                        acc[nb][kk][0] = acc[nb][kk][1] = make_float2(0.f, 0.f);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        m[nb][c] = -INFINITY;
+                        l[nb][c] = 0.f;
+                        const int col = nb * 8 + 2 * t4 + c;
+                        // keys a row sees: all of them, or up to its own position
+                        lim[nb][c] = col >= rows ? 0 : p.cu_q ? T + (r0 + col) / G + 1 : L;
+                    }
+                }
+                // the query rows may lie in the joining buffer, which a faster warp writes next
+                if (C::QREG) named_bar_sync(kBar, kConsumers);
+            }
+
+            const int s = it % S;
+            const bool ready =
+                __all_sync(0xffffffffu, mbar_wait_bounded(&full[s], (uint32_t)(it / S) & 1u, abort_flag, kWaitLimitNs));
+            if (!ready && !*abort_flag) {
+                *abort_flag = 1;
+                set_error(p, FCCI_DEV_ERR_TIMEOUT);
+            }
+            const uint32_t kt = smem_u32(tiles_sm + (size_t)s * 2 * C::TILE), vt = kt + C::TILE;
+            float* ksc = scale_sm + s * 16;
+            bool wrote = false;
+            if (sp.fused && T >= 0 && T / KEYS == at.j) {
+                // ---- append: warp 0 the key, warp 1 the value, into the tile and the page
+                named_bar_sync(kBar, kConsumers);
+                if (ready && w < 2 && ksc[(T % KEYS) / box] >= 0.f) {
+                    constexpr int E = D / 32;
+                    const bool is_v = w == 1;
+                    const int d0 = lane * E, r = T % KEYS, off = T & (p.page - 1);
+                    const __half* src = is_v ? p.v_new + at.b * p.vn_st + at.h * p.vn_sh : p.k_new + at.b * p.kn_st + at.h * p.kn_sh;
+                    float x[E];
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        x[e] = __half2float(src[d0 + e]);
+                        if (!is_v && d0 < rot) {
+                            const bool lowhalf = d0 < half;
+                            const int k = (lowhalf ? d0 : d0 - half) + e;
+                            x[e] = rotated(x[e], __half2float(src[lowhalf ? k + half : k]), cs[k], lowhalf);
+                        }
+                    }
+                    const int id = p.table[(int64_t)at.b * p.table_st + (T >> p.page_log2)];
+                    uint8_t* page = is_v ? p.v_pages + id * p.v_sp + at.h * p.v_sh : p.k_pages + id * p.k_sp + at.h * p.k_sh;
+                    const int64_t st = is_v ? p.v_st : p.k_st;
+                    uint8_t* tile = tiles_sm + (size_t)s * 2 * C::TILE + (is_v ? C::TILE : 0);
+                    const uint32_t t32 = smem_u32(tile);
+                    auto in_tile = [&](int row, int byte) { return tile + (cell(t32, row, byte >> 4) - t32) + (byte & 15); };
+                    if constexpr (!E4M3) {
+#pragma unroll
+                        for (int e = 0; e < E; e += 2) {
+                            const uint32_t v = pack_half2(x[e], x[e + 1]);
+                            *reinterpret_cast<uint32_t*>(page + off * st + (d0 + e) * 2) = v;
+                            *reinterpret_cast<uint32_t*>(in_tile(r, (d0 + e) * 2)) = v;
+                        }
+                    } else {
+                        float* slot = ksc + (is_v ? 8 : 0) + r / box;
+                        const float had = *slot;
+                        float amax = 0.f;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[e]));
+#pragma unroll
+                        for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                        float scale = exp2_int(scale_exponent(amax));
+                        if (off && had >= scale) {
+                            scale = had;
+                        } else if (off) {
+                            // the rows before take the larger scale, in the tile and in the page
+                            const float down = had / scale;
+                            for (int i = lane; i < off * (D / 4); i += 32) {
+                                const int row = i / (D / 4), byte = (i % (D / 4)) * 4;
+                                uint32_t* a = reinterpret_cast<uint32_t*>(in_tile(r - off + row, byte));
+                                const uint32_t lo2 = half2_of_e4m3x2(*a & 0xffffu), hi2 = half2_of_e4m3x2(*a >> 16);
+                                const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&lo2));
+                                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hi2));
+                                *a = e4m3x2(u.x * down, u.y * down) | (e4m3x2(v.x * down, v.y * down) << 16);
+                                *reinterpret_cast<uint32_t*>(page + row * st + byte) = *a;
+                            }
+                        }
+                        const float up = 1.f / scale;  // a power of two: exact
+#pragma unroll
+                        for (int e = 0; e < E; e += 2) {
+                            const uint16_t v = (uint16_t)e4m3x2(x[e] * up, x[e + 1] * up);
+                            *reinterpret_cast<uint16_t*>(page + off * st + d0 + e) = v;
+                            *reinterpret_cast<uint16_t*>(in_tile(r, d0 + e)) = v;
+                        }
+                        __syncwarp();
+                        if (lane == 0) {
+                            *slot = scale;
+                            uint8_t* b8 = is_v ? p.v_scales + id * p.vs_sp + at.h * p.vs_sh : p.k_scales + id * p.ks_sp + at.h * p.ks_sh;
+                            *b8 = (uint8_t)(__float_as_uint(scale) >> 23);
+                        }
+                    }
+                }
+                wrote = true;
+                named_bar_sync(kBar, kConsumers);
+            }
+            const int key0 = KEYS * at.j + 16 * MT * w;
+            if (ready && key0 < L) {
+                // ---- rows behind the last key: zero their values, so that 0 * NaN cannot be
+                const int nv = L - key0;
+                if (nv < 16 * MT) {
+                    const int end = min((nv + 15) & ~15, 16 * MT);
+                    for (int i = lane; i < (end - nv) * (C::ROWB / 16); i += 32) {
+                        const int r = 16 * MT * w + nv + i / (C::ROWB / 16);
+                        const uint32_t a = cell(vt, r, i % (C::ROWB / 16));
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0) : "memory");
+                    }
+                    wrote = true;
+                    __syncwarp();
+                }
+                // ---- S^T, 16 keys at a time
+                const int lrow = 16 * MT * w + (lane & 7) + (((lane >> 3) & 1) << 3);
+                float x[MT][NB][4];
+                bool live[MT];
+                float vs[MT];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const int bx = (16 * (MT * w + mt)) / box;
+                    const float ks = ksc[bx];
+                    vs[mt] = ksc[8 + bx];
+                    live[mt] = ks >= 0.f && key0 + 16 * mt < L;
+                    float s0[NB][4], s1[NB][4];
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) s0[nb][c] = s1[nb][c] = 0.f;
+                    if (live[mt]) {
+                        if constexpr (E4M3) {
+#pragma unroll
+                            for (int kk = 0; kk < KSTEPS; kk += 2) {
+                                uint32_t r0_, r1_, r2_, r3_;
+                                ldsm_x4(cell(kt, lrow + 16 * mt, kk + (lane >> 4)), r0_, r1_, r2_, r3_);
+                                const uint32_t a0 = half2_of_e4m3x2(r0_ & 0xffffu), a2 = half2_of_e4m3x2(r0_ >> 16);
+                                const uint32_t a1 = half2_of_e4m3x2(r1_ & 0xffffu), a3 = half2_of_e4m3x2(r1_ >> 16);
+                                const uint32_t b0 = half2_of_e4m3x2(r2_ & 0xffffu), b2 = half2_of_e4m3x2(r2_ >> 16);
+                                const uint32_t b1 = half2_of_e4m3x2(r3_ & 0xffffu), b3 = half2_of_e4m3x2(r3_ >> 16);
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                    for (int part = 0; part < 2; ++part) {
+                                        uint32_t u[2], v[2];
+                                        q_of(part, nb, kk, u);
+                                        q_of(part, nb, kk + 1, v);
+                                        mma_16816(s0[nb], a0, a1, a2, a3, u[0], u[1]);
+                                        mma_16816(s1[nb], b0, b1, b2, b3, v[0], v[1]);
+                                    }
+                            }
+                        } else {
+#pragma unroll
+                            for (int kk = 0; kk < KSTEPS; ++kk) {
+                                uint32_t a0, a1, a2, a3;
+                                ldsm_x4(cell(kt, lrow + 16 * mt, 2 * kk + (lane >> 4)), a0, a1, a2, a3);
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb) {
+                                    uint32_t u[2], v[2];
+                                    q_of(0, nb, kk, u);
+                                    q_of(1, nb, kk, v);
+                                    mma_16816(s0[nb], a0, a1, a2, a3, u[0], u[1]);
+                                    mma_16816(s1[nb], a0, a1, a2, a3, v[0], v[1]);
+                                }
+                            }
+                        }
+                    }
+                    const int k0 = key0 + 16 * mt + g;
+                    const float f2 = E4M3 ? ks * p.scale_log2 : p.scale_log2;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            x[mt][nb][c] = live[mt] && k0 + 8 * (c >> 1) < lim[nb][c & 1] ? (s0[nb][c] + s1[nb][c]) * f2 : -INFINITY;
+                }
+                // ---- running maximum and sum of each query row (log2 domain)
+                uint32_t pb[MT][NB][2];
+                float2 alpha[NB];
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    float al[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float mx = fmaxf(x[0][nb][c], x[0][nb][c + 2]);
+#pragma unroll
+                        for (int mt = 1; mt < MT; ++mt) mx = fmaxf(mx, fmaxf(x[mt][nb][c], x[mt][nb][c + 2]));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float mn = fmaxf(m[nb][c], mx);
+                        const float mu = mn == -INFINITY ? 0.f : mn;  // a row that has seen no key yet
+                        al[c] = ex2(m[nb][c] - mu);
+                        m[nb][c] = mn;
+                        float sum = 0.f;
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            x[mt][nb][c] = ex2(x[mt][nb][c] - mu);
+                            x[mt][nb][c + 2] = ex2(x[mt][nb][c + 2] - mu);
+                            sum += x[mt][nb][c] + x[mt][nb][c + 2];
+                        }
+                        l[nb][c] = l[nb][c] * al[c] + sum;
+                    }
+                    alpha[nb] = make_float2(al[0], al[1]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        pb[mt][nb][0] = movmatrix_t(pack_half2(x[mt][nb][0], x[mt][nb][1]));
+                        pb[mt][nb][1] = movmatrix_t(pack_half2(x[mt][nb][2], x[mt][nb][3]));
+                    }
+                }
+                // ---- O^T = alpha O^T + sum over 16-key groups of scale * V^T P^T
+                if constexpr (E4M3) {
+#pragma unroll
+                    for (int mb = 0; mb < KSTEPS; ++mb)
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            acc[nb][mb][0] = __fmul2_rn(acc[nb][mb][0], alpha[nb]);
+                            acc[nb][mb][1] = __fmul2_rn(acc[nb][mb][1], alpha[nb]);
+                        }
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        if (!live[mt]) continue;
+                        const float2 v2 = make_float2(vs[mt], vs[mt]);
+#pragma unroll
+                        for (int mb = 0; mb < KSTEPS; mb += 2) {
+                            uint32_t r[4];
+                            ldsm_x4_t(cell(vt, lrow + 16 * mt, mb + (lane >> 4)), r[0], r[1], r[2], r[3]);
+                            uint32_t a[8];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t y = __byte_perm(r[i], 0, 0x3120);  // (even dim: 2 keys, odd dim: 2 keys)
+                                a[2 * i] = half2_of_e4m3x2(y & 0xffffu);
+                                a[2 * i + 1] = half2_of_e4m3x2(y >> 16);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb) {
+                                    float o[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma_16816(o, a[4 * k], a[4 * k + 1], a[4 * k + 2], a[4 * k + 3], pb[mt][nb][0], pb[mt][nb][1]);
+                                    acc[nb][mb + k][0] = __ffma2_rn(make_float2(o[0], o[1]), v2, acc[nb][mb + k][0]);
+                                    acc[nb][mb + k][1] = __ffma2_rn(make_float2(o[2], o[3]), v2, acc[nb][mb + k][1]);
+                                }
+                        }
+                    }
+                } else {
+                    const int vrow = 16 * MT * w + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+                    for (int mb = 0; mb < KSTEPS; ++mb) {
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            acc[nb][mb][0] = __fmul2_rn(acc[nb][mb][0], alpha[nb]);
+                            acc[nb][mb][1] = __fmul2_rn(acc[nb][mb][1], alpha[nb]);
+                        }
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            if (!live[mt]) continue;
+                            uint32_t a0, a1, a2, a3;
+                            ldsm_x4_t(cell(vt, vrow + 16 * mt, 2 * mb + ((lane >> 3) & 1)), a0, a1, a2, a3);
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                float o[4] = {acc[nb][mb][0].x, acc[nb][mb][0].y, acc[nb][mb][1].x, acc[nb][mb][1].y};
+                                mma_16816(o, a0, a1, a2, a3, pb[mt][nb][0], pb[mt][nb][1]);
+                                acc[nb][mb][0] = make_float2(o[0], o[1]);
+                                acc[nb][mb][1] = make_float2(o[2], o[3]);
+                            }
+                        }
+                    }
+                }
+            }
+            if (wrote) fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+
+            if (at.j == at.tiles - 1 || it == ntiles - 1) {
+                // ---- the unit's (or its part's) end: join the four warps, halving them twice
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float v = l[nb][c];
+                        v += __shfl_xor_sync(0xffffffffu, v, 4);
+                        v += __shfl_xor_sync(0xffffffffu, v, 8);
+                        v += __shfl_xor_sync(0xffffffffu, v, 16);
+                        l[nb][c] = v;
+                    }
+                // dims of accumulator element (mb, k): e4m3 16 mb + 2 g + k, fp16 16 mb + g + 8 k
+                auto dim = [&](int mb, int k) { return 16 * mb + (E4M3 ? 2 * g + k : g + 8 * k); };
+#pragma unroll
+                for (int far = 2; far >= 1; far >>= 1) {
+                    if (w >= far && w < 2 * far) {
+                        float* dst = red + (w - far) * COLS * RP;
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const int c = nb * 8 + 2 * t4;
+#pragma unroll
+                            for (int mb = 0; mb < KSTEPS; ++mb)
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {
+                                    dst[c * RP + dim(mb, k)] = acc[nb][mb][k].x;
+                                    dst[(c + 1) * RP + dim(mb, k)] = acc[nb][mb][k].y;
+                                }
+                            if (g == 0)
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {
+                                    red_ml[((w - far) * COLS + c + k) * 2] = m[nb][k];
+                                    red_ml[((w - far) * COLS + c + k) * 2 + 1] = l[nb][k];
+                                }
+                        }
+                    }
+                    named_bar_sync(kBar, kConsumers);
+                    if (w < far) {
+                        const float* src = red + w * COLS * RP;
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const int c = nb * 8 + 2 * t4;
+                            float a[2], o[2];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const float om = red_ml[(w * COLS + c + k) * 2], ol = red_ml[(w * COLS + c + k) * 2 + 1];
+                                const float mn = fmaxf(m[nb][k], om), mu = mn == -INFINITY ? 0.f : mn;
+                                a[k] = ex2(m[nb][k] - mu);
+                                o[k] = ex2(om - mu);
+                                l[nb][k] = l[nb][k] * a[k] + ol * o[k];
+                                m[nb][k] = mn;
+                            }
+#pragma unroll
+                            for (int mb = 0; mb < KSTEPS; ++mb)
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {
+                                    acc[nb][mb][k].x = acc[nb][mb][k].x * a[0] + src[c * RP + dim(mb, k)] * o[0];
+                                    acc[nb][mb][k].y = acc[nb][mb][k].y * a[1] + src[(c + 1) * RP + dim(mb, k)] * o[1];
+                                }
+                        }
+                    }
+                    if (far == 2) named_bar_sync(kBar, kConsumers);
+                }
+                // warp 0 holds the joined state: the result, or this CTA's part of it
+                const long long unit0 = base[at.b] + ((long long)at.h * at.groups + at.c) * at.tiles;
+                // CTA that holds tile t of the line: ceil((t + 1) CT / N) - 1
+                const int ca = (int)(((unit0 + 1) * CT + N - 1) / N - 1);
+                const int cb = (int)(((unit0 + at.tiles) * CT + N - 1) / N - 1);
+                const bool whole = ca == cb;
+                const int64_t tok0 = p.cu_q ? p.cu_q[at.b] : at.b;
+                auto out_row = [&](int c) {
+                    const int i = (r0 + c) / G;
+                    return p.out + (tok0 + i) * p.o_st + (int64_t)(at.h * G + (r0 + c) - i * G) * p.o_sh;
+                };
+                if (w == 0) {
+                    const size_t part = 2 * (size_t)blockIdx.x + (first_tile == 0 ? 1 : 0);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int c = nb * 8 + 2 * t4 + k;
+                            if (c >= rows) continue;
+                            const float inv = l[nb][k] > 0.f ? 1.f / l[nb][k] : 0.f;
+                            __half* o16 = out_row(c);
+                            float* o32 = sp.part_o + (part * kMaxCols + c) * D;
+                            if (!whole && g == 0)
+                                sp.part_lse[part * kMaxCols + c] = l[nb][k] > 0.f ? m[nb][k] + __log2f(l[nb][k]) : -INFINITY;
+#pragma unroll
+                            for (int mb = 0; mb < KSTEPS; ++mb) {
+                                const float y0 = (k ? acc[nb][mb][0].y : acc[nb][mb][0].x) * inv;
+                                const float y1 = (k ? acc[nb][mb][1].y : acc[nb][mb][1].x) * inv;
+                                if (whole) {
+                                    if constexpr (E4M3) {
+                                        *reinterpret_cast<uint32_t*>(o16 + dim(mb, 0)) = pack_half2(y0, y1);
+                                    } else {
+                                        o16[dim(mb, 0)] = __float2half_rn(y0);
+                                        o16[dim(mb, 1)] = __float2half_rn(y1);
+                                    }
+                                } else {
+                                    o32[dim(mb, 0)] = y0;
+                                    o32[dim(mb, 1)] = y1;
+                                }
+                            }
+                        }
+                }
+                if (!whole) {
+                    // the last part to arrive joins them. Release: the barrier orders warp 0's stores
+                    // before thread 0's fence and count; acquire: its fence after the count.
+                    // The counter is that of the unit's first CTA, where no other cut unit begins.
+                    named_bar_sync(kBar, kConsumers);
+                    if (tid == 0) {
+                        __threadfence();
+                        misc[1] = atomicAdd(&sp.cut_cnt[ca], 1u) == (unsigned)(cb - ca);
+                        if (misc[1]) __threadfence();
+                    }
+                    named_bar_sync(kBar, kConsumers);
+                    if (misc[1]) {
+                        const int parts = cb - ca + 1;
+                        for (int e = tid * 4; e < rows * D; e += 4 * kConsumers) {
+                            const int c = e / D, d = e - c * D;
+                            float M = -INFINITY, W = 0.f;
+                            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                            for (int i = 0; i < parts; ++i) {
+                                const size_t part = 2 * (size_t)(ca + i) + (i == 0 ? 1 : 0);
+                                const float lse = __ldcg(sp.part_lse + part * kMaxCols + c);
+                                const float4 y = __ldcg(reinterpret_cast<const float4*>(sp.part_o + (part * kMaxCols + c) * D + d));
+                                const float mn = fmaxf(M, lse), mu = mn == -INFINITY ? 0.f : mn;
+                                const float a = ex2(M - mu), u = ex2(lse - mu);
+                                W = W * a + u;
+                                o.x = o.x * a + y.x * u, o.y = o.y * a + y.y * u;
+                                o.z = o.z * a + y.z * u, o.w = o.w * a + y.w * u;
+                                M = mn;
+                            }
+                            const float inv = W > 0.f ? 1.f / W : 0.f;
+                            uint2 v;
+                            v.x = pack_half2(o.x * inv, o.y * inv);
+                            v.y = pack_half2(o.z * inv, o.w * inv);
+                            *reinterpret_cast<uint2*>(out_row(c) + d) = v;
+                        }
+                        if (tid == 0) atomicExch(&sp.cut_cnt[ca], 0u);
+                    }
+                }
+                named_bar_sync(kBar, kConsumers);  // the joining buffer becomes the next unit's queries
+                fresh = true;
+            }
+            step(at);
+        }
+    }
+    advance_lengths(p, misc + 2);
+}
+
+template <int D, int NB, bool E4M3>
+static int launch_split_t(SplitParams& sp, const Freqs& f, int sms, int dev, cudaStream_t st) {
+    using C = Cfg<D, NB, E4M3>;
+    const Params& p = sp.p;
+    static std::once_flag once[128];
+    static cudaError_t attr[128];
+    if (dev < 0 || dev >= 128) return set_status(FCCI_EINVAL, "device index");
+    std::call_once(once[dev], [&]() {
+        attr[dev] = cudaFuncSetAttribute(paged_split_kernel<D, NB, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    });
+    if (attr[dev] != cudaSuccess) return set_cuda_status(attr[dev]);
+    // tokens whose angles a unit needs at once
+    const int rope_rows = p.cu_q ? (C::COLS + p.G - 1) / p.G + 1 : 1;
+    int stages = 0, per_sm = 0;
+    for (int ctas = kMaxCtasPerSm; ctas >= 1 && !stages; --ctas)
+        for (int s = kMaxStages; s >= 2 && !stages; --s)
+            if (C::smem(s, p.B, rope_rows, p.rot) <= (size_t)(228 * 1024 / ctas - 1024)) stages = s, per_sm = ctas;
+    if (!stages) return set_status(FCCI_EUNSUPPORTED, "paged attention: batch too large for shared memory");
+    sp.stages = stages;
+    const int elt = E4M3 ? 1 : 2;
+    CUtensorMap m[4];
+    int rc = 0;
+    for (int i = 0; i < 4 && !rc; ++i) {
+        const bool v = i & 1;
+        const uint64_t dims[4] = {(uint64_t)D, (uint64_t)p.page, (uint64_t)p.Hkv, (uint64_t)p.num_pages};
+        const int64_t sb[3] = {v ? p.v_st : p.k_st, v ? p.v_sh : p.k_sh, v ? p.v_sp : p.k_sp};
+        const uint32_t box[4] = {(uint32_t)(C::PITCH / elt), (uint32_t)(i < 2 ? (p.page < C::KEYS ? p.page : C::KEYS) : 16), 1, 1};
+        rc = encode_tiled(&m[i], E4M3, C::PITCH == 64, v ? p.v_pages : p.k_pages, 4, dims, sb, box);
+    }
+    if (rc) return set_status(rc, "paged attention: cuTensorMapEncodeTiled rejected the page layout");
+    const size_t smem = C::smem(stages, p.B, rope_rows, p.rot);
+    return launch_pdl(paged_split_kernel<D, NB, E4M3>, dim3(sms * per_sm), dim3(kThreads), smem, st, m[0], m[1], m[2], m[3], sp, f);
+}
+
+int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, uint8_t* ws, const WsLayout& L, cudaStream_t st) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
+    const int sms = device_sm_count(dev);
+    SplitParams sp;
+    sp.p = p;
+    sp.fused = fused;
+    sp.stages = 0;
+    sp.cut_cnt = reinterpret_cast<uint32_t*>(ws + 256);
+    sp.part_lse = reinterpret_cast<float*>(ws + L.part_lse);
+    sp.part_o = reinterpret_cast<float*>(ws + L.part_o);
+    if (sms * kMaxCtasPerSm > kMaxGrid) return set_status(FCCI_EUNSUPPORTED, "paged attention: too many SMs");
+    const int nb = (int64_t)p.max_q * p.G <= 8 || p.D == 256 ? 1 : 2;
+    switch ((p.D * 10 + nb) * 2 + (e4m3 ? 1 : 0)) {
+        case 1282: return launch_split_t<64, 1, false>(sp, f, sms, dev, st);
+        case 1283: return launch_split_t<64, 1, true>(sp, f, sms, dev, st);
+        case 1284: return launch_split_t<64, 2, false>(sp, f, sms, dev, st);
+        case 1285: return launch_split_t<64, 2, true>(sp, f, sms, dev, st);
+        case 2562: return launch_split_t<128, 1, false>(sp, f, sms, dev, st);
+        case 2563: return launch_split_t<128, 1, true>(sp, f, sms, dev, st);
+        case 2564: return launch_split_t<128, 2, false>(sp, f, sms, dev, st);
+        case 2565: return launch_split_t<128, 2, true>(sp, f, sms, dev, st);
+        case 5122: return launch_split_t<256, 1, false>(sp, f, sms, dev, st);
+        case 5123: return launch_split_t<256, 1, true>(sp, f, sms, dev, st);
+        default: return set_status(FCCI_EUNSUPPORTED, "paged attention: unsupported head_dim");
+    }
+}
+
+}  // namespace pg
+}  // namespace fcci

@@ -1,4 +1,4 @@
-// Attention over the paged KV cache, and the host side of the paged entry points.
+// Host side of the paged entry points: checks, workspace layout and dispatch.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -9,97 +9,6 @@
 
 namespace fcci {
 namespace pg {
-
-constexpr int kAttnThreads = 128;
-
-// One CTA per (new token, query head, sequence): warp w takes keys w, w + 4, ... with a running
-// maximum and sum, and the four states are joined at the end.
-template <int D, bool E4M3>
-__global__ void __launch_bounds__(kAttnThreads) paged_attn_kernel(const __grid_constant__ Params p) {
-    constexpr int E = D / 32, kWarps = kAttnThreads / 32;
-    __shared__ float acc_sm[kWarps][D], m_sm[kWarps], l_sm[kWarps];
-    __shared__ int flag;
-    griddep_launch_dependents();
-    griddep_wait();
-    const int i = blockIdx.x, hq = blockIdx.y, b = blockIdx.z;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d0 = lane * E;
-    const Seq s = seq_of(p, b);
-    const int n = s.ok ? s.n : 0;
-    if (!s.ok && i == 0 && hq == 0 && threadIdx.x == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
-    const bool row_there = i < n || (!s.ok && !p.cu_q);
-    if (row_there) {
-        const int keys = s.ok ? s.T + (p.append ? i + 1 : 0) : 0;
-        const int64_t row = p.cu_q ? s.tok0 + i : b;
-        const int h = hq / p.G;
-        float q[E], acc[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            q[e] = __half2float(p.q[row * p.q_st + hq * p.q_sh + d0 + e]);
-            acc[e] = 0.f;
-        }
-        for (int t = warp; t < keys; t += kWarps) {
-            const int id = page_of(p, b, t);
-            if (id < 0) continue;
-            const uint8_t* kr = p.k_pages + id * p.k_sp + h * p.k_sh + (t & (p.page - 1)) * p.k_st;
-            const uint8_t* vr = p.v_pages + id * p.v_sp + h * p.v_sh + (t & (p.page - 1)) * p.v_st;
-            float ks = 1.f, vs = 1.f, x = 0.f, k[E], v[E];
-            if constexpr (E4M3) {
-                ks = exp2_int((int)p.k_scales[id * p.ks_sp + h * p.ks_sh] - 127);
-                vs = exp2_int((int)p.v_scales[id * p.vs_sp + h * p.vs_sh] - 127);
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const uint32_t a = half2_of_e4m3x2(kr[d0 + e]), c = half2_of_e4m3x2(vr[d0 + e]);
-                    k[e] = __low2float(*reinterpret_cast<const __half2*>(&a));
-                    v[e] = __low2float(*reinterpret_cast<const __half2*>(&c));
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    k[e] = __half2float(reinterpret_cast<const __half*>(kr)[d0 + e]);
-                    v[e] = __half2float(reinterpret_cast<const __half*>(vr)[d0 + e]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) x = fmaf(q[e], k[e], x);
-#pragma unroll
-            for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-            x *= ks * p.scale_log2;
-            const float mn = fmaxf(m, x), al = ex2(m - mn), pr = ex2(x - mn);
-            l = l * al + pr;
-            m = mn;
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = acc[e] * al + pr * vs * v[e];
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc_sm[warp][d0 + e] = acc[e];
-        if (lane == 0) m_sm[warp] = m, l_sm[warp] = l;
-        __syncthreads();
-        for (int d = threadIdx.x; d < D; d += kAttnThreads) {
-            float M = -INFINITY, L = 0.f, o = 0.f;
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, m_sm[w]);
-            for (int w = 0; w < kWarps && M != -INFINITY; ++w) {
-                const float a = ex2(m_sm[w] - M);
-                L += l_sm[w] * a;
-                o += acc_sm[w][d] * a;
-            }
-            p.out[row * p.o_st + hq * p.o_sh + d] = __float2half_rn(L > 0.f ? o / L : 0.f);
-        }
-    }
-    advance_lengths(p, &flag);
-}
-
-template <int D, bool E4M3>
-static int launch_attn_t(const Params& p, cudaStream_t st) {
-    return launch_pdl(paged_attn_kernel<D, E4M3>, dim3(p.max_q, p.Hq, p.B), dim3(kAttnThreads), 0, st, p);
-}
-
-static int launch_attn(const Params& p, bool e4m3, cudaStream_t st) {
-    switch (p.D) {
-        case 64: return e4m3 ? launch_attn_t<64, true>(p, st) : launch_attn_t<64, false>(p, st);
-        case 128: return e4m3 ? launch_attn_t<128, true>(p, st) : launch_attn_t<128, false>(p, st);
-        default: return e4m3 ? launch_attn_t<256, true>(p, st) : launch_attn_t<256, false>(p, st);
-    }
-}
 
 // ------------------------------------------------------------------ host side
 
@@ -235,14 +144,16 @@ static int paged_step(const fcci_paged_desc* d, Op op, cudaStream_t stream) {
         p.advance = d->advance;
         return launch_append(p, f, e4m3, stream);
     }
-    // the append writes the rotated queries to q_rot, where the attention reads them
-    if (p.append || p.rot > 0 || d->q_rot_out) {
-        rc = launch_append(p, f, e4m3, stream);
+    uint8_t* ws = static_cast<uint8_t*>(d->workspace);
+    p.q_rot = static_cast<__half*>(d->q_rot_out);
+    if (op == Op::kPrefill) {
+        Params rows = p;
+        rows.q = nullptr;
+        rc = launch_append(rows, f, e4m3, stream);
         if (rc) return rc;
-        p.q = p.q_rot, p.q_st = (int64_t)p.Hq * p.D, p.q_sh = p.D;
     }
     p.advance = d->advance;
-    return launch_attn(p, e4m3, stream);
+    return launch_split(p, f, e4m3, op == Op::kDecode && p.append, ws, L, stream);
 }
 
 }  // namespace pg

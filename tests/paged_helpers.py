@@ -129,15 +129,16 @@ def check_q_rot(q_rot, exact):
     assert ((q_rot.double() - exact).abs() <= tol).all(), float((q_rot.double() - exact).abs().max())
 
 
-def check_attention(out, q_rot, cache, table, lens_of_row, seq_of_row, scale, what="", q_steps=0.0):
+def check_attention(out, q, cache, table, lens_of_row, seq_of_row, scale, what="", q_fp16=False):
     """out [rows, Hq, D] against 64 bits over what the pools hold, elementwise.
 
-    Given the fp16 rotated queries, a score is off by at most eps = 2^-16 * sum|q k| scale (an fp32 sum of up to 256
-    products in any order: 256 * 2^-24), so a normalised weight by 2 eps of itself; a weight is rounded to fp16
-    (2^-11, or 2^-25 absolute below its normals) and comes from an approximate power of two (2^-21 and less); the fp32
-    sums over L keys are off by L * 2^-24, above and below the fraction line; the result is rounded to fp16
-    (2^-11, or 2^-25 absolute). All of it moves out by at most that share of sum(weight |v|).
-    q_steps: fp16 steps by which one element of a query may differ from the kernel's."""
+    q [rows, Hq, D]: the queries rotated in 64 bits. The kernels rotate them in fp32 (off by 2^-21 of the pair's sizes)
+    and hold them in two fp16 parts (2^-22), or, with q_fp16, in one (2^-11). A score is then off by at most
+    eps = (2^-16 + 2^-19) * sum|q k| scale (256 fp32 products summed in any order: 256 * 2^-24), with q_fp16 by 2^-11 of
+    that sum more, so a normalised weight by 2 eps of itself; a weight is rounded to fp16 (2^-11, or 2^-25 absolute
+    below its normals) and comes from an approximate power of two (2^-21 and less); the fp32 sums over L keys
+    are off by L * 2^-24, above and below the fraction line; the result is rounded to fp16 (2^-11, or 2^-25 absolute).
+    All of it moves out by at most that share of sum(weight |v|)."""
     hq, D = out.shape[1], out.shape[2]
     hkv = cache["k"].shape[1]
     worst = 0.0
@@ -150,12 +151,10 @@ def check_attention(out, q_rot, cache, table, lens_of_row, seq_of_row, scale, wh
                 held[b] = P.keys_values(cache["k"], cache["v"], cache["k_scales"], cache["v_scales"], table[b], top, h)
             k, v = held[b][0][:L], held[b][1][:L]
             for g in range(hq // hkv):
-                o, w, s = P.attention(q_rot[r, h * (hq // hkv) + g], k, v, scale)
+                o, w, s = P.attention(q[r, h * (hq // hkv) + g], k, v, scale)
                 got = out[r, h * (hq // hkv) + g].double()
                 vmax = v.abs().max(0).values if L else torch.zeros(D, dtype=torch.float64)
-                s = s * 2.0 ** -16
-                if q_steps and L:
-                    s += q_steps * 2.0 ** -10 * scale * float((k * q_rot[r, h * (hq // hkv) + g].double()).abs().max())
+                s *= 2.0 ** -16 + 2.0 ** -19 + (2.0 ** -11 if q_fp16 else 0.0)
                 tol = w * (2 * s + 2.0 ** -11 + 2.0 ** -19 + 2 * L * 2.0 ** -24) + L * 2.0 ** -25 * vmax \
                     + o.abs() * 2.0 ** -11 + 2.0 ** -25
                 worst = max(worst, float(((got - o).abs() / tol).nan_to_num(1e9).max()))

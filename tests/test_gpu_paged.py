@@ -35,6 +35,10 @@ def exact_rotation(x, pos, rot, theta=10000.0):
     return torch.stack([P.rope(x[i], p, rot, theta) for i, p in enumerate(pos)]) if pos else x[:0].double()
 
 
+def rotated_queries(t, rot=None):
+    return exact_rotation(t["q"][: len(t["pos"])], t["pos"], t["q"].shape[2] if rot is None else rot)
+
+
 def run_append(av, c, t, varlen, rot=-1, theta=10000.0, advance=False, with_q=True, ws=None):
     d = H.to_device(c)
     q, k, v = t["q"].to(DEV), t["k"].to(DEV), t["v"].to(DEV)
@@ -216,7 +220,7 @@ def test_decode(av, e4m3, D, page, hkv, group, layout):
     assert err == 0
     check_whole_append(c, t, d, q_rot, D)
     after = H.back(d)
-    H.check_attention(out, q_rot, after, c["table"], [x + 1 for x in T], range(len(T)), D ** -0.5, "decode")
+    H.check_attention(out, rotated_queries(t), after, c["table"], [x + 1 for x in T], range(len(T)), D ** -0.5, "decode")
     assert d["T"].cpu().tolist() == [x + 1 for x in T]
 
 
@@ -233,7 +237,7 @@ def test_decode_without_new_rows(av, e4m3):
     for name in "kv":
         assert torch.equal(H.bits(after[name]), H.bits(c[name]))
     assert (out[0] == 0).all()
-    H.check_attention(out, q_rot, c, c["table"], T, range(len(T)), 128 ** -0.5, "decode")
+    H.check_attention(out, t["q"].double(), c, c["table"], T, range(len(T)), 128 ** -0.5, "decode")
 
 
 def test_decode_long_and_ragged(av):
@@ -243,7 +247,7 @@ def test_decode_long_and_ragged(av):
     t = new_tokens(c, 4, seed=72)
     d, out, q_rot, err = run_decode(av, c, t, scale=0.05)
     assert err == 0
-    H.check_attention(out, q_rot, H.back(d), c["table"], [x + 1 for x in T], range(len(T)), 0.05, "decode")
+    H.check_attention(out, rotated_queries(t), H.back(d), c["table"], [x + 1 for x in T], range(len(T)), 0.05, "decode")
 
 
 def test_decode_sharp_scores_and_uneven_scales(av):
@@ -256,11 +260,11 @@ def test_decode_sharp_scores_and_uneven_scales(av):
         c[name + "_scales"] = (e + 127).to(torch.uint8)
     t = new_tokens(c, 4, seed=83)
     d, out, q_rot, err = run_decode(av, c, t, scale=1e-6)
-    H.check_attention(out, q_rot, H.back(d), c["table"], [x + 1 for x in T], [0, 1], 1e-6, "flat")
+    H.check_attention(out, rotated_queries(t), H.back(d), c["table"], [x + 1 for x in T], [0, 1], 1e-6, "flat")
     c["k_scales"].fill_(127)
     d, out, q_rot, err = run_decode(av, c, t, scale=1.0)
     assert err == 0
-    H.check_attention(out, q_rot, H.back(d), c["table"], [x + 1 for x in T], [0, 1], 1.0, "sharp")
+    H.check_attention(out, rotated_queries(t), H.back(d), c["table"], [x + 1 for x in T], [0, 1], 1.0, "sharp")
 
 
 def test_decode_bad_page_and_capacity(av):
@@ -272,7 +276,7 @@ def test_decode_bad_page_and_capacity(av):
         d, out, q_rot, err = run_decode(av, c, t)
         assert err == PAGE_ERR
         rows = [0, 2]
-        H.check_attention(out[rows], q_rot[rows], H.back(d), c["table"], [51, 31], rows, 128 ** -0.5, "others")
+        H.check_attention(out[rows], rotated_queries(t)[rows], H.back(d), c["table"], [51, 31], rows, 128 ** -0.5, "others")
         assert not out[1].isnan().any()
     c = H.make_cache(T, [1] * 3, 2, 128, 16, True, seed=93)
     c["T"] = torch.tensor([50, 16 * c["table"].shape[1], -5], dtype=torch.int32)
@@ -280,7 +284,7 @@ def test_decode_bad_page_and_capacity(av):
     d, out, q_rot, err = run_decode(av, c, t, advance=True)
     assert err == CAPACITY and d["T"].cpu().tolist() == [51, 16 * c["table"].shape[1], -5]
     assert (out[1:] == 0).all()
-    H.check_attention(out[:1], q_rot[:1], H.back(d), c["table"], [51], [0], 128 ** -0.5, "the one that fits")
+    H.check_attention(out[:1], rotated_queries(t)[:1], H.back(d), c["table"], [51], [0], 128 ** -0.5, "the one that fits")
 
 
 def test_decode_shared_prefix_pages(av):
@@ -290,7 +294,7 @@ def test_decode_shared_prefix_pages(av):
     t = new_tokens(c, 4, seed=102)
     d, out, q_rot, err = run_decode(av, c, t)
     assert err == 0
-    H.check_attention(out, q_rot, H.back(d), c["table"], [65, 65], [0, 1], 128 ** -0.5, "shared")
+    H.check_attention(out, rotated_queries(t), H.back(d), c["table"], [65, 65], [0, 1], 128 ** -0.5, "shared")
 
 
 # ---------------------------------------------------------------- prefill
@@ -310,16 +314,14 @@ def run_prefill(av, c, t, advance=False, rot=-1, ws=None, max_new=None):
 
 
 def check_prefill(c, t, d, out, rot=128):
-    """The pools as an append leaves them, and causal attention over them with the queries that the kernel
-    multiplies: the rotation rounded to fp16. It is taken from 64 bits here, so one of a query's 128 elements may lie
-    on the other side of a rounding border, one fp16 step away."""
+    """The pools as an append leaves them, and causal attention over them (long chunks hold the queries in fp16)."""
     n = len(t["pos"])
     after = H.back(d)
     H.check_append(c, after, "k", c["T"], t["cu"], c["table"], exact_rotation(t["k"][:n], t["pos"], rot), rot > 0)
     H.check_append(c, after, "v", c["T"], t["cu"], c["table"], t["v"][:n].double(), False)
     seq = [b for b, m in enumerate(c["new"]) for _ in range(m)]
-    q = exact_rotation(t["q"][:n], t["pos"], rot).half()
-    H.check_attention(out[:n], q, after, c["table"], [p + 1 for p in t["pos"]], seq, 128 ** -0.5, "prefill", q_steps=1.0)
+    q = rotated_queries(t, rot)
+    H.check_attention(out[:n], q, after, c["table"], [p + 1 for p in t["pos"]], seq, 128 ** -0.5, "prefill", q_fp16=True)
     assert (out[n:] == 7.0).all(), "rows behind the last sequence were written"
 
 
@@ -349,8 +351,8 @@ def test_prefill_out_of_room(av):
     seq = [0] * 40 + [2] * 20
     rows = list(range(40)) + list(range(340, 360))
     pos = list(range(40)) + list(range(20))
-    q = exact_rotation(t["q"][rows], pos, 128).half()
-    H.check_attention(out[rows], q, H.back(d), c["table"], [p + 1 for p in pos], seq, 128 ** -0.5, "others", q_steps=1.0)
+    q = exact_rotation(t["q"][rows], pos, 128)
+    H.check_attention(out[rows], q, H.back(d), c["table"], [p + 1 for p in pos], seq, 128 ** -0.5, "others", q_fp16=True)
     assert (out[40:340] == 7.0).all()
     for new in ([40, 3], [100, 90]):
         c = H.make_cache([40, 17], new, 1, 128, 16, True, seed=123)
@@ -358,6 +360,6 @@ def test_prefill_out_of_room(av):
         t = new_tokens(c, 2, seed=124)
         d, out, err = run_prefill(av, c, t)
         assert err == PAGE_ERR
-        q = exact_rotation(t["q"][: new[0]], t["pos"][: new[0]], 128).half()
+        q = rotated_queries(t)[: new[0]]
         H.check_attention(out[: new[0]], q, H.back(d), c["table"], [p + 1 for p in t["pos"][: new[0]]], [0] * new[0],
-                          128 ** -0.5, "others", q_steps=1.0)
+                          128 ** -0.5, "others", q_fp16=True)
