@@ -80,13 +80,15 @@ __device__ __forceinline__ int page_of(const Params& p, int b, int t) {
     return -1;
 }
 
-// Smallest e in [kScaleMin, kScaleMax] with amax <= 448 * 2^e: 448 = 1.75 * 2^8, so with
-// amax = m * 2^E it is E - 8, one more when m > 1.75 (mantissa bits above 0x600000).
-__device__ __forceinline__ int scale_exponent(float amax) {
+// Smallest e in [lo, hi] with amax <= 448 * 2^e: 448 = 1.75 * 2^8, so with amax = m * 2^E it is
+// E - 8, one more when m > 1.75 (mantissa bits above 0x600000).
+__device__ __forceinline__ int exponent_448(float amax, int lo, int hi) {
     const uint32_t u = __float_as_uint(amax);
     const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-    return max(kScaleMin, min(kScaleMax, e));
+    return max(lo, min(hi, e));
 }
+
+__device__ __forceinline__ int scale_exponent(float amax) { return exponent_448(amax, kScaleMin, kScaleMax); }
 
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -154,6 +156,9 @@ WsLayout ws_layout(int Hq, int Hkv, int D, int total_q, int max_q, int max_kv, i
 int launch_append(const Params& p, const Freqs& f, bool e4m3, cudaStream_t st);
 // Split-KV attention; `fused`: the launch appends the one new row of each sequence itself.
 int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, uint8_t* ws, const WsLayout& L, cudaStream_t st);
+struct TileParams;
+// The same on the 5th-generation tensor cores, for e4m3 pages of head_dim 128.
+int launch_split_tc(TileParams& tp, const Freqs& f, int sms, int dev, cudaStream_t st);
 
 }  // namespace pg
 }  // namespace fcci

@@ -1,12 +1,7 @@
 // Split-KV attention over the paged cache: one new token per sequence (decode, with its append
 // fused in), or a few of them (a short chunk whose rows an append has written already).
 //
-// Work. A unit is (sequence b, kv head h, column group c): up to 8 * NB query rows of the group,
-// rows being (token, query head) pairs, so a cached key is read once for all of them. A unit's
-// keys are cut into tiles of KEYS rows; all tiles of all units form one line, of which every CTA of a
-// persistent grid takes an equal stretch, whatever the lengths are. A unit that lies in one
-// stretch is finished there; of a cut one, every CTA leaves its part (o, log-sum-exp) in the
-// workspace and the last to arrive joins them. No CTA waits for another.
+// Work: paged_tiles.cuh.
 //
 // Inside a CTA warp 4 fetches and warps 0..3 compute. A stage holds the K and the V tile, in
 // rows of 128 bytes (64 for e4m3 with head_dim 64) in the tensor-map swizzle; the pages of a tile
@@ -26,25 +21,12 @@
 
 #include <mutex>
 
-#include "paged.cuh"
+#include "paged_tiles.cuh"
 
 namespace fcci {
 namespace pg {
 
-constexpr int kConsumerWarps = 4, kConsumers = kConsumerWarps * 32, kThreads = kConsumers + 32;
-constexpr int kMaxStages = 6;
-constexpr uint64_t kWaitLimitNs = 4000000000ull;  // 4 s: far beyond any healthy wait
-constexpr uint64_t kDrainLimitNs = 500000000ull;
-constexpr int kBar = 1;
-
-struct SplitParams {
-    Params p;
-    int32_t fused;   // the kernel appends row T itself (decode)
-    int32_t stages;
-    float* part_lse;  // [2 * grid][kMaxCols]
-    float* part_o;    // [2 * grid][kMaxCols][D]
-    uint32_t* cut_cnt;  // [grid], zero between calls
-};
+constexpr int kThreads = kCompute + 32;
 
 template <int D, int NB, bool E4M3>
 struct Cfg {
@@ -53,9 +35,8 @@ struct Cfg {
     // that grows its scale rewrites the page's rows where the tile holds them
     static constexpr int KEYS = ROWB <= 128 && (E4M3 || NB == 1) ? 128 : 64;
     static constexpr int MT = KEYS / 64;                      // 16-key groups of a warp
-    static constexpr int PITCH = ROWB < 128 ? ROWB : 128;     // bytes of a row in one block
-    static constexpr int BLOCKS = ROWB / PITCH;               // blocks side by side
-    static constexpr int TILE = KEYS * ROWB;
+    using TL = Tile<KEYS, ROWB>;
+    static constexpr int TILE = TL::BYTES;
     static constexpr int COLS = 8 * NB;
     static constexpr int RP = D + 4;                          // fp32 pitch of the joining rows
     static constexpr int QP = D + 16;                         // fp16 pitch of the query rows
@@ -65,14 +46,9 @@ struct Cfg {
     static constexpr int QB = QREG ? 0 : 2 * COLS * QP * 2;   // bytes of their own buffer
     static_assert(!QREG || 2 * COLS * QP * 2 <= RED, "queries in the joining buffer");
     static size_t smem(int stages, int B, int rope_rows, int rot) {
-        return 1024 + (size_t)stages * 2 * TILE + RED + QB + (size_t)rope_rows * (rot / 2) * 8 + 2 * kConsumerWarps * COLS * 4 +
+        return 1024 + (size_t)stages * 2 * TILE + RED + QB + (size_t)rope_rows * (rot / 2) * 8 + 2 * kComputeWarps * COLS * 4 +
                kMaxStages * (2 * 8 * 4 + 16) + 64 + (size_t)(3 * B + 2) * 4;
     }
-};
-
-struct Line {  // a place on the line of tiles
-    int b, h, c, j;     // sequence, kv head, column group, tile
-    int tiles, groups;  // of sequence b
 };
 
 template <int D, int NB, bool E4M3>
@@ -80,40 +56,39 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                                                             const __grid_constant__ CUtensorMap mv,
                                                             const __grid_constant__ CUtensorMap mk16,
                                                             const __grid_constant__ CUtensorMap mv16,
-                                                            const __grid_constant__ SplitParams sp,
+                                                            const __grid_constant__ TileParams sp,
                                                             const __grid_constant__ Freqs f) {
     using C = Cfg<D, NB, E4M3>;
-    constexpr int KEYS = C::KEYS, MT = C::MT, PITCH = C::PITCH, COLS = C::COLS, RP = C::RP, QP = C::QP;
-    constexpr int KSTEPS = D / 16, CHUNKS = PITCH / 16;
+    using TL = typename C::TL;
+    constexpr int KEYS = C::KEYS, MT = C::MT, COLS = C::COLS, RP = C::RP, QP = C::QP;
+    constexpr int KSTEPS = D / 16;
     const Params& p = sp.p;
     extern __shared__ uint8_t raw[];
     uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-    const int S = sp.stages, B = p.B, Hkv = p.Hkv, G = p.G;
+    const int S = sp.stages, B = p.B, G = p.G;
     uint8_t* tiles_sm = sm;
     float* red = reinterpret_cast<float*>(sm + (size_t)S * 2 * C::TILE);
     __half* q_hi = reinterpret_cast<__half*>(C::QREG ? red : red + C::RED / 4);
     __half* q_lo = q_hi + COLS * QP;
     float* red_ml = red + (C::RED + C::QB) / 4;              // [4 warps][COLS][2]
-    uint64_t* full = reinterpret_cast<uint64_t*>(red_ml + 2 * kConsumerWarps * COLS);
+    uint64_t* full = reinterpret_cast<uint64_t*>(red_ml + 2 * kComputeWarps * COLS);
     uint64_t* empty = full + kMaxStages;
     float* scale_sm = reinterpret_cast<float*>(empty + kMaxStages);  // [stage][K, V][8 page boxes]; K -1: no such page
     int* misc = reinterpret_cast<int*>(scale_sm + kMaxStages * 16);
     volatile int* abort_flag = misc;
-    int* base = misc + 16;  // [B + 1] tiles before sequence b
-    int* seqT = base + B + 1;
-    int* seqN = seqT + B;
-    float2* cs = reinterpret_cast<float2*>(seqN + B + ((B + 1) & 1));
+    Line<KEYS, COLS> line(sp, misc + 16);
+    float2* cs = reinterpret_cast<float2*>(misc + 16 + 3 * B + 1 + ((B + 1) & 1));
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 2);  // the fetched bytes, and the scales
-            mbar_init(&empty[s], kConsumerWarps);
+            mbar_init(&empty[s], kComputeWarps);
         }
         misc[0] = 0;
         fence_mbar_init();
     }
-    if (tid == kConsumers) {
+    if (tid == kCompute) {
         prefetch_tmap(&mk);
         prefetch_tmap(&mv);
         prefetch_tmap(&mk16);
@@ -122,167 +97,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
     griddep_launch_dependents();
     griddep_wait();
 
-    // ---- the line of tiles: lengths and the prefix of the tile counts
-    auto keys_of = [&](int T, int n) { return T + (sp.fused || p.cu_q ? n : 0); };
-    auto groups_of = [&](int n) { return (n * G + COLS - 1) / COLS; };
-    auto tiles_of = [&](int T, int n) { return max(1, (keys_of(T, n) + KEYS - 1) / KEYS); };
-    bool uniform = true;
-    {
-        const int chunk = (B + kThreads - 1) / kThreads, lo = tid * chunk, hi = min(B, lo + chunk);
-        int local = 0, first = -1;
-        for (int b = lo; b < hi; ++b) {
-            const Seq s = seq_of(p, b);
-            if (!s.ok && blockIdx.x == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
-            // a sequence that is not served: its one row gets zeros in decode, none are touched otherwise
-            const int T = s.ok ? s.T : 0, n = s.ok ? s.n : (p.cu_q ? 0 : 1);
-            seqT[b] = s.ok ? s.T : -1;
-            seqN[b] = n;
-            const int cnt = (s.ok ? tiles_of(T, n) : 1) * Hkv * groups_of(n);
-            base[b + 1] = cnt;
-            local += cnt;
-            if (first < 0) first = cnt;
-            if (cnt != first) uniform = false;
-        }
-        int incl = local;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
-        }
-        int* scratch = reinterpret_cast<int*>(red_ml);
-        if (lane == 31) scratch[warp] = incl;
-        if (tid == 0) base[0] = 0, scratch[8] = first;
-        __syncthreads();
-        if (first >= 0 && first != scratch[8]) uniform = false;
-        int run = incl - local;
-        for (int w = 0; w < warp; ++w) run += scratch[w];
-        for (int b = lo; b < hi; ++b) base[b + 1] = run += base[b + 1];
-        uniform = __syncthreads_and(uniform) != 0;
-    }
-    // ---- this CTA's stretch
-    const long long N = base[B];
-    long long CT = N < (long long)gridDim.x ? N : (long long)gridDim.x;
-    if (uniform && N > 0) {
-        // equal units: a number of CTAs that is a multiple of the units keeps every cut at the same
-        // places of each, unless that leaves more than 15 % of the grid idle
-        const long long units = (long long)B * Hkv * groups_of(seqN[0]);
-        if (units <= (long long)gridDim.x) {
-            const long long k = min((long long)gridDim.x / units, N / units);
-            if (20 * units * k >= 17 * CT) CT = units * k;
-        }
-    }
-    long long t0 = 0, t1 = 0;
-    if ((long long)blockIdx.x < CT) {
-        t0 = (long long)blockIdx.x * N / CT;
-        t1 = ((long long)blockIdx.x + 1) * N / CT;
-    }
-    const int ntiles = (int)(t1 - t0);
-    auto enter = [&](Line& x) {
-        x.groups = groups_of(seqN[x.b]);
-        x.tiles = seqT[x.b] < 0 ? 1 : tiles_of(seqT[x.b], seqN[x.b]);
-    };
-    Line at = {0, 0, 0, 0, 1, 1};
-    if (ntiles > 0) {
-        int lo = 0, hi = B - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (base[mid] <= t0) lo = mid;
-            else hi = mid - 1;
-        }
-        at.b = lo;
-        enter(at);
-        int rem = (int)(t0 - base[lo]);
-        at.j = rem % at.tiles;
-        rem /= at.tiles;
-        at.c = rem % at.groups;
-        at.h = rem / at.groups;
-    }
-    auto step = [&](Line& x) {
-        if (++x.j < x.tiles) return;
-        x.j = 0;
-        if (++x.c < x.groups) return;
-        x.c = 0;
-        if (++x.h < Hkv) return;
-        x.h = 0;
-        do ++x.b;
-        while (x.b < B && base[x.b + 1] == base[x.b]);
-        if (x.b < B) enter(x);
-    };
-    auto keys_at = [&](const Line& x) { return seqT[x.b] < 0 ? 0 : keys_of(seqT[x.b], seqN[x.b]); };
-
+    At at = line.template build<kThreads>(reinterpret_cast<int*>(red_ml));
+    const int ntiles = line.ntiles;
+    const int* seqT = line.T;
+    const int* seqN = line.n;
     const int box = min(p.page, KEYS);  // rows of one page in a tile
-    const int boxes = KEYS / box;
-    if (warp == kConsumerWarps) {
-        // ============================================================ fetching warp
-        const uint64_t pol = l2_policy_evict_first();
-        const bool is_v = lane >= 16;
-        const int slot = lane & 15;  // page box of this lane, of K (lanes 0..) or V (lanes 16..)
-        auto rows_at = [&](const Line& x) {
-            return slot < boxes ? max(0, min(box, keys_at(x) - x.j * KEYS - slot * box)) : 0;
-        };
-        auto page_at = [&](const Line& x) {
-            if (rows_at(x) == 0) return -1;
-            return p.table[(int64_t)x.b * p.table_st + ((x.j * KEYS + slot * box) >> p.page_log2)];
-        };
-        int pid = ntiles > 0 ? page_at(at) : -1;
-        float sc = 0.f;
-        int it = 0;
-        auto publish = [&](int i, float v) {  // scales of tile i, then its second arrival
-            if (slot < boxes) scale_sm[(i % S) * 16 + (is_v ? 8 : 0) + slot] = v;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[i % S]);
-        };
-        for (; it < ntiles; ++it) {
-            const int s = it % S;
-            const int rows = rows_at(at), h = at.h;
-            const int row0 = (at.j * KEYS + slot * box) & (p.page - 1);
-            const bool there = rows > 0 && (unsigned)pid < (unsigned)p.num_pages;
-            if (rows > 0 && !there) set_error(p, FCCI_DEV_ERR_PAGE);
-            const int id = there ? pid : 0;
-            step(at);
-            const int pid_next = it + 1 < ntiles ? page_at(at) : -1;
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ((uint32_t)(it / S) & 1u) ^ 1u, abort_flag, kWaitLimitNs))) {
-                if (lane == 0) {
-                    *abort_flag = 1;
-                    set_error(p, FCCI_DEV_ERR_TIMEOUT);
-                }
-                break;
-            }
-            const int fetched = !there ? 0 : rows == box ? box : (rows + 15) & ~15;
-            const uint32_t bytes = __reduce_add_sync(0xffffffffu, (unsigned)(fetched * C::ROWB));
-            if (lane == 0) mbar_arrive_expect_tx(&full[s], bytes);
-            __syncwarp();
-            if (there) {
-                uint8_t* dst = tiles_sm + (size_t)s * 2 * C::TILE + (is_v ? C::TILE : 0) + slot * box * PITCH;
-                const CUtensorMap* m = is_v ? &mv : &mk;
-                const CUtensorMap* m16 = is_v ? &mv16 : &mk16;
-#pragma unroll
-                for (int k = 0; k < C::BLOCKS; ++k) {
-                    const int col = k * PITCH / (E4M3 ? 1 : 2);
-                    if (rows == box) {
-                        tma_load_4d(dst + k * KEYS * PITCH, m, col, row0, h, id, &full[s], pol);
-                    } else {
-                        for (int r = 0; r < fetched; r += 16)
-                            tma_load_4d(dst + k * KEYS * PITCH + r * PITCH, m16, col, row0 + r, h, id, &full[s], pol);
-                    }
-                }
-            }
-            float next = there ? 1.f : -1.f;
-            if (E4M3 && there) {
-                const uint8_t* a = is_v ? p.v_scales + id * p.vs_sp + h * p.vs_sh : p.k_scales + id * p.ks_sp + h * p.ks_sh;
-                next = exp2_int((int)*a - 127);
-            }
-            if (it > 0) publish(it - 1, sc);
-            sc = next;
-            pid = pid_next;
-        }
-        if (it > 0) publish(it - 1, sc);
-        if (*abort_flag) {
-            // let copies still in flight land before the CTA can exit
-            volatile int never = 0;
-            for (int i = max(0, it - S); i < it; ++i)
-                mbar_wait_bounded(&full[i % S], (uint32_t)(i / S) & 1u, &never, kDrainLimitNs);
-        }
+    if (warp == kComputeWarps) {
+        fetch_tiles<TL, E4M3, COLS>(line, at, &mk, &mv, &mk16, &mv16, tiles_sm, full, empty, scale_sm, abort_flag);
     } else {
         // ============================================================ computing warps
         const int w = warp, g = lane >> 2, t4 = lane & 3;
@@ -294,13 +115,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
         int cs_b = -1, cs_c = -1;
         bool fresh = true;
         int first_tile = at.j;
-        // address of 16-byte chunk ch of row r in a K or V tile
-        auto cell = [&](uint32_t tile, int r, int ch) {
-            const int blk = ch / CHUNKS, c = ch % CHUNKS;
-            const int sw = PITCH == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
-            return tile + blk * KEYS * PITCH + r * PITCH + sw * 16;
-        };
-
+        auto cell = [](uint32_t tile, int r, int ch) { return TL::cell(tile, r, ch); };
         // B fragment of k step kk: e4m3 lanes hold 4 neighbouring dims of a chunk, and k follows them
         auto q_fragment = [&](int part, int nb, int kk, uint32_t(&r)[2]) {
             const __half* q = (part ? q_lo : q_hi) + (nb * 8 + g) * QP + 16 * kk + (E4M3 ? 4 * t4 : 2 * t4);
@@ -319,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
         };
 
         for (int it = 0; it < ntiles; ++it) {
-            const int T = seqT[at.b], n = seqN[at.b], L = keys_at(at);
+            const int T = seqT[at.b], n = seqN[at.b], L = line.keys_at(at);
             const int r0 = at.c * COLS, rows = min(COLS, n * G - r0);  // query rows of this unit
             if (fresh) {
                 fresh = false;
@@ -327,15 +142,15 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                 const int i0 = r0 / G;  // first token of the unit
                 if (rot > 0 && (cs_b != at.b || cs_c != at.c)) {
                     const int ntok = (r0 + rows - 1) / G - i0 + 1;
-                    for (int x = tid; x < ntok * half; x += kConsumers)
+                    for (int x = tid; x < ntok * half; x += kCompute)
                         cs[x] = rope_cs(f.turn[x % half], max(T, 0) + i0 + x / half);
                     cs_b = at.b, cs_c = at.c;
-                    named_bar_sync(kBar, kConsumers);
+                    named_bar_sync(kBar, kCompute);
                 }
                 // rotated queries, fp32, as hi + lo
                 const int64_t tok0 = p.cu_q ? p.cu_q[at.b] : at.b;
 #pragma unroll 4
-                for (int e = tid * 2; e < COLS * D; e += 2 * kConsumers) {
+                for (int e = tid * 2; e < COLS * D; e += 2 * kCompute) {
                     const int c = e / D, d = e - c * D;
                     float x0 = 0.f, x1 = 0.f;
                     if (c < rows) {
@@ -358,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                     *reinterpret_cast<__half2*>(q_hi + c * QP + d) = hi;
                     *reinterpret_cast<__half2*>(q_lo + c * QP + d) = __floats2half2_rn(x0 - back.x, x1 - back.y);
                 }
-                named_bar_sync(kBar, kConsumers);
+                named_bar_sync(kBar, kCompute);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -379,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                     }
                 }
                 // the query rows may lie in the joining buffer, which a faster warp writes next
-                if (C::QREG) named_bar_sync(kBar, kConsumers);
+                if (C::QREG) named_bar_sync(kBar, kCompute);
             }
 
             const int s = it % S;
@@ -394,76 +209,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
             bool wrote = false;
             if (sp.fused && T >= 0 && T / KEYS == at.j) {
                 // ---- append: warp 0 the key, warp 1 the value, into the tile and the page
-                named_bar_sync(kBar, kConsumers);
-                if (ready && w < 2 && ksc[(T % KEYS) / box] >= 0.f) {
-                    constexpr int E = D / 32;
-                    const bool is_v = w == 1;
-                    const int d0 = lane * E, r = T % KEYS, off = T & (p.page - 1);
-                    const __half* src = is_v ? p.v_new + at.b * p.vn_st + at.h * p.vn_sh : p.k_new + at.b * p.kn_st + at.h * p.kn_sh;
-                    float x[E];
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        x[e] = __half2float(src[d0 + e]);
-                        if (!is_v && d0 < rot) {
-                            const bool lowhalf = d0 < half;
-                            const int k = (lowhalf ? d0 : d0 - half) + e;
-                            x[e] = rotated(x[e], __half2float(src[lowhalf ? k + half : k]), cs[k], lowhalf);
-                        }
-                    }
-                    const int id = p.table[(int64_t)at.b * p.table_st + (T >> p.page_log2)];
-                    uint8_t* page = is_v ? p.v_pages + id * p.v_sp + at.h * p.v_sh : p.k_pages + id * p.k_sp + at.h * p.k_sh;
-                    const int64_t st = is_v ? p.v_st : p.k_st;
-                    uint8_t* tile = tiles_sm + (size_t)s * 2 * C::TILE + (is_v ? C::TILE : 0);
-                    const uint32_t t32 = smem_u32(tile);
-                    auto in_tile = [&](int row, int byte) { return tile + (cell(t32, row, byte >> 4) - t32) + (byte & 15); };
-                    if constexpr (!E4M3) {
-#pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const uint32_t v = pack_half2(x[e], x[e + 1]);
-                            *reinterpret_cast<uint32_t*>(page + off * st + (d0 + e) * 2) = v;
-                            *reinterpret_cast<uint32_t*>(in_tile(r, (d0 + e) * 2)) = v;
-                        }
-                    } else {
-                        float* slot = ksc + (is_v ? 8 : 0) + r / box;
-                        const float had = *slot;
-                        float amax = 0.f;
-#pragma unroll
-                        for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[e]));
-#pragma unroll
-                        for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                        float scale = exp2_int(scale_exponent(amax));
-                        if (off && had >= scale) {
-                            scale = had;
-                        } else if (off) {
-                            // the rows before take the larger scale, in the tile and in the page
-                            const float down = had / scale;
-                            for (int i = lane; i < off * (D / 4); i += 32) {
-                                const int row = i / (D / 4), byte = (i % (D / 4)) * 4;
-                                uint32_t* a = reinterpret_cast<uint32_t*>(in_tile(r - off + row, byte));
-                                const uint32_t lo2 = half2_of_e4m3x2(*a & 0xffffu), hi2 = half2_of_e4m3x2(*a >> 16);
-                                const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&lo2));
-                                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hi2));
-                                *a = e4m3x2(u.x * down, u.y * down) | (e4m3x2(v.x * down, v.y * down) << 16);
-                                *reinterpret_cast<uint32_t*>(page + row * st + byte) = *a;
-                            }
-                        }
-                        const float up = 1.f / scale;  // a power of two: exact
-#pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const uint16_t v = (uint16_t)e4m3x2(x[e] * up, x[e + 1] * up);
-                            *reinterpret_cast<uint16_t*>(page + off * st + d0 + e) = v;
-                            *reinterpret_cast<uint16_t*>(in_tile(r, d0 + e)) = v;
-                        }
-                        __syncwarp();
-                        if (lane == 0) {
-                            *slot = scale;
-                            uint8_t* b8 = is_v ? p.v_scales + id * p.vs_sp + at.h * p.vs_sh : p.k_scales + id * p.ks_sp + at.h * p.ks_sh;
-                            *b8 = (uint8_t)(__float_as_uint(scale) >> 23);
-                        }
-                    }
-                }
+                named_bar_sync(kBar, kCompute);
+                const int bx = (T % KEYS) / box;
+                if (ready && w < 2 && ksc[bx] >= 0.f)
+                    append_in_tile<TL, D, E4M3>(p, at.b, at.h, T, w == 1, cs, tiles_sm + (size_t)s * 2 * C::TILE + (w ? C::TILE : 0),
+                                                ksc + 8 * w + bx);
                 wrote = true;
-                named_bar_sync(kBar, kConsumers);
+                named_bar_sync(kBar, kCompute);
             }
             const int key0 = KEYS * at.j + 16 * MT * w;
             if (ready && key0 < L) {
@@ -674,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                                 }
                         }
                     }
-                    named_bar_sync(kBar, kConsumers);
+                    named_bar_sync(kBar, kCompute);
                     if (w < far) {
                         const float* src = red + w * COLS * RP;
 #pragma unroll
@@ -699,21 +451,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                                 }
                         }
                     }
-                    if (far == 2) named_bar_sync(kBar, kConsumers);
+                    if (far == 2) named_bar_sync(kBar, kCompute);
                 }
                 // warp 0 holds the joined state: the result, or this CTA's part of it
-                const long long unit0 = base[at.b] + ((long long)at.h * at.groups + at.c) * at.tiles;
-                // CTA that holds tile t of the line: ceil((t + 1) CT / N) - 1
-                const int ca = (int)(((unit0 + 1) * CT + N - 1) / N - 1);
-                const int cb = (int)(((unit0 + at.tiles) * CT + N - 1) / N - 1);
-                const bool whole = ca == cb;
-                const int64_t tok0 = p.cu_q ? p.cu_q[at.b] : at.b;
-                auto out_row = [&](int c) {
-                    const int i = (r0 + c) / G;
-                    return p.out + (tok0 + i) * p.o_st + (int64_t)(at.h * G + (r0 + c) - i * G) * p.o_sh;
-                };
+                const int2 ctas = line.ctas_of(at);
+                const bool whole = ctas.x == ctas.y;
                 if (w == 0) {
-                    const size_t part = 2 * (size_t)blockIdx.x + (first_tile == 0 ? 1 : 0);
+                    const size_t part = part_slot(blockIdx.x, first_tile == 0);
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -721,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                             const int c = nb * 8 + 2 * t4 + k;
                             if (c >= rows) continue;
                             const float inv = l[nb][k] > 0.f ? 1.f / l[nb][k] : 0.f;
-                            __half* o16 = out_row(c);
+                            __half* o16 = out_row(p, at, r0, c);
                             float* o32 = sp.part_o + (part * kMaxCols + c) * D;
                             if (!whole && g == 0)
                                 sp.part_lse[part * kMaxCols + c] = l[nb][k] > 0.f ? m[nb][k] + __log2f(l[nb][k]) : -INFINITY;
@@ -743,55 +487,18 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                             }
                         }
                 }
-                if (!whole) {
-                    // the last part to arrive joins them. Release: the barrier orders warp 0's stores
-                    // before thread 0's fence and count; acquire: its fence after the count.
-                    // The counter is that of the unit's first CTA, where no other cut unit begins.
-                    named_bar_sync(kBar, kConsumers);
-                    if (tid == 0) {
-                        __threadfence();
-                        misc[1] = atomicAdd(&sp.cut_cnt[ca], 1u) == (unsigned)(cb - ca);
-                        if (misc[1]) __threadfence();
-                    }
-                    named_bar_sync(kBar, kConsumers);
-                    if (misc[1]) {
-                        const int parts = cb - ca + 1;
-                        for (int e = tid * 4; e < rows * D; e += 4 * kConsumers) {
-                            const int c = e / D, d = e - c * D;
-                            float M = -INFINITY, W = 0.f;
-                            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                            for (int i = 0; i < parts; ++i) {
-                                const size_t part = 2 * (size_t)(ca + i) + (i == 0 ? 1 : 0);
-                                const float lse = __ldcg(sp.part_lse + part * kMaxCols + c);
-                                const float4 y = __ldcg(reinterpret_cast<const float4*>(sp.part_o + (part * kMaxCols + c) * D + d));
-                                const float mn = fmaxf(M, lse), mu = mn == -INFINITY ? 0.f : mn;
-                                const float a = ex2(M - mu), u = ex2(lse - mu);
-                                W = W * a + u;
-                                o.x = o.x * a + y.x * u, o.y = o.y * a + y.y * u;
-                                o.z = o.z * a + y.z * u, o.w = o.w * a + y.w * u;
-                                M = mn;
-                            }
-                            const float inv = W > 0.f ? 1.f / W : 0.f;
-                            uint2 v;
-                            v.x = pack_half2(o.x * inv, o.y * inv);
-                            v.y = pack_half2(o.z * inv, o.w * inv);
-                            *reinterpret_cast<uint2*>(out_row(c) + d) = v;
-                        }
-                        if (tid == 0) atomicExch(&sp.cut_cnt[ca], 0u);
-                    }
-                }
-                named_bar_sync(kBar, kConsumers);  // the joining buffer becomes the next unit's queries
+                if (!whole) join_parts<D>(sp, at, r0, rows, ctas.x, ctas.y, misc + 1);
+                named_bar_sync(kBar, kCompute);  // the joining buffer becomes the next unit's queries
                 fresh = true;
             }
-            step(at);
+            line.step(at);
         }
     }
     advance_lengths(p, misc + 2);
 }
 
 template <int D, int NB, bool E4M3>
-static int launch_split_t(SplitParams& sp, const Freqs& f, int sms, int dev, cudaStream_t st) {
+static int launch_split_t(TileParams& sp, const Freqs& f, int sms, int dev, cudaStream_t st) {
     using C = Cfg<D, NB, E4M3>;
     const Params& p = sp.p;
     static std::once_flag once[128];
@@ -809,17 +516,9 @@ static int launch_split_t(SplitParams& sp, const Freqs& f, int sms, int dev, cud
             if (C::smem(s, p.B, rope_rows, p.rot) <= (size_t)(228 * 1024 / ctas - 1024)) stages = s, per_sm = ctas;
     if (!stages) return set_status(FCCI_EUNSUPPORTED, "paged attention: batch too large for shared memory");
     sp.stages = stages;
-    const int elt = E4M3 ? 1 : 2;
     CUtensorMap m[4];
-    int rc = 0;
-    for (int i = 0; i < 4 && !rc; ++i) {
-        const bool v = i & 1;
-        const uint64_t dims[4] = {(uint64_t)D, (uint64_t)p.page, (uint64_t)p.Hkv, (uint64_t)p.num_pages};
-        const int64_t sb[3] = {v ? p.v_st : p.k_st, v ? p.v_sh : p.k_sh, v ? p.v_sp : p.k_sp};
-        const uint32_t box[4] = {(uint32_t)(C::PITCH / elt), (uint32_t)(i < 2 ? (p.page < C::KEYS ? p.page : C::KEYS) : 16), 1, 1};
-        rc = encode_tiled(&m[i], E4M3, C::PITCH == 64, v ? p.v_pages : p.k_pages, 4, dims, sb, box);
-    }
-    if (rc) return set_status(rc, "paged attention: cuTensorMapEncodeTiled rejected the page layout");
+    const int rc = encode_pages<typename C::TL, E4M3>(p, m);
+    if (rc) return rc;
     const size_t smem = C::smem(stages, p.B, rope_rows, p.rot);
     return launch_pdl(paged_split_kernel<D, NB, E4M3>, dim3(sms * per_sm), dim3(kThreads), smem, st, m[0], m[1], m[2], m[3], sp, f);
 }
@@ -828,7 +527,7 @@ int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, uint8_t
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
     const int sms = device_sm_count(dev);
-    SplitParams sp;
+    TileParams sp;
     sp.p = p;
     sp.fused = fused;
     sp.stages = 0;
@@ -836,6 +535,8 @@ int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, uint8_t
     sp.part_lse = reinterpret_cast<float*>(ws + L.part_lse);
     sp.part_o = reinterpret_cast<float*>(ws + L.part_o);
     if (sms * kMaxCtasPerSm > kMaxGrid) return set_status(FCCI_EUNSUPPORTED, "paged attention: too many SMs");
+    // e4m3 pages of head_dim 128 go to the tensor memory kernel: 41 against 69 us at batch 32 x 4096 keys
+    if (e4m3 && p.D == 128) return launch_split_tc(sp, f, sms, dev, st);
     const int nb = (int64_t)p.max_q * p.G <= 8 || p.D == 256 ? 1 : 2;
     switch ((p.D * 10 + nb) * 2 + (e4m3 ? 1 : 0)) {
         case 1282: return launch_split_t<64, 1, false>(sp, f, sms, dev, st);
@@ -843,9 +544,7 @@ int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, uint8_t
         case 1284: return launch_split_t<64, 2, false>(sp, f, sms, dev, st);
         case 1285: return launch_split_t<64, 2, true>(sp, f, sms, dev, st);
         case 2562: return launch_split_t<128, 1, false>(sp, f, sms, dev, st);
-        case 2563: return launch_split_t<128, 1, true>(sp, f, sms, dev, st);
         case 2564: return launch_split_t<128, 2, false>(sp, f, sms, dev, st);
-        case 2565: return launch_split_t<128, 2, true>(sp, f, sms, dev, st);
         case 5122: return launch_split_t<256, 1, false>(sp, f, sms, dev, st);
         case 5123: return launch_split_t<256, 1, true>(sp, f, sms, dev, st);
         default: return set_status(FCCI_EUNSUPPORTED, "paged attention: unsupported head_dim");

@@ -1,0 +1,488 @@
+// Split-KV attention over e4m3 pages of head_dim 128 on the 5th-generation tensor cores: one new token per
+// sequence (its append fused in), or a few of them whose rows an append has written already.
+// Work and fetching: paged_tiles.cuh, tiles of 128 keys.
+//
+// The e4m3 codes go into tcgen05 (kind::f8f6f4, fp32 sums) as they lie in shared memory. With mma.sync they would
+// have to become fp16 in registers first, and that conversion unit (16 lanes a cycle and SM, for 2 codes each)
+// bound that kernel at 59 % of the memory rate. The other operand keeps its precision as a sum of
+// three e4m3 values, each the rounding of what the ones before left (within 2^-12 of it), as three rows of the
+// same product:
+//   S^T[key, (part, row)] = K Q^T     A = the K tile (128 keys), B = 3 * COLS rows of query parts
+//   O^T[dim, (part, row)] += V^T P^T  A = the V tile read dim-major, B = 3 * COLS rows of weight parts
+// The parts are summed where S is read, and where O is read at a unit's end.
+//   - A query row is rotated in fp32 and scaled by a power of two to at most 448 before it is split.
+//   - Thread t of the softmax owns key t of the tile: its scales are its own numbers. The exponent of V's scale
+//     joins the score, x = s + log2 vs, so the weight that multiplies the codes is 2^(x - m), and no
+//     scale can push it out of range; the sum l takes 2^(x - m) / vs, the weight of the value itself.
+//   - m moves only when a weight would exceed 2^8.75 (448 is the largest e4m3), to leave the largest at 2^6: O in
+//     tensor memory is scaled rarely, and four warps agree on it with one barrier a tile.
+//
+// 192 threads: warps 0..3 softmax (TMEM lane t = key t, then dim t), warp 4 fetches, warp 5 issues the products.
+// TMEM: two S tiles and O, 3 * COLS columns each (24 or 48, in strides of 32 or 64).
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <mutex>
+
+#include "paged_tiles.cuh"
+#include "tcgen05.cuh"
+
+namespace fcci {
+namespace pg {
+
+constexpr int kTcThreads = kCompute + 64;
+constexpr int kTcD = 128, kTcKeys = 128;
+constexpr float kWeightTop = 6.f, kWeightMost = 8.75f;  // log2 of the largest weight after a move of m, and at most
+constexpr float kNoMax = -1e30f;                         // m before a row has seen a key
+
+template <int NB>
+struct TcCfg {
+    using TL = Tile<kTcKeys, kTcD>;
+    static constexpr int COLS = 8 * NB;
+    static constexpr int N = NB == 1 ? 32 : 48;         // rows of a B operand: 3 * COLS, a multiple of 16
+    static constexpr int STRIDE = NB == 1 ? 32 : 64;    // TMEM columns of one accumulator
+    static constexpr int TMEM = NB == 1 ? 128 : 256;
+    static constexpr int QB = N * 128;                  // bytes of a B operand
+    // shared memory behind the stages
+    static constexpr int kP = QB, kSmall = 3 * QB;      // queries, two weight buffers, the rest
+    static size_t smem(int stages, int B) {
+        return 1024 + (size_t)stages * 2 * TL::BYTES + kSmall + 64 * 8 /* cos, sin */ + 8 * COLS * 4 /* maxima, sums */ +
+               COLS * 4 /* query scales */ + kMaxStages * 64 /* page scales */ + 256 /* barriers */ + 64 +
+               Line<kTcKeys, COLS>::ints(B) * 4;
+    }
+};
+
+struct Bars {  // mbarriers: fetched / freed stages; S written / read; P written / consumed; queries ready; row appended
+    uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], s_free[2], p_full[2], p_free[2], q_full, row_done, drain;
+};
+static_assert(sizeof(Bars) <= 256, "barrier area");
+
+__device__ __forceinline__ float redux_max(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Whether any of the computing threads says so (all of them take part).
+__device__ __forceinline__ bool any_of_compute(bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)x), "n"(kBar), "n"(kCompute)
+        : "memory");
+    return r != 0;
+}
+
+template <int NB>
+__global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __grid_constant__ CUtensorMap mk,
+                                                                   const __grid_constant__ CUtensorMap mv,
+                                                                   const __grid_constant__ CUtensorMap mk16,
+                                                                   const __grid_constant__ CUtensorMap mv16,
+                                                                   const __grid_constant__ TileParams tp,
+                                                                   const __grid_constant__ Freqs f) {
+    using C = TcCfg<NB>;
+    using TL = typename C::TL;
+    constexpr int D = kTcD, KEYS = kTcKeys, COLS = C::COLS;
+    const Params& p = tp.p;
+    extern __shared__ uint8_t raw[];
+    uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const int S = tp.stages, G = p.G;
+    uint8_t* rest = sm + (size_t)S * 2 * TL::BYTES;
+    uint8_t* q_sm = rest;             // [N rows][128 bytes], 128-byte swizzle
+    uint8_t* p_sm = rest + C::kP;     // two of the same
+    float2* cs = reinterpret_cast<float2*>(rest + C::kSmall);  // decode: cos and sin of position T
+    float* mx_sm = reinterpret_cast<float*>(cs + 64);          // [4][COLS] maxima, then sums
+    float* l_sm = mx_sm + 4 * COLS;
+    float* qs_sm = l_sm + 4 * COLS;
+    float* scale_sm = qs_sm + COLS;                            // [stage][K, V][8]
+    Bars* bar = reinterpret_cast<Bars*>(scale_sm + kMaxStages * 16);
+    int* misc = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bar) + 256);
+    volatile int* abort_flag = misc;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + 3);
+    Line<KEYS, COLS> line(tp, misc + 16);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&bar->full[s], 2);  // the fetched bytes, and the scales
+            mbar_init(&bar->empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar->s_full[i], 1);
+            mbar_init(&bar->s_free[i], kComputeWarps);
+            mbar_init(&bar->p_full[i], kComputeWarps);
+            mbar_init(&bar->p_free[i], 1);
+        }
+        mbar_init(&bar->q_full, kComputeWarps);
+        mbar_init(&bar->row_done, kComputeWarps);
+        mbar_init(&bar->drain, 1);
+        misc[0] = 0;
+        fence_mbar_init();
+    }
+    if (warp == 4 && lane == 0) {
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
+        prefetch_tmap(&mk16);
+        prefetch_tmap(&mv16);
+    }
+    if (warp == 5) {
+        tc::tmem_alloc(tmem_slot, C::TMEM);
+        tc::tmem_relinquish();
+    }
+    griddep_launch_dependents();
+    griddep_wait();
+    tc::fence_before_sync();
+    At at = line.template build<kTcThreads>(reinterpret_cast<int*>(mx_sm));  // barriers inside
+    tc::fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem_o = tmem + 2 * C::STRIDE;
+    const int ntiles = line.ntiles;
+    auto fail = [&]() {
+        *abort_flag = 1;
+        set_error(p, FCCI_DEV_ERR_TIMEOUT);
+    };
+    auto wait = [&](uint64_t* b, uint32_t parity) {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(b, parity & 1u, abort_flag, kWaitLimitNs));
+        if (!ok && !*abort_flag) fail();
+        return ok;
+    };
+    // the append of row T happens in the tile that holds it
+    auto appends = [&](const At& x) { return tp.fused && line.T[x.b] >= 0 && line.T[x.b] / KEYS == x.j; };
+
+    if (warp == 4) {
+        fetch_tiles<TL, true, COLS>(line, at, &mk, &mv, &mk16, &mv16, sm, bar->full, bar->empty, scale_sm, abort_flag);
+    } else if (warp == 5) {
+        // ============================================================ products
+        const uint32_t id_s = tc::idesc_e4m3_f32(128, C::N, 0, 0);
+        const uint32_t id_o = tc::idesc_e4m3_f32(128, C::N, 1, 0);
+        const uint64_t qd = tc::smem_desc_sw128(smem_u32(q_sm), 16, 1024);
+        int nrow = 0, nq = 0;
+        bool begins_prev = false;  // tile it - 1 is its unit's first here
+        // O += V^T P of tile i (begins: O = V^T P)
+        auto issue_o = [&](int i, bool begins) {
+            if (!wait(&bar->p_full[i & 1], i >> 1)) return false;
+            tc::fence_after_sync();
+            if (lane == 0) {
+                const uint64_t vd = tc::smem_desc_sw128(smem_u32(sm + (size_t)(i % S) * 2 * TL::BYTES + TL::BYTES), TL::BYTES, 1024);
+                const uint64_t pd = tc::smem_desc_sw128(smem_u32(p_sm + (i & 1) * C::QB), 16, 1024);
+#pragma unroll
+                for (int k = 0; k < KEYS / 32; ++k)  // 32 keys: 4 groups of 8 rows of V, 32 bytes of a row of P
+                    tc::mma_ss_f8(tmem_o, vd + (uint64_t)(k * 4096 >> 4), pd + (uint64_t)(k * 32 >> 4), id_o, !begins || k > 0);
+                tc::commit(&bar->p_free[i & 1]);
+                tc::commit(&bar->empty[i % S]);
+            }
+            __syncwarp();
+            return true;
+        };
+        bool ok = true;
+        for (int it = 0; it < ntiles && ok; ++it) {
+            const bool begins = it == 0 || at.j == 0;
+            if (begins) {
+                // the queries of the new unit come only after the last one's O was read, which needs its last product
+                if (it > 0 && !(ok = issue_o(it - 1, begins_prev))) break;
+                if (!(ok = wait(&bar->q_full, nq++))) break;
+            }
+            if (!(ok = wait(&bar->full[it % S], it / S))) break;
+            if (appends(at) && !(ok = wait(&bar->row_done, nrow++))) break;
+            if (it >= 2 && !(ok = wait(&bar->s_free[it & 1], (it >> 1) - 1))) break;
+            tc::fence_after_sync();
+            if (lane == 0) {
+                const uint64_t kd = tc::smem_desc_sw128(smem_u32(sm + (size_t)(it % S) * 2 * TL::BYTES), 16, 1024);
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k)
+                    tc::mma_ss_f8(tmem + (it & 1) * C::STRIDE, kd + (uint64_t)(k * 32 >> 4), qd + (uint64_t)(k * 32 >> 4), id_s, k > 0);
+                tc::commit(&bar->s_full[it & 1]);
+            }
+            __syncwarp();
+            if (!begins && !(ok = issue_o(it - 1, begins_prev))) break;
+            begins_prev = begins;
+            line.step(at);
+        }
+        if (ok && ntiles > 0) issue_o(ntiles - 1, begins_prev);
+        // every product has completed before TMEM is released
+        if (lane == 0) {
+            tc::commit(&bar->drain);
+            volatile int never = 0;
+            mbar_wait_bounded(&bar->drain, 0, &never, kDrainLimitNs);
+        }
+        __syncwarp();
+    } else {
+        // ============================================================ softmax
+        // A wait that fails leaves garbage behind, never a barrier that some warps skip: the loop runs on, its
+        // waits return at once, and the error word says so.
+        const uint32_t lane_row = (uint32_t)warp * 32;
+        const int rot = p.rot, half = rot >> 1;
+        const int box_log2 = min(p.page_log2, 7);
+        float mm[COLS], l[COLS], qf[COLS];  // m - kWeightTop, sum, factor of a score
+        bool fresh = true;
+        int first_tile = 0;
+        for (int it = 0; it < ntiles; ++it) {
+            const int T = line.T[at.b], n = line.n[at.b], L = line.keys_at(at);
+            const int r0 = at.c * COLS, rows = min(COLS, n * G - r0);
+            if (fresh) {
+                first_tile = at.j;
+                // ---- queries: warp w takes rows w, w + 4, ...; a lane 4 neighbouring dims
+                if (!p.cu_q && rot > 0) {
+                    if (tid < half) cs[tid] = rope_cs(f.turn[tid], max(T, 0));
+                    named_bar_sync(kBar, kCompute);
+                }
+                const int64_t tok0 = p.cu_q ? p.cu_q[at.b] : at.b;
+                const int d = 4 * lane;
+                uint2 xr[COLS / 4], yr[COLS / 4];
+#pragma unroll
+                for (int k = 0; k < COLS / 4; ++k) {
+                    const int c = 4 * k + warp, i = (r0 + c) / G;
+                    xr[k] = yr[k] = make_uint2(0, 0);
+                    if (c < rows) {
+                        const __half* q = p.q + (tok0 + i) * p.q_st + (at.h * G + (r0 + c) - i * G) * p.q_sh;
+                        xr[k] = *reinterpret_cast<const uint2*>(q + d);
+                        if (d < rot) yr[k] = *reinterpret_cast<const uint2*>(q + (d < half ? d + half : d - half));
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < COLS / 4; ++k) {
+                    const int c = 4 * k + warp, i = (r0 + c) / G;
+                    const __half* a = reinterpret_cast<const __half*>(&xr[k]);
+                    const __half* y = reinterpret_cast<const __half*>(&yr[k]);
+                    float x[4], amax = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[e] = __half2float(a[e]);
+                        if (d < rot && c < rows) {
+                            const int t = (d < half ? d : d - half) + e;
+                            const float2 w = p.cu_q ? rope_cs(f.turn[t], T + i) : cs[t];
+                            x[e] = rotated(x[e], __half2float(y[e]), w, d < half);
+                        }
+                        amax = fmaxf(amax, fabsf(x[e]));
+                    }
+                    if (p.q_rot && at.j == 0 && c < rows)
+                        *reinterpret_cast<uint2*>(p.q_rot + ((tok0 + i) * p.Hq + at.h * G + (r0 + c) - i * G) * D + d) =
+                            make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+                    const int e = exponent_448(redux_max(amax), -100, 100);
+                    const float up = exp2_int(-e);
+                    if (lane == 0) qs_sm[c] = exp2_int(e) * p.scale_log2;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] *= up;
+#pragma unroll
+                    for (int part = 0; part < 3; ++part) {
+                        const uint32_t lo = e4m3x2(x[0], x[1]), hi = e4m3x2(x[2], x[3]);
+                        const int r = part * COLS + c;
+                        *reinterpret_cast<uint32_t*>(q_sm + r * 128 + ((lane >> 2) ^ (r & 7)) * 16 + (d & 15)) = lo | (hi << 16);
+                        const uint32_t bl = half2_of_e4m3x2(lo), bh = half2_of_e4m3x2(hi);
+                        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&bl));
+                        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&bh));
+                        x[0] -= u.x, x[1] -= u.y, x[2] -= v.x, x[3] -= v.y;
+                    }
+                }
+                fence_proxy_async_smem();
+                tc::fence_before_sync();  // O of the unit before was read
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->q_full);
+                named_bar_sync(kBar, kCompute);  // the scales of the query rows
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) {
+                    mm[c] = kNoMax;
+                    l[c] = 0.f;
+                    qf[c] = qs_sm[c];
+                }
+            }
+            const int s = it % S;
+            uint8_t* kt = sm + (size_t)s * 2 * TL::BYTES;
+            float* scales = scale_sm + s * 16;
+            const bool ready = wait(&bar->full[s], it / S);
+            if (appends(at)) {
+                // ---- warp 0 the key, warp 1 the value, before the tile's first product
+                const int bx = (T & (KEYS - 1)) >> box_log2;
+                if (ready && warp < 2 && scales[bx] >= 0.f)
+                    append_in_tile<TL, D, true>(p, at.b, at.h, T, warp == 1, cs, kt + (warp ? TL::BYTES : 0), scales + 8 * warp + bx);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->row_done);
+                named_bar_sync(kBar, kCompute);  // the scales that it changed
+            }
+            // ---- this thread's key: its scales, whether it is there; values that are not are zeroed, since 0 * NaN
+            const int t = at.j * KEYS + tid, bx = tid >> box_log2;
+            const float ks = scales[bx], vs = scales[8 + bx];
+            const bool live = t < L && ks >= 0.f;
+            if (!live) {
+                const uint32_t v32 = smem_u32(kt + TL::BYTES);
+#pragma unroll
+                for (int ch = 0; ch < 8; ++ch)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(TL::cell(v32, tid, ch)), "r"(0) : "memory");
+            }
+            const float lv = live ? (float)((int)(__float_as_uint(vs) >> 23) - 127) : -INFINITY;
+            const float inv_vs = live ? 1.f / vs : 0.f;
+            const float k2 = live ? ks : 0.f;
+            // ---- scores of this key, in the log2 domain, with V's exponent
+            wait(&bar->s_full[it & 1], it >> 1);
+            tc::fence_after_sync();
+            float x[COLS];
+            {
+                uint32_t a[C::N];
+                tc::ld32(tc::taddr(tmem, lane_row, (it & 1) * C::STRIDE), *reinterpret_cast<uint32_t(*)[32]>(a));
+                if constexpr (C::N == 48) tc::ld16(tc::taddr(tmem, lane_row, (it & 1) * C::STRIDE + 32), *reinterpret_cast<uint32_t(*)[16]>(a + 32));
+                tc::wait_ld();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->s_free[it & 1]);
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) {
+                    const float sum = __uint_as_float(a[c]) + (__uint_as_float(a[COLS + c]) + __uint_as_float(a[2 * COLS + c]));
+                    x[c] = live ? fmaf(sum * k2, qf[c], lv) : -INFINITY;
+                }
+            }
+            if (p.cu_q && (at.j + 1) * KEYS > T) {  // a row sees the keys up to its own position
+#pragma unroll
+                for (int c = 0; c < COLS; ++c)
+                    if (t > T + (r0 + c) / G) x[c] = -INFINITY;
+            }
+            // ---- move m when a weight would leave e4m3's range
+            bool over = false;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) over = over || x[c] - mm[c] > kWeightMost;
+            if (any_of_compute(over)) {
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) {
+                    const float top = redux_max(x[c]);
+                    if (lane == 0) mx_sm[warp * COLS + c] = top;
+                }
+                named_bar_sync(kBar, kCompute);
+                float alpha[COLS];
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) {
+                    const float top = fmaxf(fmaxf(mx_sm[c], mx_sm[COLS + c]), fmaxf(mx_sm[2 * COLS + c], mx_sm[3 * COLS + c]));
+                    alpha[c] = 1.f;
+                    if (top - mm[c] > kWeightMost) {
+                        alpha[c] = ex2(mm[c] - (top - kWeightTop));
+                        mm[c] = top - kWeightTop;
+                        l[c] *= alpha[c];
+                    }
+                }
+                if (!fresh) {
+                    // O's rows of this thread: the product before must have completed
+                    wait(&bar->p_free[(it - 1) & 1], (it - 1) >> 1);
+                    tc::fence_after_sync();
+#pragma unroll
+                    for (int part = 0; part < 3; ++part)
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            uint32_t o[8];
+                            const uint32_t a = tc::taddr(tmem_o, lane_row, part * COLS + 8 * nb);
+                            tc::ld8(a, o);
+                            tc::wait_ld();
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha[8 * nb + c]);
+                            tc::st8(a, o);
+                        }
+                    tc::wait_st();
+                }
+            }
+            fresh = false;
+            // ---- weights, their sum, and their parts: row (part, c), byte t of the B operand
+            if (it >= 2) wait(&bar->p_free[it & 1], (it >> 1) - 1);
+            uint8_t* pw = p_sm + (it & 1) * C::QB;
+#pragma unroll
+            for (int c = 0; c < COLS; c += 2) {
+                float w0 = ex2(x[c] - mm[c]), w1 = ex2(x[c + 1] - mm[c + 1]);
+                l[c] = fmaf(w0, inv_vs, l[c]);
+                l[c + 1] = fmaf(w1, inv_vs, l[c + 1]);
+#pragma unroll
+                for (int part = 0; part < 3; ++part) {
+                    const uint32_t v = e4m3x2(w0, w1);
+                    const int ra = part * COLS + c, rb = ra + 1;
+                    pw[ra * 128 + ((tid >> 4) ^ (ra & 7)) * 16 + (tid & 15)] = (uint8_t)v;
+                    pw[rb * 128 + ((tid >> 4) ^ (rb & 7)) * 16 + (tid & 15)] = (uint8_t)(v >> 8);
+                    if (part < 2) {
+                        const uint32_t h = half2_of_e4m3x2(v);
+                        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                        w0 -= u.x, w1 -= u.y;
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->p_full[it & 1]);
+
+            if (at.j == at.tiles - 1 || it == ntiles - 1) {
+                // ---- the unit's (or its part's) end: sums over the keys, then O, of which thread t has dim t
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) {
+                    float v = l[c];
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                    if (lane == 0) l_sm[warp * COLS + c] = v;
+                }
+                named_bar_sync(kBar, kCompute);
+                const int2 ctas = line.ctas_of(at);
+                const bool whole = ctas.x == ctas.y;
+                const size_t part = part_slot(blockIdx.x, first_tile == 0);
+                wait(&bar->p_free[it & 1], it >> 1);
+                tc::fence_after_sync();
+                uint32_t a[C::N];
+                tc::ld32(tc::taddr(tmem_o, lane_row, 0), *reinterpret_cast<uint32_t(*)[32]>(a));
+                if constexpr (C::N == 48) tc::ld16(tc::taddr(tmem_o, lane_row, 32), *reinterpret_cast<uint32_t(*)[16]>(a + 32));
+                tc::wait_ld();
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) {
+                    if (c >= rows) continue;
+                    const float sum = (l_sm[c] + l_sm[COLS + c]) + (l_sm[2 * COLS + c] + l_sm[3 * COLS + c]);
+                    const float o = __uint_as_float(a[c]) + (__uint_as_float(a[COLS + c]) + __uint_as_float(a[2 * COLS + c]));
+                    const float y = sum > 0.f ? o / sum : 0.f;
+                    if (whole) {
+                        out_row(p, at, r0, c)[tid] = __float2half_rn(y);
+                    } else {
+                        tp.part_o[(part * kMaxCols + c) * D + tid] = y;
+                        if (tid == 0) tp.part_lse[part * kMaxCols + c] = sum > 0.f ? mm[c] + __log2f(sum) : -INFINITY;
+                    }
+                }
+                if (!whole) join_parts<D>(tp, at, r0, rows, ctas.x, ctas.y, misc + 1);
+                fresh = true;
+            }
+            line.step(at);
+        }
+    }
+    // ---- teardown
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 5) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, C::TMEM);
+    }
+    advance_lengths(p, misc + 2);
+}
+
+template <int NB>
+static int launch_tc(TileParams& tp, const Freqs& f, int sms, int dev, cudaStream_t st) {
+    using C = TcCfg<NB>;
+    static std::once_flag once[128];
+    static cudaError_t attr[128];
+    if (dev < 0 || dev >= 128) return set_status(FCCI_EINVAL, "device index");
+    std::call_once(once[dev], [&]() {
+        attr[dev] = cudaFuncSetAttribute(paged_split_tc_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    });
+    if (attr[dev] != cudaSuccess) return set_cuda_status(attr[dev]);
+    int stages = 0, per_sm = 0;
+    for (int ctas = kMaxCtasPerSm; ctas >= 1 && !stages; --ctas)
+        for (int s = kMaxStages; s >= 2 && !stages; --s)
+            if (C::smem(s, tp.p.B) <= (size_t)(228 * 1024 / ctas - 1024)) stages = s, per_sm = ctas;
+    if (!stages) return set_status(FCCI_EUNSUPPORTED, "paged attention: batch too large for shared memory");
+    tp.stages = stages;
+    CUtensorMap m[4];
+    const int rc = encode_pages<typename C::TL, true>(tp.p, m);
+    if (rc) return rc;
+    return launch_pdl(paged_split_tc_kernel<NB>, dim3(sms * per_sm), dim3(kTcThreads), C::smem(stages, tp.p.B), st, m[0], m[1],
+                      m[2], m[3], tp, f);
+}
+
+int launch_split_tc(TileParams& tp, const Freqs& f, int sms, int dev, cudaStream_t st) {
+    return (int64_t)tp.p.max_q * tp.p.G <= 8 ? launch_tc<1>(tp, f, sms, dev, st) : launch_tc<2>(tp, f, sms, dev, st);
+}
+
+}  // namespace pg
+}  // namespace fcci

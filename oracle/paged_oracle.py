@@ -98,10 +98,10 @@ def keys_values(k_pool, v_pool, k_scales, v_scales, table_row, length, h):
 
 
 def attention(q, k, v, scale):
-    """(out [D], weights @ |v| [D], largest |score|-like sum) of one query row in float64."""
+    """(out [D], weights @ |v| [D], largest sum|q k| scale, largest weight) of one query row in float64."""
     if k.shape[0] == 0:
         z = torch.zeros(q.shape[-1], dtype=torch.float64)
-        return z, z, 0.0
+        return z, z, 0.0, 0.0
     x = (k @ q.double()) * scale
     p = torch.softmax(x, 0)
-    return p @ v, p @ v.abs(), float(((k.abs() @ q.double().abs()) * scale).max())
+    return p @ v, p @ v.abs(), float(((k.abs() @ q.double().abs()) * scale).max()), float(p.max())
