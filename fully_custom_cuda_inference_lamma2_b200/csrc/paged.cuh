@@ -97,6 +97,17 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+__device__ __forceinline__ uint32_t e4m3x2_of_half2(uint32_t h) {
+    uint16_t c;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(h));
+    return c;
+}
+
+__device__ __forceinline__ uint32_t half2_minus(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // Two e4m3 codes to fp16 (exact).
 __device__ __forceinline__ uint32_t half2_of_e4m3x2(uint32_t codes) {
     uint32_t h;

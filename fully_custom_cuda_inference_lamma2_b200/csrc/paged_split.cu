@@ -99,8 +99,6 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
 
     At at = line.template build<kThreads>(reinterpret_cast<int*>(red_ml));
     const int ntiles = line.ntiles;
-    const int* seqT = line.T;
-    const int* seqN = line.n;
     const int box = min(p.page, KEYS);  // rows of one page in a tile
     if (warp == kComputeWarps) {
         fetch_tiles<TL, E4M3, COLS>(line, at, &mk, &mv, &mk16, &mv16, tiles_sm, full, empty, scale_sm, abort_flag);
@@ -133,8 +131,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
             else q_fragment(part, nb, kk, r);
         };
 
+        Ring ring(S);
         for (int it = 0; it < ntiles; ++it) {
-            const int T = seqT[at.b], n = seqN[at.b], L = line.keys_at(at);
+            const int T = at.T, n = at.n, L = at.L;
             const int r0 = at.c * COLS, rows = min(COLS, n * G - r0);  // query rows of this unit
             if (fresh) {
                 fresh = false;
@@ -197,9 +196,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                 if (C::QREG) named_bar_sync(kBar, kCompute);
             }
 
-            const int s = it % S;
+            const int s = ring.s;
             const bool ready =
-                __all_sync(0xffffffffu, mbar_wait_bounded(&full[s], (uint32_t)(it / S) & 1u, abort_flag, kWaitLimitNs));
+                __all_sync(0xffffffffu, mbar_wait_sparing(&full[s], ring.round & 1u, abort_flag, kWaitLimitNs));
             if (!ready && !*abort_flag) {
                 *abort_flag = 1;
                 set_error(p, FCCI_DEV_ERR_TIMEOUT);
@@ -492,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                 fresh = true;
             }
             line.step(at);
+            ring.next();
         }
     }
     advance_lengths(p, misc + 2);

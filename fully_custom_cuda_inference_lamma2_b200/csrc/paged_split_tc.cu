@@ -8,7 +8,8 @@
 // three e4m3 values, each the rounding of what the ones before left (within 2^-12 of it), as three rows of the
 // same product:
 //   S^T[key, (part, row)] = K Q^T     A = the K tile (128 keys), B = 3 * COLS rows of query parts
-//   O^T[dim, (part, row)] += V^T P^T  A = the V tile read dim-major, B = 3 * COLS rows of weight parts
+//   O^T[dim, (part, row)] += V^T P^T  A = the V tile read dim-major, B = the weight parts, 3 * COLS bytes of each
+//                                     key side by side (N-major), which is what the key's thread has
 // The parts are summed where S is read, and where O is read at a unit's end.
 //   - A query row is rotated in fp32 and scaled by a power of two to at most 448 before it is split.
 //   - Thread t of the softmax owns key t of the tile: its scales are its own numbers. The exponent of V's scale
@@ -43,9 +44,11 @@ struct TcCfg {
     static constexpr int N = NB == 1 ? 32 : 48;         // rows of a B operand: 3 * COLS, a multiple of 16
     static constexpr int STRIDE = NB == 1 ? 32 : 64;    // TMEM columns of one accumulator
     static constexpr int TMEM = NB == 1 ? 128 : 256;
-    static constexpr int QB = N * 128;                  // bytes of a B operand
+    static constexpr int QB = N * 128;                  // bytes of the query parts
+    static constexpr int PW = NB == 1 ? 32 : 64;        // bytes of a key's weight parts (the swizzle's width)
+    static constexpr int PB = kTcKeys * PW;             // bytes of a weight buffer
     // shared memory behind the stages
-    static constexpr int kP = QB, kSmall = 3 * QB;      // queries, two weight buffers, the rest
+    static constexpr int kP = QB, kSmall = QB + 2 * PB;  // queries, two weight buffers, the rest
     static size_t smem(int stages, int B) {
         return 1024 + (size_t)stages * 2 * TL::BYTES + kSmall + 64 * 8 /* cos, sin */ + 8 * COLS * 4 /* maxima, sums */ +
                COLS * 4 /* query scales */ + kMaxStages * 64 /* page scales */ + 256 /* barriers */ + 64 +
@@ -93,8 +96,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
     uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     const int S = tp.stages, G = p.G;
     uint8_t* rest = sm + (size_t)S * 2 * TL::BYTES;
-    uint8_t* q_sm = rest;             // [N rows][128 bytes], 128-byte swizzle
-    uint8_t* p_sm = rest + C::kP;     // two of the same
+    uint8_t* q_sm = rest;             // [N rows][128 dims], 128-byte swizzle
+    uint8_t* p_sm = rest + C::kP;     // two of [128 keys][PW], swizzled over PW bytes
     float2* cs = reinterpret_cast<float2*>(rest + C::kSmall);  // decode: cos and sin of position T
     float* mx_sm = reinterpret_cast<float*>(cs + 64);          // [4][COLS] maxima, then sums
     float* l_sm = mx_sm + 4 * COLS;
@@ -147,68 +150,75 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
         set_error(p, FCCI_DEV_ERR_TIMEOUT);
     };
     auto wait = [&](uint64_t* b, uint32_t parity) {
-        const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(b, parity & 1u, abort_flag, kWaitLimitNs));
-        if (!ok && !*abort_flag) fail();
-        return ok;
+        if (__all_sync(0xffffffffu, mbar_wait_sparing(b, parity & 1u, abort_flag, kWaitLimitNs))) return true;
+        if (!*abort_flag) fail();
+        return false;
     };
     // the append of row T happens in the tile that holds it
-    auto appends = [&](const At& x) { return tp.fused && line.T[x.b] >= 0 && line.T[x.b] / KEYS == x.j; };
+    auto appends = [&](const At& x) { return tp.fused && x.T >= 0 && x.T / KEYS == x.j; };
 
     if (warp == 4) {
         fetch_tiles<TL, true, COLS>(line, at, &mk, &mv, &mk16, &mv16, sm, bar->full, bar->empty, scale_sm, abort_flag);
     } else if (warp == 5) {
-        // ============================================================ products
-        const uint32_t id_s = tc::idesc_e4m3_f32(128, C::N, 0, 0);
-        const uint32_t id_o = tc::idesc_e4m3_f32(128, C::N, 1, 0);
-        const uint64_t qd = tc::smem_desc_sw128(smem_u32(q_sm), 16, 1024);
-        int nrow = 0, nq = 0;
-        bool begins_prev = false;  // tile it - 1 is its unit's first here
-        // O += V^T P of tile i (begins: O = V^T P)
-        auto issue_o = [&](int i, bool begins) {
-            if (!wait(&bar->p_full[i & 1], i >> 1)) return false;
-            tc::fence_after_sync();
-            if (lane == 0) {
-                const uint64_t vd = tc::smem_desc_sw128(smem_u32(sm + (size_t)(i % S) * 2 * TL::BYTES + TL::BYTES), TL::BYTES, 1024);
-                const uint64_t pd = tc::smem_desc_sw128(smem_u32(p_sm + (i & 1) * C::QB), 16, 1024);
+        // ============================================================ products, by one thread
+        if (elect_one()) {
+            auto wait1 = [&](uint64_t* b, uint32_t parity) {
+                if (mbar_wait_sparing(b, parity & 1u, abort_flag, kWaitLimitNs)) return true;
+                if (!*abort_flag) fail();
+                return false;
+            };
+            constexpr uint32_t id_s = tc::idesc_e4m3_f32(128, C::N, 0, 0);
+            constexpr uint32_t id_o = tc::idesc_e4m3_f32(128, C::N, 1, 1);
+            const uint64_t qd = tc::smem_desc_sw128(smem_u32(q_sm), 16, 1024);
+            const uint64_t kd0 = tc::smem_desc_sw128(smem_u32(sm), 16, 1024);
+            const uint64_t vd0 = tc::smem_desc_sw128(smem_u32(sm) + TL::BYTES, TL::BYTES, 1024);
+            const uint64_t pd0 = tc::smem_desc_sw<C::PW>(smem_u32(p_sm), C::PB, 8 * C::PW);
+            int nrow = 0, nq = 0;
+            bool begins_prev = false;  // tile it - 1 is its unit's first here
+            // O += V^T P of tile i in stage st (begins: O = V^T P)
+            auto issue_o = [&](int i, int st, bool begins) {
+                if (!wait1(&bar->p_full[i & 1], i >> 1)) return false;
+                tc::fence_after_sync();
+                const uint64_t vd = vd0 + (uint64_t)(st * (2 * TL::BYTES >> 4)), pd = pd0 + (uint64_t)((i & 1) * (C::PB >> 4));
 #pragma unroll
-                for (int k = 0; k < KEYS / 32; ++k)  // 32 keys: 4 groups of 8 rows of V, 32 bytes of a row of P
-                    tc::mma_ss_f8(tmem_o, vd + (uint64_t)(k * 4096 >> 4), pd + (uint64_t)(k * 32 >> 4), id_o, !begins || k > 0);
+                for (int k = 0; k < KEYS / 32; ++k)  // 32 keys: 4 groups of 8 rows of V and of P
+                    tc::mma_ss_f8(tmem_o, vd + (uint64_t)(k * 4096 >> 4), pd + (uint64_t)(k * 32 * C::PW >> 4), id_o, !begins || k > 0);
                 tc::commit(&bar->p_free[i & 1]);
-                tc::commit(&bar->empty[i % S]);
-            }
-            __syncwarp();
-            return true;
-        };
-        bool ok = true;
-        for (int it = 0; it < ntiles && ok; ++it) {
-            const bool begins = it == 0 || at.j == 0;
-            if (begins) {
-                // the queries of the new unit come only after the last one's O was read, which needs its last product
-                if (it > 0 && !(ok = issue_o(it - 1, begins_prev))) break;
-                if (!(ok = wait(&bar->q_full, nq++))) break;
-            }
-            if (!(ok = wait(&bar->full[it % S], it / S))) break;
-            if (appends(at) && !(ok = wait(&bar->row_done, nrow++))) break;
-            if (it >= 2 && !(ok = wait(&bar->s_free[it & 1], (it >> 1) - 1))) break;
-            tc::fence_after_sync();
-            if (lane == 0) {
-                const uint64_t kd = tc::smem_desc_sw128(smem_u32(sm + (size_t)(it % S) * 2 * TL::BYTES), 16, 1024);
+                tc::commit(&bar->empty[st]);
+                return true;
+            };
+            bool ok = true;
+            Ring ring(S);
+            int st_prev = 0;  // stage of tile it - 1
+            for (int it = 0; it < ntiles; ++it) {
+                // S of this tile first, so that the softmax has it when it is through with the last one; but not
+                // when the tile is still on its way (the last one's stage would come free late), and not
+                // over a unit's end (the new queries come after the old O was read)
+                const int st = ring.s;
+                const bool begins = it == 0 || at.j == 0;
+                const bool o_first = it > 0 && (begins || !mbar_test_wait(&bar->full[st], ring.round & 1u));
+                if (o_first && !(ok = issue_o(it - 1, st_prev, begins_prev))) break;
+                if (begins && !(ok = wait1(&bar->q_full, nq++))) break;
+                if (!(ok = wait1(&bar->full[st], ring.round))) break;
+                if (appends(at) && !(ok = wait1(&bar->row_done, nrow++))) break;
+                if (it >= 2 && !(ok = wait1(&bar->s_free[it & 1], (it >> 1) - 1))) break;
+                tc::fence_after_sync();
+                const uint64_t kd = kd0 + (uint64_t)(st * (2 * TL::BYTES >> 4));
 #pragma unroll
                 for (int k = 0; k < D / 32; ++k)
                     tc::mma_ss_f8(tmem + (it & 1) * C::STRIDE, kd + (uint64_t)(k * 32 >> 4), qd + (uint64_t)(k * 32 >> 4), id_s, k > 0);
                 tc::commit(&bar->s_full[it & 1]);
+                if (it > 0 && !o_first && !(ok = issue_o(it - 1, st_prev, begins_prev))) break;
+                begins_prev = begins;
+                st_prev = st;
+                ring.next();
+                line.step(at);
             }
-            __syncwarp();
-            if (!begins && !(ok = issue_o(it - 1, begins_prev))) break;
-            begins_prev = begins;
-            line.step(at);
-        }
-        if (ok && ntiles > 0) issue_o(ntiles - 1, begins_prev);
-        // every product has completed before TMEM is released
-        if (lane == 0) {
+            if (ok && ntiles > 0) issue_o(ntiles - 1, st_prev, begins_prev);
+            // every product has completed before TMEM is released
             tc::commit(&bar->drain);
             volatile int never = 0;
-            mbar_wait_bounded(&bar->drain, 0, &never, kDrainLimitNs);
+            mbar_wait_sparing(&bar->drain, 0, &never, kDrainLimitNs);
         }
         __syncwarp();
     } else {
@@ -221,8 +231,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
         float mm[COLS], l[COLS], qf[COLS];  // m - kWeightTop, sum, factor of a score
         bool fresh = true;
         int first_tile = 0;
+        Ring ring(S);
         for (int it = 0; it < ntiles; ++it) {
-            const int T = line.T[at.b], n = line.n[at.b], L = line.keys_at(at);
+            const int T = at.T, n = at.n, L = at.L;
             const int r0 = at.c * COLS, rows = min(COLS, n * G - r0);
             if (fresh) {
                 first_tile = at.j;
@@ -291,10 +302,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                     qf[c] = qs_sm[c];
                 }
             }
-            const int s = it % S;
+            const int s = ring.s;
             uint8_t* kt = sm + (size_t)s * 2 * TL::BYTES;
             float* scales = scale_sm + s * 16;
-            const bool ready = wait(&bar->full[s], it / S);
+            const bool ready = wait(&bar->full[s], ring.round);
             if (appends(at)) {
                 // ---- warp 0 the key, warp 1 the value, before the tile's first product
                 const int bx = (T & (KEYS - 1)) >> box_log2;
@@ -315,9 +326,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 for (int ch = 0; ch < 8; ++ch)
                     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(TL::cell(v32, tid, ch)), "r"(0) : "memory");
             }
-            const float lv = live ? (float)((int)(__float_as_uint(vs) >> 23) - 127) : -INFINITY;
-            const float inv_vs = live ? 1.f / vs : 0.f;
-            const float k2 = live ? ks : 0.f;
+            const float lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);
+            const float inv_vs = live ? exp2_int(127 - (int)(__float_as_uint(vs) >> 23)) : 0.f;
             // ---- scores of this key, in the log2 domain, with V's exponent
             wait(&bar->s_full[it & 1], it >> 1);
             tc::fence_after_sync();
@@ -328,13 +338,16 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 if constexpr (C::N == 48) tc::ld16(tc::taddr(tmem, lane_row, (it & 1) * C::STRIDE + 32), *reinterpret_cast<uint32_t(*)[16]>(a + 32));
                 tc::wait_ld();
                 tc::fence_before_sync();
-                __syncwarp();
                 if (lane == 0) mbar_arrive(&bar->s_free[it & 1]);
 #pragma unroll
                 for (int c = 0; c < COLS; ++c) {
                     const float sum = __uint_as_float(a[c]) + (__uint_as_float(a[COLS + c]) + __uint_as_float(a[2 * COLS + c]));
-                    x[c] = live ? fmaf(sum * k2, qf[c], lv) : -INFINITY;
+                    x[c] = fmaf(sum * ks, qf[c], lv);
                 }
+            }
+            if (!live) {
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) x[c] = -INFINITY;
             }
             if (p.cu_q && (at.j + 1) * KEYS > T) {  // a row sees the keys up to its own position
 #pragma unroll
@@ -342,9 +355,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                     if (t > T + (r0 + c) / G) x[c] = -INFINITY;
             }
             // ---- move m when a weight would leave e4m3's range
-            bool over = false;
+            float most = x[0] - mm[0];
 #pragma unroll
-            for (int c = 0; c < COLS; ++c) over = over || x[c] - mm[c] > kWeightMost;
+            for (int c = 1; c < COLS; ++c) most = fmaxf(most, x[c] - mm[c]);
+            const bool over = most > kWeightMost;
             if (any_of_compute(over)) {
 #pragma unroll
                 for (int c = 0; c < COLS; ++c) {
@@ -383,26 +397,35 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 }
             }
             fresh = false;
-            // ---- weights, their sum, and their parts: row (part, c), byte t of the B operand
-            if (it >= 2) wait(&bar->p_free[it & 1], (it >> 1) - 1);
-            uint8_t* pw = p_sm + (it & 1) * C::QB;
+            // ---- weights, their sum, and their parts (of the weight in fp16): bytes part * COLS + c of this key
+            uint32_t w[3 * COLS / 4];
 #pragma unroll
-            for (int c = 0; c < COLS; c += 2) {
-                float w0 = ex2(x[c] - mm[c]), w1 = ex2(x[c + 1] - mm[c + 1]);
-                l[c] = fmaf(w0, inv_vs, l[c]);
-                l[c + 1] = fmaf(w1, inv_vs, l[c + 1]);
+            for (int c = 0; c < COLS; c += 4) {
+                float u[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    u[k] = ex2(x[c + k] - mm[c + k]);
+                    l[c + k] = fmaf(u[k], inv_vs, l[c + k]);
+                }
+                uint32_t h0 = pack_half2(u[0], u[1]), h1 = pack_half2(u[2], u[3]);
 #pragma unroll
                 for (int part = 0; part < 3; ++part) {
-                    const uint32_t v = e4m3x2(w0, w1);
-                    const int ra = part * COLS + c, rb = ra + 1;
-                    pw[ra * 128 + ((tid >> 4) ^ (ra & 7)) * 16 + (tid & 15)] = (uint8_t)v;
-                    pw[rb * 128 + ((tid >> 4) ^ (rb & 7)) * 16 + (tid & 15)] = (uint8_t)(v >> 8);
-                    if (part < 2) {
-                        const uint32_t h = half2_of_e4m3x2(v);
-                        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                        w0 -= u.x, w1 -= u.y;
-                    }
+                    const uint32_t v0 = e4m3x2_of_half2(h0), v1 = e4m3x2_of_half2(h1);
+                    w[(part * COLS + c) / 4] = v0 | (v1 << 16);
+                    if (part < 2) h0 = half2_minus(h0, half2_of_e4m3x2(v0)), h1 = half2_minus(h1, half2_of_e4m3x2(v1));
                 }
+            }
+            if (it >= 2) wait(&bar->p_free[it & 1], (it >> 1) - 1);
+            {
+                // 16-byte chunk ch of key t lies at ch ^ (t >> 2 & 1) of 32 bytes, ch ^ (t >> 1 & 3) of 64
+                const uint32_t row = smem_u32(p_sm + (it & 1) * C::PB) + tid * C::PW;
+                const int sw = NB == 1 ? (tid >> 2) & 1 : (tid >> 1) & 3;
+#pragma unroll
+                for (int ch = 0; ch < 3 * NB / 2; ++ch)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + (ch ^ sw) * 16), "r"(w[4 * ch]),
+                                 "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3]) : "memory");
+                if constexpr (NB == 1)
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(row + (1 ^ sw) * 16), "r"(w[4]), "r"(w[5]) : "memory");
             }
             fence_proxy_async_smem();
             tc::fence_before_sync();
@@ -445,6 +468,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 fresh = true;
             }
             line.step(at);
+            ring.next();
         }
     }
     // ---- teardown

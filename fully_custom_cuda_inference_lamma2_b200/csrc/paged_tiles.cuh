@@ -47,10 +47,22 @@ struct Tile {
     }
 };
 
+// Ring of S stages: the stage of the present tile and the times the ring has been gone round (a division by S
+// would cost more than the rest of a loop's bookkeeping).
+struct Ring {
+    int S, s = 0;
+    uint32_t round = 0;
+    __device__ explicit Ring(int n) : S(n) {}
+    __device__ __forceinline__ void next() {
+        if (++s == S) s = 0, ++round;
+    }
+};
+
 // A place on the line.
 struct At {
     int b, h, c, j;     // sequence, kv head, column group, tile
     int tiles, groups;  // of sequence b
+    int T, n, L;        // its cached rows (-1: not served), new tokens, keys
 };
 
 template <int KEYS, int COLS>
@@ -66,11 +78,12 @@ struct Line {
     __device__ __forceinline__ int keys(int t, int m) const { return t + (tp.fused || tp.p.cu_q ? m : 0); }
     __device__ __forceinline__ int groups(int m) const { return (m * tp.p.G + COLS - 1) / COLS; }
     __device__ __forceinline__ int tiles(int t, int m) const { return max(1, (keys(t, m) + KEYS - 1) / KEYS); }
-    __device__ __forceinline__ int keys_at(const At& x) const { return T[x.b] < 0 ? 0 : keys(T[x.b], n[x.b]); }
 
     __device__ __forceinline__ void enter(At& x) const {
-        x.groups = groups(n[x.b]);
-        x.tiles = T[x.b] < 0 ? 1 : tiles(T[x.b], n[x.b]);
+        x.T = T[x.b], x.n = n[x.b];
+        x.L = x.T < 0 ? 0 : keys(x.T, x.n);
+        x.groups = groups(x.n);
+        x.tiles = x.T < 0 ? 1 : tiles(x.T, x.n);
     }
 
     __device__ __forceinline__ void step(At& x) const {
@@ -139,7 +152,7 @@ struct Line {
             t1 = ((long long)blockIdx.x + 1) * N / CT;
         }
         ntiles = (int)(t1 - t0);
-        At at = {0, 0, 0, 0, 1, 1};
+        At at = {0, 0, 0, 0, 1, 1, -1, 0, 0};
         if (ntiles > 0) {
             int l = 0, r = B - 1;
             while (l < r) {
@@ -179,29 +192,30 @@ __device__ void fetch_tiles(const Line<TL::KEYS, COLS>& line, At at, const CUten
     constexpr int KEYS = TL::KEYS, PITCH = TL::PITCH;
     const TileParams& tp = line.tp;
     const Params& p = tp.p;
-    const int S = tp.stages, lane = threadIdx.x & 31, ntiles = line.ntiles;
+    const int lane = threadIdx.x & 31, ntiles = line.ntiles;
+    Ring ring(tp.stages);
     const int box = min(p.page, KEYS), boxes = KEYS / box;
     const uint64_t pol = l2_policy_evict_first();
     const bool is_v = lane >= 16;
     const int slot = lane & 15;
     auto rows_at = [&](const At& x) {
-        return slot < boxes ? max(0, min(box, line.keys_at(x) - x.j * KEYS - slot * box)) : 0;
+        return slot < boxes ? max(0, min(box, x.L - x.j * KEYS - slot * box)) : 0;
     };
     auto page_at = [&](const At& x) {
         if (rows_at(x) == 0) return -1;
         return p.table[(int64_t)x.b * p.table_st + ((x.j * KEYS + slot * box) >> p.page_log2)];
     };
-    auto publish = [&](int i, float v) {
-        if (slot < boxes) scales[(i % S) * 16 + (is_v ? 8 : 0) + slot] = v;
+    // byte: the scale byte as loaded (turned into a number here, a tile later, so that the load has had its time)
+    auto publish = [&](int st, int byte) {
+        if (slot < boxes) scales[st * 16 + (is_v ? 8 : 0) + slot] = byte < 0 ? -1.f : exp2_int(byte - 127);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[i % S]);
+        if (lane == 0) mbar_arrive(&full[st]);
     };
     int pid = ntiles > 0 ? page_at(at) : -1;
-    float scale = 0.f;
-    int it = 0;
+    int byte = -1, it = 0, s_prev = 0;
     bool published = false;  // tile it - 1 has had its second arrival when the loop ends early
     for (; it < ntiles; ++it) {
-        const int s = it % S;
+        const int s = ring.s;
         const int rows = rows_at(at), h = at.h;
         const int row0 = (at.j * KEYS + slot * box) & (p.page - 1);
         const bool there = rows > 0 && (unsigned)pid < (unsigned)p.num_pages;
@@ -210,10 +224,10 @@ __device__ void fetch_tiles(const Line<TL::KEYS, COLS>& line, At at, const CUten
         line.step(at);
         const int pid_next = it + 1 < ntiles ? page_at(at) : -1;
         // when no stage is free, whoever frees one may need the tile before whole first
-        const uint32_t parity = ((uint32_t)(it / S) & 1u) ^ 1u;
+        const uint32_t parity = (ring.round & 1u) ^ 1u;
         const bool early = !__all_sync(0xffffffffu, mbar_test_wait(&empty[s], parity));
-        if (early && it > 0) publish(it - 1, scale);
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], parity, abort_flag, kWaitLimitNs))) {
+        if (early && it > 0) publish(s_prev, byte);
+        if (!__all_sync(0xffffffffu, mbar_wait_sparing(&empty[s], parity, abort_flag, kWaitLimitNs))) {
             if (lane == 0) {
                 *abort_flag = 1;
                 set_error(p, FCCI_DEV_ERR_TIMEOUT);
@@ -240,21 +254,20 @@ __device__ void fetch_tiles(const Line<TL::KEYS, COLS>& line, At at, const CUten
                 }
             }
         }
-        float next = there ? 1.f : -1.f;
-        if (E4M3 && there) {
-            const uint8_t* a = is_v ? p.v_scales + id * p.vs_sp + h * p.vs_sh : p.k_scales + id * p.ks_sp + h * p.ks_sh;
-            next = exp2_int((int)*a - 127);
-        }
-        if (it > 0 && !early) publish(it - 1, scale);
-        scale = next;
+        if (it > 0 && !early) publish(s_prev, byte);
+        byte = there ? 127 : -1;
+        if (E4M3 && there)
+            byte = is_v ? p.v_scales[id * p.vs_sp + h * p.vs_sh] : p.k_scales[id * p.ks_sp + h * p.ks_sh];
+        s_prev = s;
+        ring.next();
         pid = pid_next;
     }
-    if (it > 0 && !published) publish(it - 1, scale);
+    if (it > 0 && !published) publish(s_prev, byte);
     if (*abort_flag) {
         // let copies still in flight land before the CTA can exit
         volatile int never = 0;
-        for (int i = max(0, it - S); i < it; ++i)
-            mbar_wait_bounded(&full[i % S], (uint32_t)(i / S) & 1u, &never, kDrainLimitNs);
+        for (int i = max(0, it - ring.S); i < it; ++i)
+            mbar_wait_sparing(&full[i % ring.S], (uint32_t)(i / ring.S) & 1u, &never, kDrainLimitNs);
     }
 }
 

@@ -77,6 +77,36 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     }
 }
 
+// The same, for kernels whose warps wait often. The wait itself is a call, so that a loop with many
+// waits stays small in the instruction cache; a try suspends the thread for a while by itself, and the timer (a slow
+// special register) is read every 16th try only.
+static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t limit_ns) {
+    uint64_t t0 = 0;
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (*abort) return false;
+        const uint64_t now = global_timer_ns();
+        if (t0 == 0) t0 = now;
+        else if (now - t0 > limit_ns) return false;
+    }
+}
+__device__ __forceinline__ bool mbar_wait_sparing(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t limit_ns) {
+    return mbar_try_wait(bar, parity) || mbar_wait_slow(bar, parity, abort, limit_ns);
+}
+
+// True in one thread of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
                                             uint64_t* bar, uint64_t policy) {

@@ -39,6 +39,14 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t start, uint32_t lbo
     return d;
 }
 
+// The same for an operand swizzled over W = 128, 64 or 32 bytes (layout 2, 4 or 6), whose rows have W bytes.
+template <int W>
+__device__ __forceinline__ uint64_t smem_desc_sw(uint32_t start, uint32_t lbo, uint32_t sbo) {
+    static_assert(W == 128 || W == 64 || W == 32, "swizzle width");
+    const uint64_t d = smem_desc_sw128(start, lbo, sbo) & ~((uint64_t)7 << 61);
+    return d | (uint64_t)(W == 128 ? 2 : W == 64 ? 4 : 6) << 61;
+}
+
 // Instruction descriptor of tcgen05.mma.kind::f16 with fp16 A and B and an fp32
 // accumulator. a_mn / b_mn select MN-major (1) or K-major (0) operands.
 // Fields: c_format [4,6) = 1 (F32), a_format [7,10) = 0 (F16), b_format
