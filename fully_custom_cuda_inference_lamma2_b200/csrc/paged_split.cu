@@ -3,7 +3,7 @@
 //
 // Work: paged_tiles.cuh.
 //
-// Inside a CTA warp 4 fetches and warps 0..3 compute. A stage holds the K and the V tile, in
+// Inside a CTA warps 4 and 5 fetch and warps 0..3 compute. A stage holds the K and the V tile, in
 // rows of 128 bytes (64 for e4m3 with head_dim 64) in the tensor-map swizzle; the pages of a tile
 // are fetched side by side, one lane and one box each, the page that ends a sequence in boxes
 // of 16 rows. The page table is read one tile ahead and the scales arrive behind the tile
@@ -26,7 +26,7 @@
 namespace fcci {
 namespace pg {
 
-constexpr int kThreads = kCompute + 32;
+constexpr int kThreads = kCompute + 64;
 
 template <int D, int NB, bool E4M3>
 struct Cfg {
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
-            mbar_init(&full[s], 2);  // the fetched bytes, and the scales
+            mbar_init(&full[s], 4);  // the fetched bytes and the scales, of K and of V
             mbar_init(&empty[s], kComputeWarps);
         }
         misc[0] = 0;
@@ -100,8 +100,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
     At at = line.template build<kThreads>(reinterpret_cast<int*>(red_ml));
     const int ntiles = line.ntiles;
     const int box = min(p.page, KEYS);  // rows of one page in a tile
-    if (warp == kComputeWarps) {
-        fetch_tiles<TL, E4M3, COLS>(line, at, &mk, &mv, &mk16, &mv16, tiles_sm, full, empty, scale_sm, abort_flag);
+    if (warp >= kComputeWarps) {
+        const bool is_v = warp > kComputeWarps;
+        fetch_tiles<TL, E4M3, COLS>(line, at, is_v, is_v ? &mv : &mk, is_v ? &mv16 : &mk16, tiles_sm, full, empty, scale_sm, abort_flag);
     } else {
         // ============================================================ computing warps
         const int w = warp, g = lane >> 2, t4 = lane & 3;

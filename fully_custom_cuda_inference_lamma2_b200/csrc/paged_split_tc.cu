@@ -18,7 +18,8 @@
 //   - m moves only when a weight would exceed 2^8.75 (448 is the largest e4m3), to leave the largest at 2^6: O in
 //     tensor memory is scaled rarely, and four warps agree on it with one barrier a tile.
 //
-// 192 threads: warps 0..3 softmax (TMEM lane t = key t, then dim t), warp 4 fetches, warp 5 issues the products.
+// 224 threads: warps 0..3 softmax (TMEM lane t = key t, then dim t), warps 4 and 6 fetch K and V, warp 5 issues the
+// products.
 // TMEM: two S tiles and O, 3 * COLS columns each (24 or 48, in strides of 32 or 64).
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -32,7 +33,7 @@
 namespace fcci {
 namespace pg {
 
-constexpr int kTcThreads = kCompute + 64;
+constexpr int kTcThreads = kCompute + 96;
 constexpr int kTcD = 128, kTcKeys = 128;
 constexpr float kWeightTop = 6.f, kWeightMost = 8.75f;  // log2 of the largest weight after a move of m, and at most
 constexpr float kNoMax = -1e30f;                         // m before a row has seen a key
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
-            mbar_init(&bar->full[s], 2);  // the fetched bytes, and the scales
+            mbar_init(&bar->full[s], 4);  // the fetched bytes and the scales, of K and of V
             mbar_init(&bar->empty[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
         tc::tmem_alloc(tmem_slot, C::TMEM);
         tc::tmem_relinquish();
     }
+    const uint64_t turn = tid < p.rot / 2 ? f.turn[tid] : 0;  // a launch constant: its cold read is over before the wait is
     griddep_launch_dependents();
     griddep_wait();
     tc::fence_before_sync();
@@ -157,8 +159,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
     // the append of row T happens in the tile that holds it
     auto appends = [&](const At& x) { return tp.fused && x.T >= 0 && x.T / KEYS == x.j; };
 
-    if (warp == 4) {
-        fetch_tiles<TL, true, COLS>(line, at, &mk, &mv, &mk16, &mv16, sm, bar->full, bar->empty, scale_sm, abort_flag);
+    if (warp == 4 || warp == 6) {
+        const bool is_v = warp == 6;
+        fetch_tiles<TL, true, COLS>(line, at, is_v, is_v ? &mv : &mk, is_v ? &mv16 : &mk16, sm, bar->full, bar->empty, scale_sm,
+                                    abort_flag);
     } else if (warp == 5) {
         // ============================================================ products, by one thread
         if (elect_one()) {
@@ -238,10 +242,6 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
             if (fresh) {
                 first_tile = at.j;
                 // ---- queries: warp w takes rows w, w + 4, ...; a lane 4 neighbouring dims
-                if (!p.cu_q && rot > 0) {
-                    if (tid < half) cs[tid] = rope_cs(f.turn[tid], max(T, 0));
-                    named_bar_sync(kBar, kCompute);
-                }
                 const int64_t tok0 = p.cu_q ? p.cu_q[at.b] : at.b;
                 const int d = 4 * lane;
                 uint2 xr[COLS / 4], yr[COLS / 4];
@@ -254,6 +254,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                         xr[k] = *reinterpret_cast<const uint2*>(q + d);
                         if (d < rot) yr[k] = *reinterpret_cast<const uint2*>(q + (d < half ? d + half : d - half));
                     }
+                }
+                if (!p.cu_q && rot > 0) {  // while the loads are under way
+                    if (tid < half) cs[tid] = rope_cs(turn, max(T, 0));
+                    named_bar_sync(kBar, kCompute);
                 }
 #pragma unroll
                 for (int k = 0; k < COLS / 4; ++k) {

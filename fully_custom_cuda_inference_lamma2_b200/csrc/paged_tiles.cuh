@@ -181,14 +181,15 @@ struct Line {
 // Slot of this CTA's part of a cut unit: it has at most two parts, one that begins a unit and one that does not.
 __device__ __forceinline__ size_t part_slot(int cta, bool begins) { return 2 * (size_t)cta + (begins ? 1 : 0); }
 
-// The fetching warp. A lane has one page box of the tile: lanes 0.. those of K, lanes 16.. those of V. The
-// page table is read a tile ahead, and a tile's scales are published (its second arrival on `full`)
-// after the next tile's copies are under way, so neither latency delays a copy.
+// A fetching warp: that of K or of V (an issue of a copy takes the thread some 90 cycles, and a tile of 16-row pages
+// has 8 boxes of each). A lane has one page box of the tile. The page table is read a tile ahead, and a tile's
+// scales are published (the warp's second arrival on `full`) after the next tile's copies are under way,
+// so neither latency delays a copy.
 // scales: [stage][K, V][8]: 2^e of the box's page (fp16 pages: 1); -1 where there is none.
 template <class TL, bool E4M3, int COLS>
-__device__ void fetch_tiles(const Line<TL::KEYS, COLS>& line, At at, const CUtensorMap* mk, const CUtensorMap* mv,
-                            const CUtensorMap* mk16, const CUtensorMap* mv16, uint8_t* tiles, uint64_t* full,
-                            uint64_t* empty, float* scales, volatile int* abort_flag) {
+__device__ void fetch_tiles(const Line<TL::KEYS, COLS>& line, At at, bool is_v, const CUtensorMap* map,
+                            const CUtensorMap* map16, uint8_t* tiles, uint64_t* full, uint64_t* empty, float* scales,
+                            volatile int* abort_flag) {
     constexpr int KEYS = TL::KEYS, PITCH = TL::PITCH;
     const TileParams& tp = line.tp;
     const Params& p = tp.p;
@@ -196,18 +197,20 @@ __device__ void fetch_tiles(const Line<TL::KEYS, COLS>& line, At at, const CUten
     Ring ring(tp.stages);
     const int box = min(p.page, KEYS), boxes = KEYS / box;
     const uint64_t pol = l2_policy_evict_first();
-    const bool is_v = lane >= 16;
-    const int slot = lane & 15;
-    auto rows_at = [&](const At& x) {
-        return slot < boxes ? max(0, min(box, x.L - x.j * KEYS - slot * box)) : 0;
-    };
+    const int32_t* table = p.table;
+    const int64_t table_st = p.table_st;
+    const int page_log2 = p.page_log2, row_mask = p.page - 1, first_row = lane * box;
+    const unsigned num_pages = (unsigned)p.num_pages;
+    const uint8_t* scale_bytes = is_v ? p.v_scales : p.k_scales;
+    const int64_t ssp = is_v ? p.vs_sp : p.ks_sp, ssh = is_v ? p.vs_sh : p.ks_sh;
+    if (is_v) tiles += TL::BYTES, scales += 8;
+    auto rows_at = [&](const At& x) { return lane < boxes ? max(0, min(box, x.L - x.j * KEYS - first_row)) : 0; };
     auto page_at = [&](const At& x) {
-        if (rows_at(x) == 0) return -1;
-        return p.table[(int64_t)x.b * p.table_st + ((x.j * KEYS + slot * box) >> p.page_log2)];
+        return rows_at(x) > 0 ? table[x.b * table_st + ((x.j * KEYS + first_row) >> page_log2)] : -1;
     };
     // byte: the scale byte as loaded (turned into a number here, a tile later, so that the load has had its time)
     auto publish = [&](int st, int byte) {
-        if (slot < boxes) scales[st * 16 + (is_v ? 8 : 0) + slot] = byte < 0 ? -1.f : exp2_int(byte - 127);
+        if (lane < boxes) scales[st * 16 + lane] = byte < 0 ? -1.f : exp2_int(byte - 127);
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[st]);
     };
@@ -217,12 +220,12 @@ __device__ void fetch_tiles(const Line<TL::KEYS, COLS>& line, At at, const CUten
     for (; it < ntiles; ++it) {
         const int s = ring.s;
         const int rows = rows_at(at), h = at.h;
-        const int row0 = (at.j * KEYS + slot * box) & (p.page - 1);
-        const bool there = rows > 0 && (unsigned)pid < (unsigned)p.num_pages;
+        const int row0 = (at.j * KEYS + first_row) & row_mask;
+        const bool there = rows > 0 && (unsigned)pid < num_pages;
         if (rows > 0 && !there) set_error(p, FCCI_DEV_ERR_PAGE);
         const int id = there ? pid : 0;
         line.step(at);
-        const int pid_next = it + 1 < ntiles ? page_at(at) : -1;
+        if (it + 1 < ntiles) pid = page_at(at);
         // when no stage is free, whoever frees one may need the tile before whole first
         const uint32_t parity = (ring.round & 1u) ^ 1u;
         const bool early = !__all_sync(0xffffffffu, mbar_test_wait(&empty[s], parity));
@@ -240,27 +243,23 @@ __device__ void fetch_tiles(const Line<TL::KEYS, COLS>& line, At at, const CUten
         if (lane == 0) mbar_arrive_expect_tx(&full[s], bytes);
         __syncwarp();
         if (there) {
-            uint8_t* dst = tiles + (size_t)s * 2 * TL::BYTES + (is_v ? TL::BYTES : 0) + slot * box * PITCH;
-            const CUtensorMap* m = is_v ? mv : mk;
-            const CUtensorMap* m16 = is_v ? mv16 : mk16;
+            uint8_t* dst = tiles + (size_t)s * 2 * TL::BYTES + first_row * PITCH;
 #pragma unroll
             for (int k = 0; k < TL::BLOCKS; ++k) {
                 const int col = k * PITCH / (E4M3 ? 1 : 2);
                 if (rows == box) {
-                    tma_load_4d(dst + k * KEYS * PITCH, m, col, row0, h, id, &full[s], pol);
+                    tma_load_4d(dst + k * KEYS * PITCH, map, col, row0, h, id, &full[s], pol);
                 } else {  // the page that ends the sequence: only the 16-row boxes that hold rows of it
                     for (int r = 0; r < fetched; r += 16)
-                        tma_load_4d(dst + k * KEYS * PITCH + r * PITCH, m16, col, row0 + r, h, id, &full[s], pol);
+                        tma_load_4d(dst + k * KEYS * PITCH + r * PITCH, map16, col, row0 + r, h, id, &full[s], pol);
                 }
             }
         }
         if (it > 0 && !early) publish(s_prev, byte);
         byte = there ? 127 : -1;
-        if (E4M3 && there)
-            byte = is_v ? p.v_scales[id * p.vs_sp + h * p.vs_sh] : p.k_scales[id * p.ks_sp + h * p.ks_sh];
+        if (E4M3 && there) byte = scale_bytes[id * ssp + h * ssh];
         s_prev = s;
         ring.next();
-        pid = pid_next;
     }
     if (it > 0 && !published) publish(s_prev, byte);
     if (*abort_flag) {
