@@ -29,8 +29,9 @@ GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 LIB = os.path.join(PKG, "libfcci_decode.so")
 LIB_SOURCES = ["decode_attn.cu", "capi.cu", "compat.cu", "noalloc.cu", "prefill_attn.cu", "gemv.cu", "step.cu", "exchange.cu",
                "paged_append.cu", "paged_split.cu",
-               "paged_split_tc.cu", "paged_step.cu"]
-LIB_HEADERS = ["ptx.cuh", "tcgen05.cuh", "fcci_internal.h", "paged.cuh", "paged_tiles.cuh"]
+               "paged_split_tc.cu", "paged_prefill.cu", "paged_step.cu"]
+LIB_HEADERS = ["ptx.cuh", "tcgen05.cuh", "fcci_internal.h", "paged.cuh", "paged_tiles.cuh",
+               "prefill_list.cuh"]
 MODULES = {
     "attn_varlen": "attn_varlen_module.cpp",
     "capture_decode_step": "capture_decode_step_module.cpp",

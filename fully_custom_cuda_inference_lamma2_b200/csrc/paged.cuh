@@ -40,6 +40,11 @@ struct Params {
     __half* out;
     int64_t o_st, o_sh;
     __half* q_rot;  // [total_q, Hq, D] contiguous
+    // long chunks: rows [cu_kv[b], cu_kv[b + 1]) of the expanded fp16 keys and values are sequence b's
+    const int32_t* cu_kv;
+    __half* exp_k;
+    __half* exp_v;
+    int64_t exp_sh;
     float scale_log2;
     int32_t rot;
     int32_t advance;
@@ -115,6 +120,19 @@ __device__ __forceinline__ uint32_t half2_of_e4m3x2(uint32_t codes) {
     return h;
 }
 
+// Eight e4m3 codes times the scale, as fp16; clamp: the product may pass 65504.
+__device__ __forceinline__ uint4 expanded(uint2 codes, __half2 scale, bool clamp) {
+    uint32_t h[4] = {half2_of_e4m3x2(codes.x & 0xffffu), half2_of_e4m3x2(codes.x >> 16),
+                     half2_of_e4m3x2(codes.y & 0xffffu), half2_of_e4m3x2(codes.y >> 16)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), scale);
+        if (clamp) v = __hmin2_nan(__hmax2_nan(v, __float2half2_rn(-65504.f)), __float2half2_rn(65504.f));
+        h[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    return make_uint4(h[0], h[1], h[2], h[3]);
+}
+
 // cos and sin of pos * freq. The top 32 bits of the wrapped product are the angle in units of
 // 2^-32 turns; the nearest quarter turn is taken off as an integer, so what is rounded to fp32 is at
 // most an eighth of a turn (angle off by 2^-25 at most), and put back as a swap and signs.
@@ -160,13 +178,20 @@ constexpr int kMaxGrid = 1024;  // CTAs of the split attention launch, at most
 constexpr size_t kHeadBytes = 256 + kMaxGrid * 4;
 constexpr int kMaxCols = 16;  // query rows of one attention unit
 struct WsLayout {
-    size_t part_lse, part_o, q_rot, total;
+    size_t part_lse, part_o, q_rot, cu_kv, items, expanded, total;
 };
-WsLayout ws_layout(int Hq, int Hkv, int D, int total_q, int max_q, int max_kv, int grid);
+// Work items of a prefill: 256 new tokens of one query head each.
+inline int64_t max_items(int B, int Hq, int max_q) { return (int64_t)B * ((max_q + 255) / 256) * Hq; }
+// Query rows of one kv head up to which a chunk takes the split-KV kernels.
+constexpr int kSplitRows = 64;
+inline bool long_chunk(int Hq, int Hkv, int max_q) { return (int64_t)max_q * (Hq / Hkv) > kSplitRows; }
+WsLayout ws_layout(int B, int Hq, int Hkv, int D, int total_q, int max_q, int max_kv, int grid);
 
 int launch_append(const Params& p, const Freqs& f, bool e4m3, cudaStream_t st);
 // Split-KV attention; `fused`: the launch appends the one new row of each sequence itself.
 int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, uint8_t* ws, const WsLayout& L, cudaStream_t st);
+int launch_prefill(const Params& p, const Freqs& f, bool e4m3, uint8_t* ws, const WsLayout& L, int max_kv, float scale_log2,
+                   int advance, cudaStream_t st);
 struct TileParams;
 // The same on the 5th-generation tensor cores, for e4m3 pages of head_dim 128.
 int launch_split_tc(TileParams& tp, const Freqs& f, int sms, int dev, cudaStream_t st);

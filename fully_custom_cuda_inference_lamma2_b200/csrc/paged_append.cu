@@ -158,6 +158,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
         const int heads = (p.q ? p.Hq : 0) + 2 * p.Hkv;
         const int per = (heads + gridDim.z - 1) / gridDim.z;
         const int h_end = min(heads, (int)(blockIdx.z + 1) * per);
+        // a long chunk's attention reads fp16 rows: write these while they are here
+        const int64_t exp_row = p.exp_k && p.cu_kv[b + 1] - p.cu_kv[b] == s.T + s.n ? p.cu_kv[b] : -1;
         int buf = 0;
         for (int hb = blockIdx.z * per; hb < h_end; hb += groups, buf ^= 1) {
             const int item = hb + grp;
@@ -248,6 +250,12 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                             w.y = e4m3x2(x[i][12] * up, x[i][13] * up) | (e4m3x2(x[i][14] * up, x[i][15] * up) << 16);
                             *reinterpret_cast<uint2*>(row + dlo) = u;
                             *reinterpret_cast<uint2*>(row + dhi) = w;
+                            if (exp_row >= 0) {
+                                __half* er = (is_v ? p.exp_v : p.exp_k) + h * p.exp_sh + (exp_row + pos) * D;
+                                const __half2 s2 = __float2half2_rn(exp2_int(ex));
+                                *reinterpret_cast<uint4*>(er + dlo) = expanded(u, s2, ex >= kScaleMax);
+                                *reinterpret_cast<uint4*>(er + dhi) = expanded(w, s2, ex >= kScaleMax);
+                            }
                         } else if (grows) {
                             for (int k = 0; k < 4; ++k) {
                                 uint32_t* w = reinterpret_cast<uint32_t*>(row + (k < 2 ? dlo : dhi) + (k & 1) * 4);
@@ -270,6 +278,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     __half* row = is_q ? p.q_rot + ((int64_t)(s.tok0 + pos - s.T) * p.Hq + h) * D
                                        : reinterpret_cast<__half*>(page + r * st);
                     store16(row, i);
+                    if (!is_q && exp_row >= 0)
+                        store16((is_v ? p.exp_v : p.exp_k) + h * p.exp_sh + (exp_row + pos) * D, i);
                 }
             }
         }

@@ -12,13 +12,21 @@ namespace pg {
 
 // ------------------------------------------------------------------ host side
 
-WsLayout ws_layout(int Hq, int Hkv, int D, int total_q, int max_q, int max_kv, int grid) {
+WsLayout ws_layout(int B, int Hq, int Hkv, int D, int total_q, int max_q, int max_kv, int grid) {
     auto up = [](size_t x) { return (x + 1023) & ~size_t(1023); };
     WsLayout w;
     w.part_lse = up(kHeadBytes);
     w.part_o = w.part_lse + up((size_t)2 * grid * kMaxCols * 4);
     w.q_rot = w.part_o + up((size_t)2 * grid * kMaxCols * D * 4);
-    w.total = w.q_rot + up((size_t)total_q * Hq * D * 2);
+    w.total = w.q_rot;
+    if (max_kv != 0 && long_chunk(Hq, Hkv, max_q)) {
+        w.cu_kv = w.q_rot + up((size_t)total_q * Hq * D * 2);
+        w.items = w.cu_kv + up((size_t)(B + 1) * 4);
+        w.expanded = w.items + up((size_t)max_items(B, Hq, max_q) * 16);
+        w.total = w.expanded + (max_kv > 0 ? up((size_t)max_kv * Hkv * D * 4) : 0);
+    } else {
+        w.cu_kv = w.items = w.expanded = w.total;
+    }
     return w;
 }
 
@@ -84,7 +92,9 @@ static int fill(const fcci_paged_desc* d, Op op, Params& p, Freqs& f, WsLayout& 
     if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
     const int sms = device_sm_count(dev);
     if (sms <= 0) return bad(FCCI_ECUDA, "no device");
-    L = ws_layout(d->Hq, d->Hkv, d->D, d->total_q, d->max_seqlen_q, op == Op::kPrefill ? d->max_kv_tokens : 0,
+    if (op == Op::kPrefill && max_items(d->B, d->Hq, d->max_seqlen_q) > 0x7fffffff)
+        return bad(FCCI_EINVAL, "prefill: too many work items");
+    L = ws_layout(d->B, d->Hq, d->Hkv, d->D, d->total_q, d->max_seqlen_q, op == Op::kPrefill ? d->max_kv_tokens : 0,
                   sms * kMaxCtasPerSm);
     if (!d->workspace || d->workspace_bytes < L.total) return bad(FCCI_EWORKSPACE, "workspace missing or too small");
     if (!aligned16(d->workspace)) return bad(FCCI_EINVAL, "workspace must be 16-byte aligned");
@@ -109,7 +119,7 @@ static int fill(const fcci_paged_desc* d, Op op, Params& p, Freqs& f, WsLayout& 
     p.seq_lens = d->seq_lens;
     p.out = static_cast<__half*>(d->out), p.o_st = d->out_stride_t, p.o_sh = d->out_stride_h;
     uint8_t* ws = static_cast<uint8_t*>(d->workspace);
-    p.q_rot = d->q_rot_out ? static_cast<__half*>(d->q_rot_out) : reinterpret_cast<__half*>(ws + L.q_rot);
+    p.q_rot = static_cast<__half*>(d->q_rot_out);
     p.scale_log2 = d->scale * 1.4426950408889634f;
     p.rot = d->rotary_dim;
     p.append = d->k_new ? 1 : 0;
@@ -145,7 +155,12 @@ static int paged_step(const fcci_paged_desc* d, Op op, cudaStream_t stream) {
         return launch_append(p, f, e4m3, stream);
     }
     uint8_t* ws = static_cast<uint8_t*>(d->workspace);
-    p.q_rot = static_cast<__half*>(d->q_rot_out);
+    if (op == Op::kPrefill && long_chunk(p.Hq, p.Hkv, p.max_q)) {
+        p.q_rot = reinterpret_cast<__half*>(ws + L.q_rot);
+        int64_t kv = d->max_kv_tokens;
+        if (kv < 0) kv = (int64_t)((d->workspace_bytes - L.expanded) / ((size_t)p.Hkv * p.D * 4));
+        return launch_prefill(p, f, e4m3, ws, L, (int)(kv < 0x7fffffff ? kv : 0x7fffffff), p.scale_log2, d->advance, stream);
+    }
     if (op == Op::kPrefill) {
         Params rows = p;
         rows.q = nullptr;
@@ -178,7 +193,7 @@ extern "C" size_t fcci_paged_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv,
         return 0;
     const int sms = fcci::device_sm_count(device);
     if (sms <= 0) return 0;
-    return fcci::pg::ws_layout(Hq, Hkv, D, total_q, max_seqlen_q, max_kv_tokens, sms * fcci::kMaxCtasPerSm).total;
+    return fcci::pg::ws_layout(B, Hq, Hkv, D, total_q, max_seqlen_q, max_kv_tokens, sms * fcci::kMaxCtasPerSm).total;
 }
 
 extern "C" int fcci_paged_workspace_init(void* workspace, size_t bytes, cudaStream_t stream) {

@@ -48,16 +48,15 @@
 #include "fcci_decode.h"
 #include "fcci_internal.h"
 #include "fcci_prefill.h"
+#include "prefill_list.cuh"
 #include "ptx.cuh"
 #include "tcgen05.cuh"
 
 namespace fcci {
 namespace pf {
 
-constexpr int D = 128;
 constexpr int kThreads = 384;
 constexpr int kTileRows = 128;
-constexpr int kPairRows = 256;
 constexpr int kTileBytes = kTileRows * D * 2;  // 32 KB: 128 rows x 128 fp16
 constexpr int kHalfBytes = kTileBytes / 2;     // one 64-column block
 // K tiles in flight: 2 (K_j + 1 is read one tile ahead of the PV of tile j). V tiles: 3. A
@@ -70,7 +69,6 @@ constexpr uint64_t kWaitLimitNs = 4000000000ull;  // 4 s: far beyond any healthy
 constexpr uint64_t kDrainLimitNs = 500000000ull;
 constexpr float kRescaleLog2 = 8.0f;
 constexpr uint32_t kTableMagic = 0x52504531u;  // "RPE1"
-constexpr int kMaxSortB = 1024;                 // sequences ranked by length up to this batch size
 constexpr int kPrepThreads = 256;
 
 // Column pairs of each 32-column slice of S whose exponentials run on the FMA
@@ -88,42 +86,6 @@ constexpr uint32_t kPolyMask = FCCI_PF_POLY_MASK;
 #define FCCI_PF_REG_SPLIT 1
 #endif
 constexpr int kRegsLow = 104, kRegsHigh = 200;
-
-struct Params {
-    const __half* q;
-    int64_t q_st, q_sh;
-    const __half* k_new;
-    int64_t kn_st, kn_sh;
-    const __half* v_new;
-    int64_t vn_st, vn_sh;
-    __half* k_cache;
-    int64_t k_sb, k_sh, k_st;
-    __half* v_cache;
-    int64_t v_sb, v_sh, v_st;
-    int32_t capacity;
-    const int32_t* cu_q;
-    const int32_t* cu_kv;
-    int32_t* seq_lens;
-    int32_t fixed_len;
-    __half* out;
-    int64_t o_st, o_sh;
-    float scale_log2;
-    float rope_theta;
-    int32_t rotary_dim;
-    int32_t advance;
-    int32_t B, Hq, Hkv, G, total_q, max_q;
-    int32_t table_pos;  // positions covered by the table (= capacity)
-    // workspace
-    uint32_t* err;
-    uint32_t* item_cnt;
-    uint32_t* exit_cnt;
-    int32_t* n_items;
-    uint32_t* table_hdr;  // magic, theta bits, rotary_dim, positions
-    uint32_t* table_cnt;
-    int4* items;
-    __half* q_rot;
-    float2* table;
-};
 
 struct WsLayout {
     size_t items, q_rot, table, total;
@@ -145,34 +107,6 @@ static WsLayout ws_layout(int B, int Hq, int total_q, int max_q, int capacity, i
 }
 
 // ------------------------------------------------------------------ device helpers
-
-struct SeqRange {
-    int T, n, tok0, kvrow0, kvb;
-    bool ok;
-};
-
-__device__ __forceinline__ SeqRange seq_range(const Params& p, int b) {
-    SeqRange s;
-    s.tok0 = p.cu_q[b];
-    s.n = p.cu_q[b + 1] - s.tok0;
-    s.T = p.seq_lens ? p.seq_lens[b] : p.fixed_len;
-    int cap = p.capacity;
-    bool ok = true;
-    if (p.cu_kv) {
-        const int lo = p.cu_kv[b], hi = p.cu_kv[b + 1];
-        s.kvrow0 = lo;
-        s.kvb = 0;
-        cap = hi - lo;
-        ok = lo >= 0 && hi >= lo && hi <= p.capacity;
-    } else {
-        s.kvrow0 = 0;
-        s.kvb = b;
-    }
-    ok = ok && s.T >= 0 && s.n >= 0 && s.n <= p.max_q && s.tok0 >= 0 && s.tok0 + s.n <= p.total_q &&
-         (long long)s.T + s.n <= cap;
-    s.ok = ok;
-    return s;
-}
 
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
     float d;
@@ -203,10 +137,6 @@ __device__ __forceinline__ float2 exp2_fma2(float2 x) {
     // field they add n to the exponent of p in [2^-1/2, 2^1/2]
     return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(j.x) << 23)),
                        __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(j.y) << 23)));
-}
-
-__device__ __forceinline__ void set_error(const Params& p, uint32_t bit) {
-    if (p.err) atomicOr(p.err, bit);
 }
 
 // RoPE angle and cos/sin exactly as the decode path (and the reference driver,
@@ -256,63 +186,6 @@ __global__ void __launch_bounds__(256) rope_table_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------ 2. prep
-
-// Work list: items (b, h, pair) sequence-major with sequences ranked by T_b + n_b
-// (longest first), then head, then pair from last to first. Also resets the
-// attention kernel's counters. One CTA.
-__device__ void build_work_list(const Params& p, int* sm) {
-    const int tid = threadIdx.x;
-    const int B = p.B;
-    int* np = sm;              // [B] pairs of sequence b (0 when invalid)
-    int* key = np + B;         // [B] ranking key
-    int* order = key + B;      // [B] rank -> b
-    int* off = order + B;      // [B+1] first item of rank r
-    for (int b = tid; b < B; b += blockDim.x) {
-        const SeqRange s = seq_range(p, b);
-        np[b] = s.ok ? (s.n + kPairRows - 1) / kPairRows : 0;
-        key[b] = s.ok ? s.T + s.n : -1;
-        order[b] = b;
-    }
-    __syncthreads();
-    if (B <= kMaxSortB) {
-        for (int b = tid; b < B; b += blockDim.x) {
-            const int kb = key[b];
-            int r = 0;
-            for (int o = 0; o < B; ++o) {
-                const int ko = key[o];
-                r += (ko > kb) || (ko == kb && o < b);
-            }
-            order[r] = b;
-        }
-        __syncthreads();
-    }
-    if (tid == 0) {
-        int acc = 0;
-        for (int r = 0; r < B; ++r) {
-            off[r] = acc;
-            acc += np[order[r]] * p.Hq;
-        }
-        off[B] = acc;
-        *p.n_items = acc;
-        *p.item_cnt = 0u;
-        *p.exit_cnt = 0u;
-    }
-    __syncthreads();
-    const int total = off[B];
-    for (int v = tid; v < total; v += blockDim.x) {
-        int lo = 0, hi = B - 1;  // last rank with off[r] <= v
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (off[mid] <= v) lo = mid; else hi = mid - 1;
-        }
-        const int b = order[lo];
-        const int n = np[b];
-        const int w = v - off[lo];
-        const int h = w / n;
-        const int pair = n - 1 - (w % n);
-        p.items[v] = make_int4(b, h, pair, 0);
-    }
-}
 
 // Last sequence b with cu_q[b] <= t.
 __device__ __forceinline__ int seq_of_row(const int32_t* cu, int B, int t) {
@@ -996,24 +869,12 @@ static int fill(const fcci_prefill_desc* d, Params& p, WsLayout& L) {
     return FCCI_OK;
 }
 
-// Validated launch state shared by the two halves of a step.
-struct Launch {
-    Params p;
-    WsLayout L;
-    int dev, sms;
-};
-
-static int setup(const fcci_prefill_desc* d, Launch& x) {
-    int rc = fill(d, x.p, x.L);
-    if (rc) return rc;
-    if (cudaGetDevice(&x.dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
-    x.sms = device_sm_count(x.dev);
-    if (x.sms <= 0) return set_status(FCCI_ECUDA, "fcci_prefill_attention: no device");
-    if (x.dev < 0 || x.dev >= 128) return set_status(FCCI_EINVAL, "fcci_prefill_attention: device index");
+// Kernel attributes of device `dev`, once; on failure records the reason and returns its FCCI_E* code.
+static int ready_device(int dev) {
+    if (dev < 0 || dev >= 128) return set_status(FCCI_EINVAL, "fcci_prefill_attention: device index");
     static std::once_flag flags[128];
     static cudaError_t attr_err[128];
     static bool regs_short[128];
-    const int dev = x.dev;
     std::call_once(flags[dev], [dev]() {
         attr_err[dev] =
             cudaFuncSetAttribute(prefill_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem::kAlloc);
@@ -1040,6 +901,22 @@ static int setup(const fcci_prefill_desc* d, Launch& x) {
     return FCCI_OK;
 }
 
+// Validated launch state shared by the two halves of a step.
+struct Launch {
+    Params p;
+    WsLayout L;
+    int dev, sms;
+};
+
+static int setup(const fcci_prefill_desc* d, Launch& x) {
+    int rc = fill(d, x.p, x.L);
+    if (rc) return rc;
+    if (cudaGetDevice(&x.dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
+    x.sms = device_sm_count(x.dev);
+    if (x.sms <= 0) return set_status(FCCI_ECUDA, "fcci_prefill_attention: no device");
+    return ready_device(x.dev);
+}
+
 // RoPE table check, RoPE + append of the new tokens, work list.
 int prefill_prepare(const fcci_prefill_desc* d, cudaStream_t stream) {
     Launch x;
@@ -1064,13 +941,13 @@ int prefill_prepare(const fcci_prefill_desc* d, cudaStream_t stream) {
     return set_cuda_status(cudaGetLastError());
 }
 
-// Causal attention over the work list written by prefill_prepare (same descriptor).
-int prefill_attend(const fcci_prefill_desc* d, cudaStream_t stream) {
-    Launch x;
-    int rc = setup(d, x);
+int launch_attend(const Params& p, int64_t max_items, cudaStream_t stream) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
+    const int sms = device_sm_count(dev);
+    if (sms <= 0) return set_status(FCCI_ECUDA, "fcci_prefill_attention: no device");
+    int rc = ready_device(dev);
     if (rc) return rc;
-    Params& p = x.p;
-    if (p.total_q == 0) return FCCI_OK;
     // tensor maps: rotated queries [total_q, Hq, D] (workspace) and the arena
     CUtensorMap mq, mk, mv;
     {
@@ -1089,11 +966,20 @@ int prefill_attend(const fcci_prefill_desc* d, cudaStream_t stream) {
         if (!rc) rc = encode_f16_sw128(&mv, p.v_cache, 4, dims, sbv, box);
     }
     if (rc) return set_status(rc, "fcci_prefill_attention: cuTensorMapEncodeTiled rejected a layout");
-    int grid = x.sms;
-    if (x.L.max_items < grid) grid = (int)(x.L.max_items > 0 ? x.L.max_items : 1);
+    int grid = sms;
+    if (max_items < grid) grid = (int)(max_items > 0 ? max_items : 1);
     prefill_attn_kernel<<<grid, kThreads, Smem::kAlloc, stream>>>(mq, mk, mv, p);
     count_launch();
     return set_cuda_status(cudaGetLastError());
+}
+
+// Causal attention over the work list written by prefill_prepare (same descriptor).
+int prefill_attend(const fcci_prefill_desc* d, cudaStream_t stream) {
+    Launch x;
+    int rc = setup(d, x);
+    if (rc) return rc;
+    if (x.p.total_q == 0) return FCCI_OK;
+    return launch_attend(x.p, x.L.max_items, stream);
 }
 
 }  // namespace pf
