@@ -126,7 +126,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
     constexpr int PL = D / 16;       // lanes per row
     constexpr int RP = 32 / PL;      // rows per pass
     constexpr int kWarps = kRowsThreads / 32;
-    extern __shared__ float2 cs_table[];  // [page][rot / 2]
+    // [page][4][rot / 16][2]: angles 8 j + 2 m, 8 j + 2 m + 1 of a row at [row][m][j], so that the lanes of a row, which
+    // have neighbouring j, read 16 neighbouring bytes each
+    extern __shared__ __align__(16) float2 cs_table[];
     __shared__ int flag;
     __shared__ float amax_sm[2][kWarps];
     griddep_launch_dependents();
@@ -142,7 +144,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
         const int half = p.rot >> 1;
         for (int i = tid; i < p.page * half; i += kRowsThreads) {
             const int r = i / half, k = i - r * half;
-            if (p0 + r >= s.T && p0 + r < s.T + s.n) cs_table[i] = rope_cs(f.turn[k], p0 + r);
+            if (p0 + r >= s.T && p0 + r < s.T + s.n)
+                cs_table[r * half + ((k >> 1) & 3) * (half >> 2) + (k >> 3) * 2 + (k & 1)] = rope_cs(f.turn[k], p0 + r);
         }
         const int id = page_of(p, b, p0);
         __syncthreads();
@@ -197,17 +200,24 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                 const int r = row0 + i * RP, pos = p0 + r;
                 const bool fresh = r < p.page && pos >= s.T && pos < s.T + s.n;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float u = __half2float(a[e]), w = __half2float(c[e]);
-                    if (turn_j && !is_v && fresh) {
-                        const float2 cs = cs_table[r * half + dlo + e];
-                        const float t = rotated(u, w, cs, true);
-                        w = rotated(w, u, cs, false);
-                        u = t;
+                for (int m = 0; m < 4; ++m) {
+                    float4 cs = make_float4(1.f, 0.f, 1.f, 0.f);
+                    const bool turn = turn_j && !is_v && fresh;
+                    if (turn) cs = *reinterpret_cast<const float4*>(&cs_table[r * half + m * (half >> 2) + j * 2]);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int e = 2 * m + k;
+                        float u = __half2float(a[e]), w = __half2float(c[e]);
+                        if (turn) {
+                            const float2 c2 = k ? make_float2(cs.z, cs.w) : make_float2(cs.x, cs.y);
+                            const float t = rotated(u, w, c2, true);
+                            w = rotated(w, u, c2, false);
+                            u = t;
+                        }
+                        x[i][e] = u;
+                        x[i][8 + e] = w;
+                        amax = fmaxf(amax, fmaxf(fabsf(u), fabsf(w)));
                     }
-                    x[i][e] = u;
-                    x[i][8 + e] = w;
-                    amax = fmaxf(amax, fmaxf(fabsf(u), fabsf(w)));
                 }
             }
             auto store16 = [&](__half* row, int i) {
@@ -225,11 +235,11 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                 // old rows of the call's first page keep (or grow) the page's scale
                 const bool old = p0 < s.T;
                 const int had = old && sp ? (int)*sp - 127 : -1000;
-                if (W > 1) {
+                if (W > 1 && work && !is_q) {
                     // every warp of the page has read the old scale before this barrier;
                     // two buffers: a warp may be one head ahead of another's reads
                     if (lane == 0) amax_sm[buf][warp] = amax;
-                    __syncthreads();
+                    named_bar_sync(1 + grp, 32 * W);
                     for (int w = 0; w < W; ++w) amax = fmaxf(amax, amax_sm[buf][grp * W + w]);
                 }
                 if (work && !is_q) {
