@@ -126,9 +126,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
     constexpr int PL = D / 16;       // lanes per row
     constexpr int RP = 32 / PL;      // rows per pass
     constexpr int kWarps = kRowsThreads / 32;
-    // [page][4][rot / 16][2]: angles 8 j + 2 m, 8 j + 2 m + 1 of a row at [row][m][j], so that the lanes of a row, which
-    // have neighbouring j, read 16 neighbouring bytes each
-    extern __shared__ __align__(16) float2 cs_table[];
+    // [page][4][rot / 16]: (cos, cos, sin, sin) of angles 8 j + 2 m and 8 j + 2 m + 1 of a row at [row][m][j], so that the
+    // lanes of a row, which have neighbouring j, read 16 neighbouring bytes each
+    extern __shared__ float4 cs_table[];
     __shared__ int flag;
     __shared__ float amax_sm[2][kWarps];
     griddep_launch_dependents();
@@ -144,8 +144,12 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
         const int half = p.rot >> 1;
         for (int i = tid; i < p.page * half; i += kRowsThreads) {
             const int r = i / half, k = i - r * half;
-            if (p0 + r >= s.T && p0 + r < s.T + s.n)
-                cs_table[r * half + ((k >> 1) & 3) * (half >> 2) + (k >> 3) * 2 + (k & 1)] = rope_cs(f.turn[k], p0 + r);
+            if (p0 + r >= s.T && p0 + r < s.T + s.n) {
+                const float2 cs = rope_cs(f.turn[k], p0 + r);
+                float* at = reinterpret_cast<float*>(&cs_table[r * (half >> 1) + ((k >> 1) & 3) * (half >> 3) + (k >> 3)]);
+                at[k & 1] = cs.x;
+                at[2 + (k & 1)] = cs.y;
+            }
         }
         const int id = page_of(p, b, p0);
         __syncthreads();
@@ -163,6 +167,15 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
         const int h_end = min(heads, (int)(blockIdx.z + 1) * per);
         // a long chunk's attention reads fp16 rows: write these while they are here
         const int64_t exp_row = p.exp_k && p.cu_kv[b + 1] - p.cu_kv[b] == s.T + s.n ? p.cu_kv[b] : -1;
+        // passes whose row is new, and those whose row the page held before
+        uint32_t is_new = 0, is_old = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = row0 + i * RP, pos = p0 + r;
+            if (r < p.page && pos >= s.T && pos < s.T + s.n) is_new |= 1u << i;
+            if (r < p.page && pos < s.T) is_old |= 1u << i;
+        }
+        const int64_t src_row = s.tok0 + p0 + row0 - s.T;
         int buf = 0;
         for (int hb = blockIdx.z * per; hb < h_end; hb += groups, buf ^= 1) {
             const int item = hb + grp;
@@ -180,54 +193,42 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     sp = is_v ? p.v_scales + id * p.vs_sp + h * p.vs_sh : p.k_scales + id * p.ks_sp + h * p.ks_sh;
             }
             const bool work = live && (is_q || page);
-            float x[4][16];
+            float2 x[4][8];
             float amax = 0.f;
             uint4 lo[4], hi[4];
+            src += src_row * sst;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int pos = p0 + row0 + i * RP;
                 lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
-                if (work && row0 + i * RP < p.page && pos >= s.T && pos < s.T + s.n) {
-                    const __half* a = src + (int64_t)(s.tok0 + pos - s.T) * sst;
-                    lo[i] = *reinterpret_cast<const uint4*>(a + dlo);
-                    hi[i] = *reinterpret_cast<const uint4*>(a + dhi);
+                if (work && (is_new >> i & 1)) {
+                    lo[i] = *reinterpret_cast<const uint4*>(src + i * RP * sst + dlo);
+                    hi[i] = *reinterpret_cast<const uint4*>(src + i * RP * sst + dhi);
                 }
             }
+            const bool turn = turn_j && !is_v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const __half* a = reinterpret_cast<const __half*>(&lo[i]);
-                const __half* c = reinterpret_cast<const __half*>(&hi[i]);
-                const int r = row0 + i * RP, pos = p0 + r;
-                const bool fresh = r < p.page && pos >= s.T && pos < s.T + s.n;
+                const __half2* a = reinterpret_cast<const __half2*>(&lo[i]);
+                const __half2* c = reinterpret_cast<const __half2*>(&hi[i]);
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
-                    float4 cs = make_float4(1.f, 0.f, 1.f, 0.f);
-                    const bool turn = turn_j && !is_v && fresh;
-                    if (turn) cs = *reinterpret_cast<const float4*>(&cs_table[r * half + m * (half >> 2) + j * 2]);
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int e = 2 * m + k;
-                        float u = __half2float(a[e]), w = __half2float(c[e]);
-                        if (turn) {
-                            const float2 c2 = k ? make_float2(cs.z, cs.w) : make_float2(cs.x, cs.y);
-                            const float t = rotated(u, w, c2, true);
-                            w = rotated(w, u, c2, false);
-                            u = t;
-                        }
-                        x[i][e] = u;
-                        x[i][8 + e] = w;
-                        amax = fmaxf(amax, fmaxf(fabsf(u), fabsf(w)));
+                    float2 u = __half22float2(a[m]), w = __half22float2(c[m]);
+                    if (turn && (is_new >> i & 1)) {
+                        const float4 cs = cs_table[(row0 + i * RP) * (half >> 1) + m * (half >> 3) + j];
+                        const float2 co = make_float2(cs.x, cs.y), si = make_float2(cs.z, cs.w);
+                        const float2 y = __fmul2_rn(w, si), z = __fmul2_rn(u, si);
+                        u = __ffma2_rn(u, co, make_float2(-y.x, -y.y));
+                        w = __ffma2_rn(w, co, z);
                     }
+                    x[i][m] = u;
+                    x[i][4 + m] = w;
+                    if (E4M3) amax = fmaxf(fmaxf(amax, fmaxf(fabsf(u.x), fabsf(u.y))), fmaxf(fabsf(w.x), fabsf(w.y)));
                 }
             }
             auto store16 = [&](__half* row, int i) {
-                uint4 u, w;
-                u.x = pack_half2(x[i][0], x[i][1]), u.y = pack_half2(x[i][2], x[i][3]);
-                u.z = pack_half2(x[i][4], x[i][5]), u.w = pack_half2(x[i][6], x[i][7]);
-                w.x = pack_half2(x[i][8], x[i][9]), w.y = pack_half2(x[i][10], x[i][11]);
-                w.z = pack_half2(x[i][12], x[i][13]), w.w = pack_half2(x[i][14], x[i][15]);
-                *reinterpret_cast<uint4*>(row + dlo) = u;
-                *reinterpret_cast<uint4*>(row + dhi) = w;
+                auto two = [](float2 v) { return pack_half2(v.x, v.y); };
+                *reinterpret_cast<uint4*>(row + dlo) = make_uint4(two(x[i][0]), two(x[i][1]), two(x[i][2]), two(x[i][3]));
+                *reinterpret_cast<uint4*>(row + dhi) = make_uint4(two(x[i][4]), two(x[i][5]), two(x[i][6]), two(x[i][7]));
             };
             if constexpr (E4M3) {
 #pragma unroll
@@ -247,17 +248,18 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     const bool grows = old && ex > had;
                     ex = max(ex, had);
                     const float up = exp2_int(-ex), down = grows ? exp2_int(max(had, -126) - ex) : 1.f;
+                    const float2 up2 = make_float2(up, up);
+                    auto four = [&](float2 u, float2 w) {
+                        u = __fmul2_rn(u, up2), w = __fmul2_rn(w, up2);
+                        return e4m3x2(u.x, u.y) | (e4m3x2(w.x, w.y) << 16);
+                    };
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int r = row0 + i * RP, pos = p0 + r;
-                        if (r >= p.page || pos >= s.T + s.n) continue;
-                        uint8_t* row = page + r * st;
-                        if (pos >= s.T) {
-                            uint2 u, w;
-                            u.x = e4m3x2(x[i][0] * up, x[i][1] * up) | (e4m3x2(x[i][2] * up, x[i][3] * up) << 16);
-                            u.y = e4m3x2(x[i][4] * up, x[i][5] * up) | (e4m3x2(x[i][6] * up, x[i][7] * up) << 16);
-                            w.x = e4m3x2(x[i][8] * up, x[i][9] * up) | (e4m3x2(x[i][10] * up, x[i][11] * up) << 16);
-                            w.y = e4m3x2(x[i][12] * up, x[i][13] * up) | (e4m3x2(x[i][14] * up, x[i][15] * up) << 16);
+                        uint8_t* row = page + (row0 + i * RP) * st;
+                        if (is_new >> i & 1) {
+                            const int pos = p0 + row0 + i * RP;
+                            const uint2 u = make_uint2(four(x[i][0], x[i][1]), four(x[i][2], x[i][3]));
+                            const uint2 w = make_uint2(four(x[i][4], x[i][5]), four(x[i][6], x[i][7]));
                             *reinterpret_cast<uint2*>(row + dlo) = u;
                             *reinterpret_cast<uint2*>(row + dhi) = w;
                             if (exp_row >= 0) {
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                                 *reinterpret_cast<uint4*>(er + dlo) = expanded(u, s2, ex >= kScaleMax);
                                 *reinterpret_cast<uint4*>(er + dhi) = expanded(w, s2, ex >= kScaleMax);
                             }
-                        } else if (grows) {
+                        } else if (grows && (is_old >> i & 1)) {
                             for (int k = 0; k < 4; ++k) {
                                 uint32_t* w = reinterpret_cast<uint32_t*>(row + (k < 2 ? dlo : dhi) + (k & 1) * 4);
                                 const uint32_t c = *w;
@@ -283,10 +285,10 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
             if (work && (is_q || !E4M3)) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int r = row0 + i * RP, pos = p0 + r;
-                    if (r >= p.page || pos < s.T || pos >= s.T + s.n) continue;
-                    __half* row = is_q ? p.q_rot + ((int64_t)(s.tok0 + pos - s.T) * p.Hq + h) * D
-                                       : reinterpret_cast<__half*>(page + r * st);
+                    if (!(is_new >> i & 1)) continue;
+                    const int pos = p0 + row0 + i * RP;
+                    __half* row = is_q ? p.q_rot + ((src_row + i * RP) * p.Hq + h) * D
+                                       : reinterpret_cast<__half*>(page + (row0 + i * RP) * st);
                     store16(row, i);
                     if (!is_q && exp_row >= 0)
                         store16((is_v ? p.exp_v : p.exp_k) + h * p.exp_sh + (exp_row + pos) * D, i);
