@@ -176,6 +176,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
             if (r < p.page && pos < s.T) is_old |= 1u << i;
         }
         const int64_t src_row = s.tok0 + p0 + row0 - s.T;
+        const int ahead_pos = p0 + part * R + lane / (D / 64);
+        const int64_t ahead_row = s.tok0 + ahead_pos - s.T;
+        const bool ahead = ahead_pos >= s.T && ahead_pos < s.T + s.n && ahead_pos < p0 + p.page;
         int buf = 0;
         for (int hb = blockIdx.z * per; hb < h_end; hb += groups, buf ^= 1) {
             const int item = hb + grp;
@@ -204,6 +207,15 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     lo[i] = *reinterpret_cast<const uint4*>(src + i * RP * sst + dlo);
                     hi[i] = *reinterpret_cast<const uint4*>(src + i * RP * sst + dhi);
                 }
+            }
+            // the warp's next item on its way into L2 (its rows are 32 lines of 128 bytes, one a lane): the registers are full
+            if (item + groups < h_end && ahead) {
+                const int nx = item + groups;
+                const bool nq = nx >= 2 * p.Hkv, nv = !nq && nx >= p.Hkv;
+                const int nh = nq ? nx - 2 * p.Hkv : (nv ? nx - p.Hkv : nx);
+                const __half* a = nq ? p.q + nh * p.q_sh : (nv ? p.v_new + nh * p.vn_sh : p.k_new + nh * p.kn_sh);
+                a += ahead_row * (nq ? p.q_st : (nv ? p.vn_st : p.kn_st)) + (lane % (D / 64)) * 64;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(a));
             }
             const bool turn = turn_j && !is_v;
 #pragma unroll
