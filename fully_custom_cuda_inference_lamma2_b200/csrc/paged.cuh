@@ -108,8 +108,10 @@ __device__ __forceinline__ uint32_t e4m3x2_of_half2(uint32_t h) {
     return c;
 }
 
-__device__ __forceinline__ uint32_t half2_minus(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+// 16 (a - b), exact where b is the e4m3 rounding of a
+__device__ __forceinline__ uint32_t half2_rest16(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b)),
+                              __float2half2_rn(16.f));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 

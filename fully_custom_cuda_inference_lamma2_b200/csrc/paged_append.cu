@@ -13,97 +13,122 @@
 namespace fcci {
 namespace pg {
 
-constexpr int kTokenThreads = 256;
+constexpr int kTokenWarps = 16, kTokenThreads = kTokenWarps * 32;
+constexpr int kTokenTasks = 4;  // rows of a warp, at most
 
-// One token per sequence. A warp takes one row (a query head, or the key or value of a kv
-// head): few rows in all, so the rows spread over as many warps as there are, and the chain
-// length -> page -> scale is what the time goes into.
+// One token per sequence. A warp takes `tasks` rows (query heads, or the key or value of a kv head): one when there are few
+// sequences, so that the rows spread over as many warps as there are, else up to four, whose loads are
+// under way together while the CTA gets through the chain length -> page -> scale and the angles, which all rows share.
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(kTokenThreads) paged_append_token_kernel(const __grid_constant__ Params p,
-                                                                         const __grid_constant__ Freqs f) {
+                                                                         const __grid_constant__ Freqs f, int tasks) {
     constexpr int E = D / 32;  // elements of a row per lane
     __shared__ int flag;
+    __shared__ float2 cs[D / 2];
+    const int half = p.rot >> 1;
+    const uint64_t turn = threadIdx.x < half ? f.turn[threadIdx.x] : 0;  // a launch constant: read before the wait
     griddep_launch_dependents();
     griddep_wait();
-    const int b = blockIdx.x;
-    const int lane = threadIdx.x & 31;
-    const int task = blockIdx.y * (kTokenThreads / 32) + (threadIdx.x >> 5);
-    const int nkv = p.append ? 2 * p.Hkv : 0;
-    const Seq s = seq_of(p, b);
-    if (!s.ok) {
-        if (task == 0 && lane == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
-    } else if (task < nkv + (p.q ? p.Hq : 0)) {
+    const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int nkv = 2 * p.Hkv, all = nkv + (p.q ? p.Hq : 0);
+    const int d0 = lane * E;
+    const bool first = d0 < half;
+    __align__(16) __half raw[kTokenTasks][E], other[kTokenTasks][E];
+    auto load = [](__half(&dst)[E], const __half* a) {
+        if constexpr (E == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(a);
+        else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(a);
+        else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(a);
+    };
+    const int task0 = blockIdx.y * tasks * kTokenWarps + warp;  // task k: + k * kTokenWarps
+#pragma unroll
+    for (int k = 0; k < kTokenTasks; ++k) {
+        const int task = task0 + k * kTokenWarps;
+        if (k >= tasks || task >= all) continue;
         const bool is_q = task >= nkv, is_v = !is_q && task >= p.Hkv;
         const int h = is_q ? task - nkv : (is_v ? task - p.Hkv : task);
         const __half* src = is_q ? p.q + b * p.q_st + h * p.q_sh
                                  : (is_v ? p.v_new + b * p.vn_st + h * p.vn_sh : p.k_new + b * p.kn_st + h * p.kn_sh);
-        const int d0 = lane * E, half = p.rot >> 1;
-        float x[E];
-        __align__(16) __half raw[E], other[E];
-        auto load = [](__half(&dst)[E], const __half* a) {
-            if constexpr (E == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(a);
-            else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(a);
-            else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(a);
-        };
-        load(raw, src + d0);
-        const bool turn = !is_v && d0 < p.rot, first = d0 < half;
-        if (turn) load(other, src + (first ? d0 + half : d0 - half));
+        load(raw[k], src + d0);
+        if (!is_v && d0 < p.rot) load(other[k], src + (first ? d0 + half : d0 - half));
+    }
+    const Seq s = seq_of(p, b);
+    if (!s.ok) {
+        if (blockIdx.y == 0 && threadIdx.x == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
+    } else {
+        const bool kv_here = blockIdx.y * tasks * kTokenWarps < nkv;  // the CTA has a key or a value
+        const int id = kv_here ? page_of(p, b, s.T) : -1;
+        if (threadIdx.x < half) cs[threadIdx.x] = rope_cs(turn, s.T);
+        const int off = s.T & (p.page - 1);
+        int had[kTokenTasks];
+        uint8_t* sp[kTokenTasks];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            x[e] = __half2float(raw[e]);
-            if (turn) {
-                const float2 cs = rope_cs(f.turn[(first ? d0 : d0 - half) + e], s.T);
-                x[e] = rotated(x[e], __half2float(other[e]), cs, first);
-            }
+        for (int k = 0; k < kTokenTasks; ++k) {
+            const int task = task0 + k * kTokenWarps;
+            had[k] = -1000;  // a fresh page has no scale yet
+            sp[k] = nullptr;
+            if (!E4M3 || k >= tasks || task >= nkv || id < 0) continue;
+            const int h = task >= p.Hkv ? task - p.Hkv : task;
+            sp[k] = task >= p.Hkv ? p.v_scales + id * p.vs_sp + h * p.vs_sh : p.k_scales + id * p.ks_sp + h * p.ks_sh;
+            if (off) had[k] = (int)*sp[k] - 127;
         }
-        auto store16 = [&](__half* dst) {
+        __syncthreads();
 #pragma unroll
-            for (int e = 0; e < E; e += 2)
-                *reinterpret_cast<uint32_t*>(dst + d0 + e) = pack_half2(x[e], x[e + 1]);
-        };
-        if (is_q) {
-            store16(p.q_rot + ((int64_t)b * p.Hq + h) * D);
-        } else {
-            const int id = page_of(p, b, s.T);
-            if (id >= 0) {
-                const int off = s.T & (p.page - 1);
-                uint8_t* page = is_v ? p.v_pages + id * p.v_sp + h * p.v_sh : p.k_pages + id * p.k_sp + h * p.k_sh;
-                const int64_t st = is_v ? p.v_st : p.k_st;
-                if constexpr (!E4M3) {
-                    store16(reinterpret_cast<__half*>(page + off * st));
-                } else {
-                    uint8_t* sp = is_v ? p.v_scales + id * p.vs_sp + h * p.vs_sh : p.k_scales + id * p.ks_sp + h * p.ks_sh;
-                    const int had = off ? (int)*sp - 127 : -1000;  // a fresh page has no scale yet
-                    float amax = 0.f;
+        for (int k = 0; k < kTokenTasks; ++k) {
+            const int task = task0 + k * kTokenWarps;
+            if (k >= tasks || task >= all) continue;
+            const bool is_q = task >= nkv, is_v = !is_q && task >= p.Hkv;
+            const int h = is_q ? task - nkv : (is_v ? task - p.Hkv : task);
+            float x[E];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[e]));
+            for (int e = 0; e < E; ++e) {
+                x[e] = __half2float(raw[k][e]);
+                if (!is_v && d0 < p.rot)
+                    x[e] = rotated(x[e], __half2float(other[k][e]), cs[(first ? d0 : d0 - half) + e], first);
+            }
+            auto store16 = [&](__half* dst) {
 #pragma unroll
-                    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                    int ex = scale_exponent(amax);
-                    if (off && ex > had) {
-                        // the rows before this one take the larger scale (rare: the page's largest value grew past a power of two)
-                        const float down = exp2_int(max(had, -126) - ex);
-                        for (int i = lane; i < off * (D / 4); i += 32) {
-                            uint32_t* w = reinterpret_cast<uint32_t*>(page + (i / (D / 4)) * st + (i % (D / 4)) * 4);
-                            const uint32_t c = *w;
-                            const uint32_t lo = half2_of_e4m3x2(c & 0xffffu), hi = half2_of_e4m3x2(c >> 16);
-                            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-                            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                            *w = e4m3x2(a.x * down, a.y * down) | (e4m3x2(g.x * down, g.y * down) << 16);
-                        }
+                for (int e = 0; e < E; e += 2)
+                    *reinterpret_cast<uint32_t*>(dst + d0 + e) = pack_half2(x[e], x[e + 1]);
+            };
+            if (is_q) {
+                store16(p.q_rot + ((int64_t)b * p.Hq + h) * D);
+                continue;
+            }
+            if (id < 0) continue;
+            uint8_t* page = is_v ? p.v_pages + id * p.v_sp + h * p.v_sh : p.k_pages + id * p.k_sp + h * p.k_sh;
+            const int64_t st = is_v ? p.v_st : p.k_st;
+            if constexpr (!E4M3) {
+                store16(reinterpret_cast<__half*>(page + off * st));
+            } else {
+                float amax = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(x[e]));
+#pragma unroll
+                for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                int ex = scale_exponent(amax);
+                if (off && ex > had[k]) {
+                    // the rows before this one take the larger scale (rare: the page's largest value grew past a power of two)
+                    const float down = exp2_int(max(had[k], -126) - ex);
+                    for (int i = lane; i < off * (D / 4); i += 32) {
+                        uint32_t* w = reinterpret_cast<uint32_t*>(page + (i / (D / 4)) * st + (i % (D / 4)) * 4);
+                        const uint32_t c = *w;
+                        const uint32_t lo = half2_of_e4m3x2(c & 0xffffu), hi = half2_of_e4m3x2(c >> 16);
+                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+                        const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                        *w = e4m3x2(a.x * down, a.y * down) | (e4m3x2(g.x * down, g.y * down) << 16);
                     }
-                    ex = max(ex, had);
-                    const float up = exp2_int(-ex);
-                    if constexpr (E == 2) {
-                        *reinterpret_cast<uint16_t*>(page + off * st + d0) = (uint16_t)e4m3x2(x[0] * up, x[1] * up);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < E; e += 4)
-                            *reinterpret_cast<uint32_t*>(page + off * st + d0 + e) =
-                                e4m3x2(x[e] * up, x[e + 1] * up) | (e4m3x2(x[e + 2] * up, x[e + 3] * up) << 16);
-                    }
-                    if (lane == 0) *sp = (uint8_t)(ex + 127);
                 }
+                ex = max(ex, had[k]);
+                const float up = exp2_int(-ex);
+                if constexpr (E == 2) {
+                    *reinterpret_cast<uint16_t*>(page + off * st + d0) = (uint16_t)e4m3x2(x[0] * up, x[1] * up);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; e += 4)
+                        *reinterpret_cast<uint32_t*>(page + off * st + d0 + e) =
+                            e4m3x2(x[e] * up, x[e + 1] * up) | (e4m3x2(x[e + 2] * up, x[e + 3] * up) << 16);
+                }
+                if (lane == 0) *sp[k] = (uint8_t)(ex + 127);
             }
         }
     }
@@ -313,11 +338,13 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
 
 template <int D, bool E4M3>
 static int launch_append_t(const Params& p, const Freqs& f, cudaStream_t st) {
-    const int heads = (p.q ? p.Hq : 0) + (p.append ? 2 * p.Hkv : 0);
+    const int heads = (p.q ? p.Hq : 0) + 2 * p.Hkv;
     if (!p.cu_q) {
-        const int per = kTokenThreads / 32;
-        return launch_pdl(paged_append_token_kernel<D, E4M3>, dim3(p.B, (heads + per - 1) / per), dim3(kTokenThreads), 0,
-                          st, p, f);
+        // one row a warp while that fits the GPU at once (4 CTAs an SM), else as many as it takes, up to four
+        int tasks = 1;
+        while (tasks < kTokenTasks && (int64_t)p.B * ((heads + tasks * kTokenWarps - 1) / (tasks * kTokenWarps)) > 4 * 148) ++tasks;
+        const int y = (heads + tasks * kTokenWarps - 1) / (tasks * kTokenWarps);
+        return launch_pdl(paged_append_token_kernel<D, E4M3>, dim3(p.B, y), dim3(kTokenThreads), 0, st, p, f, tasks);
     }
     // pages that the longest run of new tokens can touch, and a head split that fills the GPU
     // when there are few pages

@@ -5,12 +5,13 @@
 // The e4m3 codes go into tcgen05 (kind::f8f6f4, fp32 sums) as they lie in shared memory. With mma.sync they would
 // have to become fp16 in registers first, and that conversion unit (16 lanes a cycle and SM, for 2 codes each)
 // bound that kernel at 59 % of the memory rate. The other operand keeps its precision as a sum of
-// three e4m3 values, each the rounding of what the ones before left (within 2^-12 of it), as three rows of the
-// same product:
+// three e4m3 values, p0 + p1 / 16 + p2 / 256, each the rounding of what the ones before left, times 16 (within 2^-12 of
+// the value, or 2^-18 absolute), as three rows of the same product:
 //   S^T[key, (part, row)] = K Q^T     A = the K tile (128 keys), B = 3 * COLS rows of query parts
 //   O^T[dim, (part, row)] += V^T P^T  A = the V tile read dim-major, B = the weight parts, 3 * COLS bytes of each
 //                                     key side by side (N-major), which is what the key's thread has
-// The parts are summed where S is read, and where O is read at a unit's end.
+// The parts are summed where S is read, and where O is read at a unit's end. (Unscaled parts would lose every weight below
+// 2^-16 of the largest: the many small ones beside a key that takes most of the attention.)
 //   - A query row is rotated in fp32 and scaled by a power of two to at most 448 before it is split.
 //   - Thread t of the softmax owns key t of the tile: its scales are its own numbers. The exponent of V's scale
 //     joins the score, x = s + log2 vs, so the weight that multiplies the codes is 2^(x - m), and no
@@ -50,6 +51,7 @@ struct TcCfg {
     static constexpr int PB = kTcKeys * PW;             // bytes of a weight buffer
     // shared memory behind the stages
     static constexpr int kP = QB, kSmall = QB + 2 * PB;  // queries, two weight buffers, the rest
+    static_assert(2 * PB >= COLS * (kTcD / 2) * 8, "angles of COLS tokens in the weight buffers");
     static size_t smem(int stages, int B) {
         return 1024 + (size_t)stages * 2 * TL::BYTES + kSmall + 64 * 8 /* cos, sin */ + 8 * COLS * 4 /* maxima, sums */ +
                COLS * 4 /* query scales */ + kMaxStages * 64 /* page scales */ + 256 /* barriers */ + 64 +
@@ -66,6 +68,10 @@ __device__ __forceinline__ float redux_max(float x) {
     float y;
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float of_parts(uint32_t a, uint32_t b, uint32_t c) {
+    return fmaf(__uint_as_float(c), 1.f / 256.f, fmaf(__uint_as_float(b), 1.f / 16.f, __uint_as_float(a)));
 }
 
 // Whether any of the computing threads says so (all of them take part).
@@ -255,8 +261,20 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                         if (d < rot) yr[k] = *reinterpret_cast<const uint2*>(q + (d < half ? d + half : d - half));
                     }
                 }
-                if (!p.cu_q && rot > 0) {  // while the loads are under way
-                    if (tid < half) cs[tid] = rope_cs(turn, max(T, 0));
+                // ---- angles, while the loads are under way: of position T, or of each of the unit's tokens (the weight
+                // buffers hold them: the last product that read those has completed)
+                const int i0 = r0 / G;
+                const float2* angles = cs;
+                if (rot > 0) {
+                    if (!p.cu_q) {
+                        if (tid < half) cs[tid] = rope_cs(turn, max(T, 0));
+                    } else {
+                        float2* table = reinterpret_cast<float2*>(p_sm);
+                        const int ntok = (r0 + rows - 1) / G - i0 + 1;
+                        for (int x = warp; x < ntok; x += kComputeWarps)
+                            for (int k = lane; k < half; k += 32) table[x * half + k] = rope_cs(f.turn[k], T + i0 + x);
+                        angles = table;
+                    }
                     named_bar_sync(kBar, kCompute);
                 }
 #pragma unroll
@@ -270,8 +288,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                         x[e] = __half2float(a[e]);
                         if (d < rot && c < rows) {
                             const int t = (d < half ? d : d - half) + e;
-                            const float2 w = p.cu_q ? rope_cs(f.turn[t], T + i) : cs[t];
-                            x[e] = rotated(x[e], __half2float(y[e]), w, d < half);
+                            x[e] = rotated(x[e], __half2float(y[e]), angles[(i - i0) * half + t], d < half);
                         }
                         amax = fmaxf(amax, fabsf(x[e]));
                     }
@@ -291,7 +308,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                         const uint32_t bl = half2_of_e4m3x2(lo), bh = half2_of_e4m3x2(hi);
                         const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&bl));
                         const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&bh));
-                        x[0] -= u.x, x[1] -= u.y, x[2] -= v.x, x[3] -= v.y;
+                        x[0] = (x[0] - u.x) * 16.f, x[1] = (x[1] - u.y) * 16.f;
+                        x[2] = (x[2] - v.x) * 16.f, x[3] = (x[3] - v.y) * 16.f;
                     }
                 }
                 fence_proxy_async_smem();
@@ -345,7 +363,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 if (lane == 0) mbar_arrive(&bar->s_free[it & 1]);
 #pragma unroll
                 for (int c = 0; c < COLS; ++c) {
-                    const float sum = __uint_as_float(a[c]) + (__uint_as_float(a[COLS + c]) + __uint_as_float(a[2 * COLS + c]));
+                    const float sum = of_parts(a[c], a[COLS + c], a[2 * COLS + c]);
                     x[c] = fmaf(sum * ks, qf[c], lv);
                 }
             }
@@ -416,7 +434,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 for (int part = 0; part < 3; ++part) {
                     const uint32_t v0 = e4m3x2_of_half2(h0), v1 = e4m3x2_of_half2(h1);
                     w[(part * COLS + c) / 4] = v0 | (v1 << 16);
-                    if (part < 2) h0 = half2_minus(h0, half2_of_e4m3x2(v0)), h1 = half2_minus(h1, half2_of_e4m3x2(v1));
+                    if (part < 2) h0 = half2_rest16(h0, half2_of_e4m3x2(v0)), h1 = half2_rest16(h1, half2_of_e4m3x2(v1));
                 }
             }
             if (it >= 2) wait(&bar->p_free[it & 1], (it >> 1) - 1);
@@ -459,7 +477,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 for (int c = 0; c < COLS; ++c) {
                     if (c >= rows) continue;
                     const float sum = (l_sm[c] + l_sm[COLS + c]) + (l_sm[2 * COLS + c] + l_sm[3 * COLS + c]);
-                    const float o = __uint_as_float(a[c]) + (__uint_as_float(a[COLS + c]) + __uint_as_float(a[2 * COLS + c]));
+                    const float o = of_parts(a[c], a[COLS + c], a[2 * COLS + c]);
                     const float y = sum > 0.f ? o / sum : 0.f;
                     if (whole) {
                         out_row(p, at, r0, c)[tid] = __float2half_rn(y);

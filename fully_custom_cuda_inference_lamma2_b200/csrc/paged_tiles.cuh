@@ -69,8 +69,9 @@ template <int KEYS, int COLS>
 struct Line {
     const TileParams& tp;
     int *base, *T, *n;  // shared: [B + 1] tiles before a sequence; cached rows (-1: not served), new tokens
-    long long N, CT, t0;  // tiles in all, CTAs that take some, this CTA's first
-    int ntiles;
+    unsigned N, CT;     // tiles in all, CTAs that take some
+    unsigned per, more;  // N / CT and N % CT
+    int ntiles;         // of this CTA
 
     static size_t ints(int B) { return 3 * (size_t)B + 1; }
     __device__ Line(const TileParams& tp_, int* sm) : tp(tp_), base(sm), T(sm + tp_.p.B + 1), n(T + tp_.p.B) {}
@@ -134,35 +135,32 @@ struct Line {
         for (int b = lo; b < hi; ++b) base[b + 1] = run += base[b + 1];
         uniform = __syncthreads_and(uniform) != 0;
 
-        N = base[B];
-        CT = N < (long long)gridDim.x ? N : (long long)gridDim.x;
+        N = (unsigned)base[B];
+        CT = min(N, gridDim.x);
         if (uniform && N > 0) {
             // equal units: a number of CTAs that is a multiple of the units keeps every cut at the same
             // places of each, unless that leaves more than 15 % of the grid idle
-            const long long units = (long long)B * p.Hkv * groups(n[0]);
-            if (units <= (long long)gridDim.x) {
-                const long long k = min((long long)gridDim.x / units, N / units);
+            const unsigned units = (unsigned)B * p.Hkv * groups(n[0]);  // at most N
+            if (units > 0 && units <= gridDim.x) {
+                const unsigned k = min(gridDim.x / units, N / units);
                 if (20 * units * k >= 17 * CT) CT = units * k;
             }
         }
-        long long t1 = 0;
-        t0 = 0;
-        if ((long long)blockIdx.x < CT) {
-            t0 = (long long)blockIdx.x * N / CT;
-            t1 = ((long long)blockIdx.x + 1) * N / CT;
-        }
-        ntiles = (int)(t1 - t0);
+        per = CT ? N / CT : 0;
+        more = N - per * CT;
+        const unsigned t0 = blockIdx.x < CT ? start(blockIdx.x) : 0;
+        ntiles = blockIdx.x < CT ? (int)(start(blockIdx.x + 1) - t0) : 0;
         At at = {0, 0, 0, 0, 1, 1, -1, 0, 0};
         if (ntiles > 0) {
             int l = 0, r = B - 1;
             while (l < r) {
                 const int mid = (l + r + 1) >> 1;
-                if (base[mid] <= t0) l = mid;
+                if ((unsigned)base[mid] <= t0) l = mid;
                 else r = mid - 1;
             }
             at.b = l;
             enter(at);
-            int rem = (int)(t0 - base[l]);
+            int rem = (int)t0 - base[l];
             at.j = rem % at.tiles;
             rem /= at.tiles;
             at.c = rem % at.groups;
@@ -171,10 +169,22 @@ struct Line {
         return at;
     }
 
-    // First and last CTA of the unit at x: tile t of the line is in CTA ceil((t + 1) CT / N) - 1.
+    // First tile of CTA c: floor(c N / CT), in 32 bits (c * more < CT^2).
+    __device__ __forceinline__ unsigned start(unsigned c) const { return c * per + c * more / CT; }
+
+    // CTA that has tile t: a guess in fp32 (off by one at most), put right.
+    __device__ __forceinline__ int cta_of(unsigned t) const {
+        int c = (int)(((float)t + 0.5f) * ((float)CT / (float)N));
+        c = max(0, min((int)CT - 1, c));
+        while (start(c) > t) --c;
+        while (start(c + 1) <= t) ++c;
+        return c;
+    }
+
+    // First and last CTA of the unit at x.
     __device__ __forceinline__ int2 ctas_of(const At& x) const {
-        const long long u = base[x.b] + ((long long)x.h * x.groups + x.c) * x.tiles;
-        return make_int2((int)(((u + 1) * CT + N - 1) / N - 1), (int)(((u + x.tiles) * CT + N - 1) / N - 1));
+        const unsigned u = base[x.b] + ((unsigned)x.h * x.groups + x.c) * x.tiles;
+        return make_int2(cta_of(u), cta_of(u + x.tiles - 1));
     }
 };
 

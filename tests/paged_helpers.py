@@ -134,11 +134,11 @@ def check_attention(out, q, cache, table, lens_of_row, seq_of_row, scale, what="
 
     q [rows, Hq, D]: the queries rotated in 64 bits. The kernels rotate them in fp32 (off by 2^-21 of the pair's sizes)
     and hold them in two fp16 parts (2^-22), in three e4m3 parts (each at most 2^-4 of what the one before left: 2^-12;
-    an element below 2^-10 of its row's largest keeps 2^-19 of that one, and the row's largest times sum|k| is at most
-    2^6 sum|q k| for the inputs here), or, with q_fp16, in one (2^-11). A score is then off by at most
-    eps = (2^-12 + 2^-13 + 2^-16) * sum|q k| scale (256 fp32 products summed in any order: 256 * 2^-24), with q_fp16 by
+    below 2^-10 / 256 of 448 nothing: 2^-26 of the row's largest element, which times sum|k| is at most 2^6 sum|q k|
+    for the inputs here), or, with q_fp16, in one (2^-11). A score is then off by at most
+    eps = (2^-12 + 2^-16 + 2^-20) * sum|q k| scale (256 fp32 products summed in any order: 256 * 2^-24), with q_fp16 by
     2^-11 of that sum, so a normalised weight by 2 eps of itself. A weight is rounded to fp16 (2^-11, or 2^-25 absolute
-    below its normals), to three e4m3 parts after it (2^-12, or 2^-18 absolute, of the largest weight) and comes from an
+    below its normals), to three e4m3 parts after it (2^-12, or 2^-24 of the largest weight) and comes from an
     approximate power of two (2^-21 and less); the fp32 sums over L keys are off by L * 2^-24, above and below the
     fraction line; the result is rounded to fp16 (2^-11, or 2^-25 absolute). All of it moves out by at most that
     share of sum(weight |v|); the largest weight is at most the sum of the weights."""
@@ -157,8 +157,8 @@ def check_attention(out, q, cache, table, lens_of_row, seq_of_row, scale, what="
                 o, w, s, top = P.attention(q[r, h * (hq // hkv) + g], k, v, scale)
                 got = out[r, h * (hq // hkv) + g].double()
                 vmax = v.abs().max(0).values if L else torch.zeros(D, dtype=torch.float64)
-                s *= 2.0 ** -16 + (2.0 ** -11 if q_fp16 else 2.0 ** -12 + 2.0 ** -13)
-                tol = w * (2 * s + 2.0 ** -11 + 2.0 ** -12 + 2.0 ** -19 + 2 * L * 2.0 ** -24) + L * 2.0 ** -18 * top * vmax \
+                s *= 2.0 ** -16 + (2.0 ** -11 if q_fp16 else 2.0 ** -12 + 2.0 ** -20)
+                tol = w * (2 * s + 2.0 ** -11 + 2.0 ** -12 + 2.0 ** -19 + 2 * L * 2.0 ** -24) + L * 2.0 ** -24 * top * vmax \
                     + o.abs() * 2.0 ** -11 + 2.0 ** -25
                 worst = max(worst, float(((got - o).abs() / tol).nan_to_num(1e9).max()))
     assert worst <= 1.0, f"{what}: {worst:.3g} times the tolerance"

@@ -267,6 +267,33 @@ def test_decode_sharp_scores_and_uneven_scales(av):
     H.check_attention(out, rotated_queries(t), H.back(d), c["table"], [x + 1 for x in T], [0, 1], 1.0, "sharp")
 
 
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("gap", [8.0, 11.0, 14.0])
+def test_decode_one_key_beside_many_small(av, e4m3, gap):
+    """One key takes most of a row's attention and thousands share the rest: the small weights still count."""
+    T = 12000
+    c = H.make_cache([T], [0], 1, 128, 64, e4m3, seed=84)
+    c["new"] = [1]
+    t = new_tokens(c, 2, seed=85)
+    u = torch.zeros(128)
+    u[0] = 1.0
+    for name in "kv":  # keys orthogonal to the query but for one; values of one sign, so that a lost mass shows
+        raw = torch.zeros(c[name].shape) if name == "k" else torch.ones(c[name].shape) * 0.75
+        if e4m3:
+            c[name + "_scales"].fill_(127)
+        if name == "k":
+            page, row = int(c["table"][0, 31]), 17
+            raw[page, 0, row] = u * 8.0
+        else:
+            page, row = int(c["table"][0, 31]), 17
+            raw[page, 0, row] = -1.0
+        c[name] = raw.to(c[name].dtype)
+    t["q"] = (u * 8.0).half().expand(1, 2, 128).contiguous()
+    d, out, q_rot, err = run_decode(av, c, t, append=False, scale=gap / 64.0)
+    assert err == 0
+    H.check_attention(out, t["q"].double(), c, c["table"], [T], [0], gap / 64.0, "sink")
+
+
 def test_decode_bad_page_and_capacity(av):
     T = [50, 40, 30]
     for wrong in (-1, 10 ** 9):
