@@ -39,6 +39,7 @@ except ImportError as exc:  # pragma: no cover - exercised only when unbuilt
     ) from exc
 
 from .arena import KVArena, decode_attention  # noqa: E402
+from .paged import PagedKVCache, paged_append, paged_decode, paged_prefill  # noqa: E402
 from . import sharding  # noqa: E402
 
 __all__ = [
@@ -46,6 +47,10 @@ __all__ = [
     "capture_decode_step",
     "KVArena",
     "decode_attention",
+    "PagedKVCache",
+    "paged_append",
+    "paged_decode",
+    "paged_prefill",
     "sharding",
     "dropin_path",
     "library_path",

@@ -24,6 +24,9 @@ Projections (default) are this library's fused batch-1 GEMVs
 in the gate/up epilogue, the residual adds in the O and down epilogues, five
 launches per layer. `projections="cublas"` runs them as torch/cuBLAS products with
 the separate RMSNorm / SwiGLU kernels instead. All fp16, as the reference's model.
+
+The cache is a KVArena by default; kv_cache="paged" or "paged_e4m3" keeps it in pages (paged.py), fp16 or
+e4m3 codes, with the same step in the same graph.
 """
 from __future__ import annotations
 
@@ -34,6 +37,7 @@ import torch
 
 from . import attn_varlen, capture_decode_step
 from .arena import KVArena, decode_attention
+from .paged import PagedKVCache, paged_decode, paged_prefill
 
 
 @dataclass(frozen=True)
@@ -99,17 +103,28 @@ class LlamaWeights:
 
 
 class GreedyDecoder:
-    """Batch-1 greedy decoding with a persistent KV arena and one CUDA graph per token step."""
+    """Batch-1 greedy decoding with a persistent KV cache (an arena, or pages of fp16 or e4m3) and one CUDA
+    graph per token step."""
 
-    def __init__(self, weights: LlamaWeights, capacity: int, max_new_tokens: int = 1024, projections: str = "fused"):
+    def __init__(self, weights: LlamaWeights, capacity: int, max_new_tokens: int = 1024, projections: str = "fused",
+                 kv_cache: str = "arena", page_size: int = 64):
         if projections not in ("fused", "cublas"):
             raise ValueError("projections must be 'fused' or 'cublas'")
+        if kv_cache not in ("arena", "paged", "paged_e4m3"):
+            raise ValueError("kv_cache must be 'arena', 'paged' or 'paged_e4m3'")
         self.projections = projections
         self.w = weights
         s = self.s = weights.shape
         dev = weights.embed.device
         self.device = dev
-        self.arena = KVArena(s.layers, 1, s.kv_heads, s.head_dim, capacity=capacity, q_heads=s.heads, device=dev)
+        if kv_cache == "arena":
+            self.arena = KVArena(s.layers, 1, s.kv_heads, s.head_dim, capacity=capacity, q_heads=s.heads, device=dev)
+        else:
+            pages = -(-capacity // page_size)
+            self.arena = PagedKVCache(s.layers, 1, s.kv_heads, s.head_dim, num_pages=pages, page_size=page_size,
+                                      q_heads=s.heads, device=dev, max_tokens=capacity, max_seqlen=capacity,
+                                      dtype=torch.float16 if kv_cache == "paged" else torch.float8_e4m3fn)
+            self.arena.reserve(0, capacity)
         H, I = s.hidden, s.intermediate
         f16 = dict(dtype=torch.float16, device=dev)
         self.x = torch.zeros(H, **f16)
@@ -128,6 +143,16 @@ class GreedyDecoder:
         self._prefill_ws = None
 
     # ------------------------------------------------------------------ one token step
+    def _attend(self, l: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
+        """The attention of layer l (RoPE, append, keys 0 .. T) into self.ctx; the last layer moves T."""
+        s = self.s
+        out = self.ctx.view(1, s.heads, s.head_dim)
+        if isinstance(self.arena, PagedKVCache):
+            paged_decode(self.arena, l, q, out, k_new=k, v_new=v, advance=(l == s.layers - 1), rope_theta=s.rope_theta)
+        else:
+            decode_attention(self.arena, l, q, out, k_new=k, v_new=v, advance=(l == s.layers - 1),
+                             rope_theta=s.rope_theta, prefetch_kv=True)
+
     def _layer(self, l: int):
         if self.projections == "fused":
             return self._layer_fused(l)
@@ -138,8 +163,7 @@ class GreedyDecoder:
         q = self.qkv[: Hq * D].view(1, Hq, D)
         k = self.qkv[Hq * D: (Hq + Hkv) * D].view(1, Hkv, D)
         v = self.qkv[(Hq + Hkv) * D:].view(1, Hkv, D)
-        decode_attention(self.arena, l, q, self.ctx.view(1, Hq, D), k_new=k, v_new=v,
-                         advance=(l == s.layers - 1), rope_theta=s.rope_theta, prefetch_kv=True)
+        self._attend(l, q, k, v)
         torch.mv(w.w_o[l], self.ctx, out=self.tmp)
         self.x.add_(self.tmp)
         capture_decode_step.rmsnorm(self.x, w.rms_post[l], self.h, s.eps)
@@ -159,8 +183,7 @@ class GreedyDecoder:
         q = self.qkv[: Hq * D].view(1, Hq, D)
         k = self.qkv[Hq * D: (Hq + Hkv) * D].view(1, Hkv, D)
         v = self.qkv[(Hq + Hkv) * D:].view(1, Hkv, D)
-        decode_attention(self.arena, l, q, self.ctx.view(1, Hq, D), k_new=k, v_new=v,
-                         advance=(l == s.layers - 1), rope_theta=s.rope_theta, prefetch_kv=True)
+        self._attend(l, q, k, v)
         gemv(w.w_o[l], self.ctx, self.x, "residual")
         gemv(w.w_gu[l], self.x, self.act, "swiglu", w.rms_post[l], s.eps)
         gemv(w.w_down[l], self.act, self.x, "residual")
@@ -219,10 +242,11 @@ class GreedyDecoder:
         s, w = self.s, self.w
         n = int(prompt.numel())
         Hq, Hkv, D, H, I = s.heads, s.kv_heads, s.head_dim, s.hidden, s.intermediate
-        if self._prefill_ws is None or self._prefill_ws[1] < n:
+        paged = isinstance(self.arena, PagedKVCache)
+        if not paged and (self._prefill_ws is None or self._prefill_ws[1] < n):
             ws = attn_varlen.make_prefill_workspace(1, Hq, Hkv, D, n, n, self.arena.capacity, D, self.device)
             self._prefill_ws = (ws, n)
-        ws = self._prefill_ws[0]
+        ws = None if paged else self._prefill_ws[0]
         cu = torch.tensor([0, n], dtype=torch.int32, device=self.device)
         x = w.embed.index_select(0, prompt)
         h = torch.empty_like(x)
@@ -234,10 +258,14 @@ class GreedyDecoder:
             k = qkv[:, Hq * D: (Hq + Hkv) * D].reshape(n, Hkv, D)
             v = qkv[:, (Hq + Hkv) * D:].reshape(n, Hkv, D)
             ctx = torch.empty(n, Hq, D, dtype=torch.float16, device=self.device)
-            kl, vl = self.arena.layer(l)
-            attn_varlen.prefill_varlen(q.contiguous(), k.contiguous(), v.contiguous(), kl, vl, ctx, cu, n,
-                                       seq_lens=self.arena.seq_lens, advance=(l == s.layers - 1),
-                                       rope_theta=s.rope_theta, workspace=ws)
+            if paged:
+                paged_prefill(self.arena, l, q.contiguous(), k.contiguous(), v.contiguous(), ctx, cu, n,
+                              advance=(l == s.layers - 1), rope_theta=s.rope_theta)
+            else:
+                kl, vl = self.arena.layer(l)
+                attn_varlen.prefill_varlen(q.contiguous(), k.contiguous(), v.contiguous(), kl, vl, ctx, cu, n,
+                                           seq_lens=self.arena.seq_lens, advance=(l == s.layers - 1),
+                                           rope_theta=s.rope_theta, workspace=ws)
             x = x + ctx.reshape(n, Hq * D) @ w.w_o[l].t()
             for i in range(n):
                 capture_decode_step.rmsnorm(x[i], w.rms_post[l], h[i], s.eps)
