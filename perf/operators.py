@@ -152,7 +152,7 @@ def prepare(case, seed):
         s[name + "_pages"], s[name + "_scales"] = pool, None if scales is None else scales.view(torch.float8_e8m0fnu)
     if own:
         from fully_custom_cuda_inference_lamma2_b200 import attn_varlen
-        s["workspace"] = attn_varlen.make_paged_workspace(B, hq, hkv, d, tokens, max(new), sum(cached) + tokens)
+        s["workspace"] = attn_varlen.make_paged_workspace(B, hq, hkv, d, tokens, case["new_hi"], sum(cached) + tokens)
     return s
 
 
