@@ -137,12 +137,19 @@ __device__ __forceinline__ uint4 expanded(uint2 codes, __half2 scale, bool clamp
 
 // cos and sin of pos * freq. The top 32 bits of the wrapped product are the angle in units of
 // 2^-32 turns; the nearest quarter turn is taken off as an integer, so what is rounded to fp32 is at
-// most an eighth of a turn (angle off by 2^-25 at most), and put back as a swap and signs.
+// most an eighth of a turn, what that rounding leaves off is put on to first order, and the quarters go back as
+// a swap and signs.
 __device__ __forceinline__ float2 rope_cs(uint64_t turn, int pos) {
     const uint32_t a = (uint32_t)(((uint64_t)(uint32_t)pos * turn) >> 32);
     const uint32_t quarter = (a + 0x20000000u) >> 30;
+    const int32_t rest = (int32_t)(a - (quarter << 30));
+    const float x32 = (float)rest;
     float s, c;
-    sincospif((float)(int32_t)(a - (quarter << 30)) * 4.656612873077393e-10f, &s, &c);
+    sincospif(x32 * 4.656612873077393e-10f, &s, &c);
+    const float off = (float)(rest - (int32_t)x32) * 1.4629180792671596e-9f;  // pi * 2^-31 each
+    const float s0 = s;
+    s = fmaf(c, off, s);
+    c = fmaf(-s0, off, c);
     const bool odd = quarter & 1;
     const float x = odd ? s : c, y = odd ? c : s;
     // quarter 0: (c, s), 1: (-s, c), 2: (-c, -s), 3: (s, -c)
@@ -182,8 +189,8 @@ constexpr int kMaxCols = 16;  // query rows of one attention unit
 struct WsLayout {
     size_t part_lse, part_o, q_rot, cu_kv, items, expanded, total;
 };
-// Work items of a prefill: 256 new tokens of one query head each.
-inline int64_t max_items(int B, int Hq, int max_q) { return (int64_t)B * ((max_q + 255) / 256) * Hq; }
+// Work items of a prefill, at most: 256 new tokens of one sequence and query head each.
+inline int64_t max_items(int B, int Hq, int total_q) { return ((int64_t)total_q / 256 + B) * Hq; }
 // Query rows of one kv head up to which a chunk takes the split-KV kernels.
 constexpr int kSplitRows = 64;
 inline bool long_chunk(int Hq, int Hkv, int max_q) { return (int64_t)max_q * (Hq / Hkv) > kSplitRows; }

@@ -24,8 +24,10 @@ constexpr int kPlanThreads = 256, kExpandThreads = 256;
 // One CTA: rows [cu_kv[b], cu_kv[b + 1]) of the expanded arrays for every sequence with new tokens, and the work list.
 // A sequence for which no rows are left gets none, is reported and not served.
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_constant__ Params p,
-                                                               const __grid_constant__ pf::Params a, int32_t* cu_kv) {
+                                                               const __grid_constant__ pf::Params a, int32_t* cu_kv,
+                                                               int64_t max_items) {
     extern __shared__ int plan_sm[];
+    __shared__ int64_t need;
     griddep_launch_dependents();
     griddep_wait();
     for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
@@ -36,14 +38,30 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
     __syncthreads();
     if (threadIdx.x == 0) {
         int at = 0;
+        int64_t items = 0;
         cu_kv[0] = 0;
         for (int b = 0; b < p.B; ++b) {
-            if (plan_sm[b] > a.capacity - at) set_error(p, FCCI_DEV_ERR_CAPACITY);
-            else at += plan_sm[b];
+            if (plan_sm[b] > a.capacity - at) {
+                set_error(p, FCCI_DEV_ERR_CAPACITY);
+            } else {
+                at += plan_sm[b];
+                if (plan_sm[b] > 0) items += (int64_t)((p.cu_q[b + 1] - p.cu_q[b] + 255) / 256) * p.Hq;
+            }
             cu_kv[b + 1] = at;
         }
+        need = items;
     }
     __syncthreads();
+    if (need > max_items) {
+        // only offsets that run backwards, so that sequences share rows, can ask for so many: nothing is served
+        if (threadIdx.x == 0) {
+            set_error(p, FCCI_DEV_ERR_CAPACITY);
+            *a.n_items = 0;
+            *a.item_cnt = 0u;
+            *a.exit_cnt = 0u;
+        }
+        return;
+    }
     pf::build_work_list(a, plan_sm);
 }
 
@@ -140,6 +158,7 @@ int launch_prefill(const Params& base, const Freqs& f, bool e4m3, uint8_t* ws, c
     p.exp_sh = (int64_t)max_kv * p.D;
     p.exp_v = p.exp_k + p.Hkv * p.exp_sh;
     p.advance = 0;
+    const int64_t items = max_items(p.B, p.Hq, p.total_q);
 
     pf::Params a;
     memset(&a, 0, sizeof(a));
@@ -157,11 +176,11 @@ int launch_prefill(const Params& base, const Freqs& f, bool e4m3, uint8_t* ws, c
     a.items = reinterpret_cast<int4*>(ws + L.items);
     a.q_rot = p.q_rot;
 
-    int rc = launch_pdl(paged_plan_kernel, dim3(1), dim3(kPlanThreads), plan_smem, st, p, a, cu_kv);
+    int rc = launch_pdl(paged_plan_kernel, dim3(1), dim3(kPlanThreads), plan_smem, st, p, a, cu_kv, items);
     if (!rc) rc = launch_append(p, f, e4m3, st);
     if (!rc) rc = launch_pdl(e4m3 ? paged_expand_kernel<true> : paged_expand_kernel<false>, dim3(8 * sms), dim3(kExpandThreads),
                              (size_t)(p.B + 1) * sizeof(int), st, p);
-    if (!rc) rc = pf::launch_attend(a, max_items(p.B, p.Hq, p.max_q), st);
+    if (!rc) rc = pf::launch_attend(a, items, st);
     return rc;
 }
 

@@ -22,7 +22,7 @@ WsLayout ws_layout(int B, int Hq, int Hkv, int D, int total_q, int max_q, int ma
     if (max_kv != 0 && long_chunk(Hq, Hkv, max_q)) {
         w.cu_kv = w.q_rot + up((size_t)total_q * Hq * D * 2);
         w.items = w.cu_kv + up((size_t)(B + 1) * 4);
-        w.expanded = w.items + up((size_t)max_items(B, Hq, max_q) * 16);
+        w.expanded = w.items + up((size_t)max_items(B, Hq, total_q) * 16);
         w.total = w.expanded + (max_kv > 0 ? up((size_t)max_kv * Hkv * D * 4) : 0);
     } else {
         w.cu_kv = w.items = w.expanded = w.total;
@@ -92,7 +92,7 @@ static int fill(const fcci_paged_desc* d, Op op, Params& p, Freqs& f, WsLayout& 
     if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
     const int sms = device_sm_count(dev);
     if (sms <= 0) return bad(FCCI_ECUDA, "no device");
-    if (op == Op::kPrefill && max_items(d->B, d->Hq, d->max_seqlen_q) > 0x7fffffff)
+    if (op == Op::kPrefill && max_items(d->B, d->Hq, d->total_q) > 0x7fffffff)
         return bad(FCCI_EINVAL, "prefill: too many work items");
     L = ws_layout(d->B, d->Hq, d->Hkv, d->D, d->total_q, d->max_seqlen_q, op == Op::kPrefill ? d->max_kv_tokens : 0,
                   sms * kMaxCtasPerSm);
