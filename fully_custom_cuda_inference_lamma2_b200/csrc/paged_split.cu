@@ -47,7 +47,7 @@ struct Cfg {
     static_assert(!QREG || 2 * COLS * QP * 2 <= RED, "queries in the joining buffer");
     static size_t smem(int stages, int B, int rope_rows, int rot) {
         return 1024 + (size_t)stages * 2 * TILE + RED + QB + (size_t)rope_rows * (rot / 2) * 8 + 2 * kComputeWarps * COLS * 4 +
-               kMaxStages * (2 * 8 * 4 + 16) + 64 + (size_t)(3 * B + 2) * 4;
+               kMaxStages * (2 * 8 * 4 + 16) + 64 + (4 * (size_t)B + 2) * 4;
     }
 };
 
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
     int* misc = reinterpret_cast<int*>(scale_sm + kMaxStages * 16);
     volatile int* abort_flag = misc;
     Line<KEYS, COLS> line(sp, misc + 16);
-    float2* cs = reinterpret_cast<float2*>(misc + 16 + 3 * B + 1 + ((B + 1) & 1));
+    float2* cs = reinterpret_cast<float2*>(misc + 16 + 4 * B + 2);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {

@@ -527,7 +527,7 @@ static int launch_tc(TileParams& tp, const Freqs& f, int sms, int dev, cudaStrea
 }
 
 int launch_split_tc(TileParams& tp, const Freqs& f, int sms, int dev, cudaStream_t st) {
-    return (int64_t)tp.p.max_q * tp.p.G <= 8 ? launch_tc<1>(tp, f, sms, dev, st) : launch_tc<2>(tp, f, sms, dev, st);
+    return tp.p.cu_q || tp.p.G <= 8 ? launch_tc<1>(tp, f, sms, dev, st) : launch_tc<2>(tp, f, sms, dev, st);
 }
 
 }  // namespace pg

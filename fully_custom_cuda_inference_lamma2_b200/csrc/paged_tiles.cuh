@@ -5,7 +5,9 @@
 // A unit is (sequence b, kv head h, column group c): up to COLS query rows of the group, rows being
 // (token, query head) pairs, so a cached key is read once for all of them. A unit's keys are cut into tiles
 // of KEYS rows; all tiles of all units form one line, of which every CTA of a persistent grid takes an
-// equal stretch, whatever the lengths are. A unit that lies in one stretch is finished there; of a cut
+// equal stretch, whatever the lengths are. On the line a unit begins with kHead places that hold no tile: what
+// its queries and its end cost (17 sequences of 1 to 5000 keys x 8 kv heads, fp16: 57 us with none, 44 us with
+// 2; a CTA with eight units of one tile held up all). A unit that lies in one stretch is finished there; of a cut
 // one, every CTA leaves its part (o, log-sum-exp) in the workspace and the last to arrive joins them. No
 // CTA waits for another.
 #pragma once
@@ -21,6 +23,7 @@ constexpr int kMaxStages = 6;
 constexpr uint64_t kWaitLimitNs = 4000000000ull;  // 4 s: far beyond any healthy wait
 constexpr uint64_t kDrainLimitNs = 500000000ull;
 constexpr int kBar = 1;
+constexpr int kHead = 2;  // places of a unit's head on the line
 
 struct TileParams {
     Params p;
@@ -68,13 +71,15 @@ struct At {
 template <int KEYS, int COLS>
 struct Line {
     const TileParams& tp;
-    int *base, *T, *n;  // shared: [B + 1] tiles before a sequence; cached rows (-1: not served), new tokens
-    unsigned N, CT;     // tiles in all, CTAs that take some
+    // shared: [B + 1] places and units before a sequence; its cached rows (-1: not served) and new tokens
+    int *base, *units, *T, *n;
+    unsigned N, CT;     // places in all, CTAs that take some
     unsigned per, more;  // N / CT and N % CT
     int ntiles;         // of this CTA
 
-    static size_t ints(int B) { return 3 * (size_t)B + 1; }
-    __device__ Line(const TileParams& tp_, int* sm) : tp(tp_), base(sm), T(sm + tp_.p.B + 1), n(T + tp_.p.B) {}
+    static size_t ints(int B) { return 4 * (size_t)B + 2; }
+    __device__ Line(const TileParams& tp_, int* sm)
+        : tp(tp_), base(sm), units(sm + tp_.p.B + 1), T(units + tp_.p.B + 1), n(T + tp_.p.B) {}
 
     __device__ __forceinline__ int keys(int t, int m) const { return t + (tp.fused || tp.p.cu_q ? m : 0); }
     __device__ __forceinline__ int groups(int m) const { return (m * tp.p.G + COLS - 1) / COLS; }
@@ -99,13 +104,13 @@ struct Line {
         if (x.b < tp.p.B) enter(x);
     }
 
-    // Lengths, prefix of the tile counts, and this CTA's stretch. All threads; scratch: 16 shared ints.
+    // Lengths, prefixes of places and units, and this CTA's stretch. All threads; scratch: 32 shared ints.
     template <int THREADS>
     __device__ At build(int* scratch) {
         const Params& p = tp.p;
         const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = p.B;
         const int chunk = (B + THREADS - 1) / THREADS, lo = tid * chunk, hi = min(B, lo + chunk);
-        int local = 0, first = -1;
+        int local = 0, local_u = 0, first = -1;
         bool uniform = true;
         for (int b = lo; b < hi; ++b) {
             const Seq s = seq_of(p, b);
@@ -114,25 +119,30 @@ struct Line {
             const int m = s.ok ? s.n : (p.cu_q ? 0 : 1);
             T[b] = s.ok ? s.T : -1;
             n[b] = m;
-            const int cnt = (s.ok ? tiles(s.T, m) : 1) * p.Hkv * groups(m);
+            const int u = p.Hkv * groups(m), cnt = ((s.ok ? tiles(s.T, m) : 1) + kHead) * u;
             base[b + 1] = cnt;
+            units[b + 1] = u;
             local += cnt;
+            local_u += u;
             if (first < 0) first = cnt;
             if (cnt != first) uniform = false;
         }
-        int incl = local;
+        int incl = local, incl_u = local_u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
+            const int v = __shfl_up_sync(0xffffffffu, incl, o), u = __shfl_up_sync(0xffffffffu, incl_u, o);
+            if (lane >= o) incl += v, incl_u += u;
         }
-        if (lane == 31) scratch[warp] = incl;
-        if (tid == 0) base[0] = 0, scratch[8] = first;
+        if (lane == 31) scratch[warp] = incl, scratch[16 + warp] = incl_u;
+        if (tid == 0) base[0] = 0, units[0] = 0, scratch[8] = first;
         __syncthreads();
         if (first >= 0 && first != scratch[8]) uniform = false;
-        int run = incl - local;
-        for (int w = 0; w < warp; ++w) run += scratch[w];
-        for (int b = lo; b < hi; ++b) base[b + 1] = run += base[b + 1];
+        int run = incl - local, run_u = incl_u - local_u;
+        for (int w = 0; w < warp; ++w) run += scratch[w], run_u += scratch[16 + w];
+        for (int b = lo; b < hi; ++b) {
+            base[b + 1] = run += base[b + 1];
+            units[b + 1] = run_u += units[b + 1];
+        }
         uniform = __syncthreads_and(uniform) != 0;
 
         N = (unsigned)base[B];
@@ -140,39 +150,47 @@ struct Line {
         if (uniform && N > 0) {
             // equal units: a number of CTAs that is a multiple of the units keeps every cut at the same
             // places of each, unless that leaves more than 15 % of the grid idle
-            const unsigned units = (unsigned)B * p.Hkv * groups(n[0]);  // at most N
-            if (units > 0 && units <= gridDim.x) {
-                const unsigned k = min(gridDim.x / units, N / units);
-                if (20 * units * k >= 17 * CT) CT = units * k;
+            const unsigned all = (unsigned)units[B];
+            if (all <= gridDim.x) {
+                const unsigned k = min(gridDim.x / all, N / all);
+                if (20 * all * k >= 17 * CT) CT = all * k;
             }
         }
         per = CT ? N / CT : 0;
         more = N - per * CT;
-        const unsigned t0 = blockIdx.x < CT ? start(blockIdx.x) : 0;
-        ntiles = blockIdx.x < CT ? (int)(start(blockIdx.x + 1) - t0) : 0;
         At at = {0, 0, 0, 0, 1, 1, -1, 0, 0};
-        if (ntiles > 0) {
-            int l = 0, r = B - 1;
-            while (l < r) {
-                const int mid = (l + r + 1) >> 1;
-                if ((unsigned)base[mid] <= t0) l = mid;
-                else r = mid - 1;
-            }
-            at.b = l;
-            enter(at);
-            int rem = (int)t0 - base[l];
-            at.j = rem % at.tiles;
-            rem /= at.tiles;
-            at.c = rem % at.groups;
-            at.h = rem / at.groups;
+        ntiles = 0;
+        if (blockIdx.x < CT) {
+            At end = at;
+            const int first_tile = place(start(blockIdx.x), at);
+            ntiles = place(start(blockIdx.x + 1), end) - first_tile;
         }
         return at;
     }
 
-    // First tile of CTA c: floor(c N / CT), in 32 bits (c * more < CT^2).
+    // The first tile at or behind place t: where it is, and the tiles before it on the line.
+    __device__ int place(unsigned t, At& x) const {
+        const int B = tp.p.B;
+        if (t >= N) return base[B] - kHead * units[B];
+        int l = 0, r = B - 1;
+        while (l < r) {
+            const int mid = (l + r + 1) >> 1;
+            if ((unsigned)base[mid] <= t) l = mid;
+            else r = mid - 1;
+        }
+        x.b = l;
+        enter(x);
+        const int rem = (int)t - base[l], unit = rem / (x.tiles + kHead);
+        x.j = max(0, rem - unit * (x.tiles + kHead) - kHead);
+        x.h = unit / x.groups;
+        x.c = unit - x.h * x.groups;
+        return base[l] - kHead * units[l] + unit * x.tiles + x.j;
+    }
+
+    // First place of CTA c: floor(c N / CT), in 32 bits (c * more < CT^2).
     __device__ __forceinline__ unsigned start(unsigned c) const { return c * per + c * more / CT; }
 
-    // CTA that has tile t: a guess in fp32 (off by one at most), put right.
+    // CTA that has place t: a guess in fp32 (off by one at most), put right.
     __device__ __forceinline__ int cta_of(unsigned t) const {
         int c = (int)(((float)t + 0.5f) * ((float)CT / (float)N));
         c = max(0, min((int)CT - 1, c));
@@ -183,7 +201,7 @@ struct Line {
 
     // First and last CTA of the unit at x.
     __device__ __forceinline__ int2 ctas_of(const At& x) const {
-        const unsigned u = base[x.b] + ((unsigned)x.h * x.groups + x.c) * x.tiles;
+        const unsigned u = base[x.b] + ((unsigned)x.h * x.groups + x.c) * (x.tiles + kHead) + kHead;  // of its first tile
         return make_int2(cta_of(u), cta_of(u + x.tiles - 1));
     }
 };
