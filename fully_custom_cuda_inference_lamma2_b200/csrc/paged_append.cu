@@ -161,11 +161,12 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int b = blockIdx.y;
     const Seq s = seq_of(p, b);
-    const int pj = (s.T >> p.page_log2) + blockIdx.x;
-    const int p0 = pj << p.page_log2;  // first position of the page
+    const int64_t first = ((int64_t)(s.T >> p.page_log2) + blockIdx.x) << p.page_log2;
+    const bool here = s.ok && s.n > 0 && first < (int64_t)s.T + s.n;
+    const int p0 = here ? (int)first : 0;  // first position of the page
     if (!s.ok) {
         if (blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
-    } else if (s.n > 0 && p0 < s.T + s.n) {
+    } else if (here) {
         const int half = p.rot >> 1;
         for (int i = tid; i < p.page * half; i += kRowsThreads) {
             const int r = i / half, k = i - r * half;

@@ -70,8 +70,8 @@ static int fill(const fcci_paged_desc* d, Op op, Params& p, Freqs& f, WsLayout& 
     if (!d->cu_seqlens_q && d->total_q != d->B) return bad(FCCI_EINVAL, "total_q must be B without cu_seqlens_q");
     if (d->rotary_dim < 0 || d->rotary_dim > d->D || d->rotary_dim % 16)
         return bad(FCCI_EUNSUPPORTED, "rotary_dim must be a multiple of 16 within head_dim");
-    if (d->rotary_dim > 0 && !(d->rope_theta > 0.f && d->rope_theta < INFINITY))
-        return bad(FCCI_EINVAL, "rope_theta must be positive");
+    if (d->rotary_dim > 0 && !(d->rope_theta >= 1e-6f && d->rope_theta < INFINITY))
+        return bad(FCCI_EINVAL, "rope_theta must be positive (1e-6 at least)");
     if (op != Op::kAppend && !(d->scale > 0.f && d->scale < INFINITY)) return bad(FCCI_EINVAL, "scale must be positive");
     if (d->advance && !d->k_new) return bad(FCCI_EINVAL, "advance needs k_new");
     const int64_t elt = e4m3 ? 1 : 2;
@@ -132,9 +132,10 @@ static int fill(const fcci_paged_desc* d, Op op, Params& p, Freqs& f, WsLayout& 
         static thread_local Freqs kept;
         if (theta != d->rope_theta || rot != p.rot) {
             const int half = p.rot / 2;
-            for (int i = 0; i < half; ++i)
-                kept.turn[i] = (uint64_t)(powl((long double)d->rope_theta, -(long double)i / half) *
-                                              0.15915494309189533576888L * 18446744073709551616.0L + 0.5L);
+            for (int i = 0; i < half; ++i) {
+                const long double turns = powl((long double)d->rope_theta, -(long double)i / half) * 0.15915494309189533576888L;
+                kept.turn[i] = (uint64_t)ldexpl(turns - floorl(turns), 64);  // whole turns per position change nothing
+            }
             theta = d->rope_theta, rot = p.rot;
         }
         f = kept;

@@ -6,8 +6,8 @@
 // (token, query head) pairs, so a cached key is read once for all of them. A unit's keys are cut into tiles
 // of KEYS rows; all tiles of all units form one line, of which every CTA of a persistent grid takes an
 // equal stretch, whatever the lengths are. On the line a unit begins with kHead places that hold no tile: what
-// its queries and its end cost (17 sequences of 1 to 5000 keys x 8 kv heads, fp16: 57 us with none, 44 us with
-// 2; a CTA with eight units of one tile held up all). A unit that lies in one stretch is finished there; of a cut
+// its queries and its end cost (17 sequences of 1 to 5000 keys x 8 kv heads, fp16: 56 us with none, 41 us with
+// 2, 40 us with 4; a CTA with eight units of one tile held up all). A unit that lies in one stretch is finished there; of a cut
 // one, every CTA leaves its part (o, log-sum-exp) in the workspace and the last to arrive joins them. No
 // CTA waits for another.
 #pragma once
@@ -23,7 +23,7 @@ constexpr int kMaxStages = 6;
 constexpr uint64_t kWaitLimitNs = 4000000000ull;  // 4 s: far beyond any healthy wait
 constexpr uint64_t kDrainLimitNs = 500000000ull;
 constexpr int kBar = 1;
-constexpr int kHead = 2;  // places of a unit's head on the line
+constexpr int kHead = 4;  // places of a unit's head on the line
 
 struct TileParams {
     Params p;
@@ -111,7 +111,9 @@ struct Line {
         const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = p.B;
         const int chunk = (B + THREADS - 1) / THREADS, lo = tid * chunk, hi = min(B, lo + chunk);
         int local = 0, local_u = 0, first = -1;
-        bool uniform = true;
+        bool uniform = true, too_many = false;
+        constexpr long long kMostPlaces = 1 << 23;  // of a thread: the line stays below 2^31 (8 M tiles are 10^9 keys)
+        static_assert(THREADS <= 256, "places in 31 bits");
         for (int b = lo; b < hi; ++b) {
             const Seq s = seq_of(p, b);
             if (!s.ok && blockIdx.x == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
@@ -119,10 +121,13 @@ struct Line {
             const int m = s.ok ? s.n : (p.cu_q ? 0 : 1);
             T[b] = s.ok ? s.T : -1;
             n[b] = m;
-            const int u = p.Hkv * groups(m), cnt = ((s.ok ? tiles(s.T, m) : 1) + kHead) * u;
+            const int u = p.Hkv * groups(m);
+            const long long places = (long long)((s.ok ? tiles(s.T, m) : 1) + kHead) * u;
+            const int cnt = (int)min(places, kMostPlaces);
+            too_many = too_many || local + places > kMostPlaces;
             base[b + 1] = cnt;
             units[b + 1] = u;
-            local += cnt;
+            local = (int)min(local + places, kMostPlaces);
             local_u += u;
             if (first < 0) first = cnt;
             if (cnt != first) uniform = false;
@@ -143,9 +148,12 @@ struct Line {
             base[b + 1] = run += base[b + 1];
             units[b + 1] = run_u += units[b + 1];
         }
-        uniform = __syncthreads_and(uniform) != 0;
-
+        uniform = __syncthreads_and(uniform && !too_many) != 0;
         N = (unsigned)base[B];
+        if (!uniform && __syncthreads_or(too_many)) {
+            if (blockIdx.x == 0 && tid == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
+            N = 0;  // nothing is served
+        }
         CT = min(N, gridDim.x);
         if (uniform && N > 0) {
             // equal units: a number of CTAs that is a multiple of the units keeps every cut at the same

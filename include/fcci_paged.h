@@ -68,9 +68,11 @@ extern "C" {
  *                that gets rows must belong to one sequence alone.
  *   attention    out = softmax_t(q_rot . k_t * scale) v_t, fp32 accumulation; a token that
  *                sees no key gets 0. What pages hold behind a sequence's rows (NaN
- *                among it) has no effect.
+ *                among it) has no effect. Among the new tokens of one prefill, a value that is
+ *                NaN or infinite may reach tokens before its own (its weight there is 0, and
+ *                0 * NaN is NaN); keys that are not finite do not.
  *   advance      when non-zero, seq_lens[b] += n_b after the step
- * head_dim 64, 128 or 256 (prefill: 128); page_size 16, 32, 64 or 128 with
+ * rope_theta 1e-6 at least. head_dim 64, 128 or 256 (prefill: 128); page_size 16, 32, 64 or 128 with
  * page_size * D <= 16384; Hq a multiple of Hkv, at most 16 query heads a kv head (8 with
  * head_dim 256).
  *

@@ -314,6 +314,38 @@ def test_decode_bad_page_and_capacity(av):
     H.check_attention(out[:1], rotated_queries(t)[:1], H.back(d), c["table"], [51], [0], 128 ** -0.5, "the one that fits")
 
 
+@pytest.mark.parametrize("e4m3,D", [(True, 128), (True, 64), (False, 128)])
+def test_decode_many_short_sequences(av, e4m3, D):
+    """More sequences than CTAs, most of a few keys and some long: units of every kind on one CTA."""
+    T = [(7 * i) % 40 for i in range(331)] + [1500, 0, 700]
+    c = H.make_cache(T, [1] * len(T), 1, D, 16, e4m3, seed=131)
+    t = new_tokens(c, 2, seed=132)
+    d, out, q_rot, err = run_decode(av, c, t, advance=True)
+    assert err == 0 and d["T"].cpu().tolist() == [x + 1 for x in T]
+    H.check_attention(out, rotated_queries(t), H.back(d), c["table"], [x + 1 for x in T], range(len(T)), D ** -0.5, "many")
+
+
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_decode_largest_queries(av, e4m3):
+    """Queries whose rotation passes fp16's range."""
+    c = H.make_cache([33, 200], [1, 1], 1, 128, 32, e4m3, seed=133)
+    t = new_tokens(c, 2, seed=134)
+    t["q"] = (torch.sign(t["q"].float()) * 65504.0).half()
+    d, out, q_rot, err = run_decode(av, c, t, scale=1e-6)
+    assert err == 0 and rotated_queries(t).abs().max() > 70000
+    H.check_attention(out, rotated_queries(t), H.back(d), c["table"], [34, 201], [0, 1], 1e-6, "largest")
+
+
+@pytest.mark.parametrize("theta", [0.3, 1.0, 5e5, 1e30])
+def test_append_odd_thetas(av, theta):
+    c = H.make_cache([1000, 3], [1, 1], 1, 64, 16, False, seed=135)
+    t = new_tokens(c, 1, seed=136)
+    d, q_rot, err = run_append(av, c, t, varlen=False, theta=theta)
+    assert err == 0
+    # the entry points take theta in fp32
+    check_whole_append(c, t, d, q_rot, 64, float(torch.tensor(theta, dtype=torch.float32)))
+
+
 def test_decode_shared_prefix_pages(av):
     """Two sequences that name the same full pages read the same rows."""
     c = H.make_cache([64, 64], [1, 1], 2, 128, 16, True, seed=101)

@@ -43,7 +43,7 @@ BAD = [
     ("max_pages", 0, EINVAL), ("max_pages", 1 << 30, EINVAL), ("page_table_stride", -4, EINVAL), ("k_new", None, EINVAL),
     ("total_q", -1, EINVAL), ("total_q", 3, EINVAL), ("max_seqlen_q", -1, EINVAL), ("rotary_dim", 8, EUNSUPPORTED),
     ("rotary_dim", 144, EUNSUPPORTED), ("rotary_dim", -16, EUNSUPPORTED), ("rope_theta", 0.0, EINVAL),
-    ("rope_theta", float("nan"), EINVAL), ("rope_theta", float("inf"), EINVAL), ("k_pages", 0x40008, EINVAL),
+    ("rope_theta", float("nan"), EINVAL), ("rope_theta", 1e-7, EINVAL), ("rope_theta", float("inf"), EINVAL), ("k_pages", 0x40008, EINVAL),
     ("v_new", 0x30002, EINVAL), ("q", 0x10004, EINVAL), ("k_stride_p", 8, EINVAL), ("v_stride_t", 64, EINVAL),
     ("k_stride_t", 0, EINVAL), ("k_stride_h", -128, EINVAL), ("q_stride_h", 132, EINVAL), ("k_scales_stride_p", -1, EINVAL),
     ("workspace", None, None), ("workspace_bytes", 1000, None),
