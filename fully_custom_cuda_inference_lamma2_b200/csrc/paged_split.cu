@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
         prefetch_tmap(&mk16);
         prefetch_tmap(&mv16);
     }
+    __syncthreads();
     griddep_launch_dependents();
     griddep_wait();
 

@@ -145,11 +145,12 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
         tc::tmem_relinquish();
     }
     const uint64_t turn = tid < p.rot / 2 ? f.turn[tid] : 0;  // a launch constant: its cold read is over before the wait is
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
     griddep_launch_dependents();
     griddep_wait();
-    tc::fence_before_sync();
-    At at = line.template build<kTcThreads>(reinterpret_cast<int*>(mx_sm));  // barriers inside
-    tc::fence_after_sync();
+    At at = line.template build<kTcThreads>(reinterpret_cast<int*>(mx_sm));
     const uint32_t tmem = *tmem_slot;
     const uint32_t tmem_o = tmem + 2 * C::STRIDE;
     const int ntiles = line.ntiles;

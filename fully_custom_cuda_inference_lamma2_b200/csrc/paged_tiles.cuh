@@ -109,12 +109,11 @@ struct Line {
     __device__ At build(int* scratch) {
         const Params& p = tp.p;
         const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = p.B;
-        const int chunk = (B + THREADS - 1) / THREADS, lo = tid * chunk, hi = min(B, lo + chunk);
-        int local = 0, local_u = 0, first = -1;
         bool uniform = true, too_many = false;
         constexpr long long kMostPlaces = 1 << 23;  // of a thread: the line stays below 2^31 (8 M tiles are 10^9 keys)
         static_assert(THREADS <= 256, "places in 31 bits");
-        for (int b = lo; b < hi; ++b) {
+        // (places, units) of sequence b; writes its T and n
+        auto count = [&](int b, long long& places) {
             const Seq s = seq_of(p, b);
             if (!s.ok && blockIdx.x == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
             // a sequence that is not served: its one row gets zeros in decode, none are touched otherwise
@@ -122,35 +121,62 @@ struct Line {
             T[b] = s.ok ? s.T : -1;
             n[b] = m;
             const int u = p.Hkv * groups(m);
-            const long long places = (long long)((s.ok ? tiles(s.T, m) : 1) + kHead) * u;
+            places = (long long)((s.ok ? tiles(s.T, m) : 1) + kHead) * u;
+            return u;
+        };
+        if (B <= 32) {
+            // every warp does the same by itself: no barrier between the lengths' arrival and the first copy
+            long long places = 0;
+            const int u = lane < B ? count(lane, places) : 0;
+            too_many = __any_sync(0xffffffffu, places > kMostPlaces);
             const int cnt = (int)min(places, kMostPlaces);
-            too_many = too_many || local + places > kMostPlaces;
-            base[b + 1] = cnt;
-            units[b + 1] = u;
-            local = (int)min(local + places, kMostPlaces);
-            local_u += u;
-            if (first < 0) first = cnt;
-            if (cnt != first) uniform = false;
-        }
-        int incl = local, incl_u = local_u;
+            int incl = cnt, incl_u = u;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, o), u = __shfl_up_sync(0xffffffffu, incl_u, o);
-            if (lane >= o) incl += v, incl_u += u;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o), w = __shfl_up_sync(0xffffffffu, incl_u, o);
+                if (lane >= o) incl += v, incl_u += w;
+            }
+            if (lane == 0) base[0] = 0, units[0] = 0;
+            if (lane < B) base[lane + 1] = incl, units[lane + 1] = incl_u;
+            const int cnt0 = __shfl_sync(0xffffffffu, cnt, 0);
+            uniform = __all_sync(0xffffffffu, lane >= B || cnt == cnt0);
+            __syncwarp();
+        } else {
+            const int chunk = (B + THREADS - 1) / THREADS, lo = tid * chunk, hi = min(B, lo + chunk);
+            int local = 0, local_u = 0, first = -1;
+            for (int b = lo; b < hi; ++b) {
+                long long places;
+                const int u = count(b, places), cnt = (int)min(places, kMostPlaces);
+                too_many = too_many || local + places > kMostPlaces;
+                base[b + 1] = cnt;
+                units[b + 1] = u;
+                local = (int)min(local + places, kMostPlaces);
+                local_u += u;
+                if (first < 0) first = cnt;
+                if (cnt != first) uniform = false;
+            }
+            int incl = local, incl_u = local_u;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o), u = __shfl_up_sync(0xffffffffu, incl_u, o);
+                if (lane >= o) incl += v, incl_u += u;
+            }
+            if (lane == 31) scratch[warp] = incl, scratch[16 + warp] = incl_u;
+            if (tid == 0) base[0] = 0, units[0] = 0, scratch[8] = first;
+            __syncthreads();
+            if (first >= 0 && first != scratch[8]) uniform = false;
+            int run = incl - local, run_u = incl_u - local_u;
+            for (int w = 0; w < warp; ++w) run += scratch[w], run_u += scratch[16 + w];
+            for (int b = lo; b < hi; ++b) {
+                base[b + 1] = run += base[b + 1];
+                units[b + 1] = run_u += units[b + 1];
+            }
+            too_many = __syncthreads_or(too_many) != 0;
+            uniform = __syncthreads_and(uniform) != 0;
         }
-        if (lane == 31) scratch[warp] = incl, scratch[16 + warp] = incl_u;
-        if (tid == 0) base[0] = 0, units[0] = 0, scratch[8] = first;
-        __syncthreads();
-        if (first >= 0 && first != scratch[8]) uniform = false;
-        int run = incl - local, run_u = incl_u - local_u;
-        for (int w = 0; w < warp; ++w) run += scratch[w], run_u += scratch[16 + w];
-        for (int b = lo; b < hi; ++b) {
-            base[b + 1] = run += base[b + 1];
-            units[b + 1] = run_u += units[b + 1];
-        }
-        uniform = __syncthreads_and(uniform && !too_many) != 0;
+
         N = (unsigned)base[B];
-        if (!uniform && __syncthreads_or(too_many)) {
+        if (too_many) {
             if (blockIdx.x == 0 && tid == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
             N = 0;  // nothing is served
         }
@@ -190,13 +216,13 @@ struct Line {
         enter(x);
         const int rem = (int)t - base[l], unit = rem / (x.tiles + kHead);
         x.j = max(0, rem - unit * (x.tiles + kHead) - kHead);
-        x.h = unit / x.groups;
+        x.h = x.groups == 1 ? unit : unit / x.groups;
         x.c = unit - x.h * x.groups;
         return base[l] - kHead * units[l] + unit * x.tiles + x.j;
     }
 
     // First place of CTA c: floor(c N / CT), in 32 bits (c * more < CT^2).
-    __device__ __forceinline__ unsigned start(unsigned c) const { return c * per + c * more / CT; }
+    __device__ __forceinline__ unsigned start(unsigned c) const { return c * per + (more ? c * more / CT : 0); }
 
     // CTA that has place t: a guess in fp32 (off by one at most), put right.
     __device__ __forceinline__ int cta_of(unsigned t) const {
