@@ -9,6 +9,9 @@
 // kernels do, would add half to the products of a kernel that the products bound (results are off by 3.5e-4 to
 // 5.4e-4 in the 2-norm, 2.1e-4 of it their own rounding).
 //
+// Measured: 2 x 2048 new tokens after 12000 to 14000, 64 / 8 heads: attention 1598 us, append 61, expansion 45 (3.6 TB/s
+// in and out); 16 prompts of 256 to 4096, 32 heads: attention 722 us, append 335.
+//
 // Launches: the plan (row ranges, work list), the append (which also writes its own rows expanded, while it has
 // them), the expansion of the rows cached before, the attention.
 #include <cuda_fp16.h>
@@ -39,6 +42,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
         const Seq s = seq_of(p, b);
         if (!s.ok) set_error(p, FCCI_DEV_ERR_CAPACITY);
         plan_sm[b] = s.ok && s.n > 0 ? s.T + s.n : 0;
+        plan_sm[p.B + b] = s.n;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -50,7 +54,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
                 set_error(p, FCCI_DEV_ERR_CAPACITY);
             } else {
                 at += plan_sm[b];
-                if (plan_sm[b] > 0) items += (int64_t)((p.cu_q[b + 1] - p.cu_q[b] + 255) / 256) * p.Hq;
+                if (plan_sm[b] > 0) items += (int64_t)((plan_sm[p.B + b] + 255) / 256) * p.Hq;
             }
             cu_kv[b + 1] = at;
         }
