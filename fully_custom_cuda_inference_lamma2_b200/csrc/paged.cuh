@@ -201,7 +201,9 @@ WsLayout ws_layout(int B, int Hq, int Hkv, int D, int total_q, int max_q, int ma
 
 int launch_append(const Params& p, const Freqs& f, bool e4m3, cudaStream_t st);
 // Split-KV attention; `fused`: the launch appends the one new row of each sequence itself.
-int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, uint8_t* ws, const WsLayout& L, cudaStream_t st);
+// early: FCCI_PAGED_PREFETCH_KV.
+int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, bool early, uint8_t* ws, const WsLayout& L,
+                 cudaStream_t st);
 int launch_prefill(const Params& p, const Freqs& f, bool e4m3, uint8_t* ws, const WsLayout& L, int max_kv, float scale_log2,
                    int advance, cudaStream_t st);
 struct TileParams;

@@ -194,7 +194,7 @@ inline void paged_decode(const at::Tensor& q, const at::Tensor& k_pages, const a
                          const at::Tensor& page_table, const at::Tensor& seq_lens, const OptTensor& k_scales,
                          const OptTensor& v_scales, const OptTensor& k_new, const OptTensor& v_new, double scale,
                          double rope_theta, int64_t rotary_dim, bool advance, const OptTensor& q_rot_out,
-                         const OptTensor& workspace) {
+                         const OptTensor& workspace, bool prefetch_kv) {
     PagedCall c;
     bind_cache(c, k_pages, v_pages, k_scales, v_scales, page_table, seq_lens);
     const at::Device dev = k_pages.device();
@@ -213,6 +213,7 @@ inline void paged_decode(const at::Tensor& q, const at::Tensor& k_pages, const a
     bind_rope(c, rope_theta, rotary_dim, given(k_new));
     c.d.advance = advance ? 1 : 0;
     bind_paged_workspace(c, workspace, dev);
+    c.d.flags = prefetch_kv ? FCCI_PAGED_PREFETCH_KV : 0u;
     check_rc(fcci_paged_decode(&c.d, current_stream()), "attn_varlen.paged_decode");
 }
 
@@ -263,7 +264,7 @@ inline void def_paged(py::module& m) {
           py::arg("seq_lens"), py::kw_only(), py::arg("k_scales") = py::none(), py::arg("v_scales") = py::none(),
           py::arg("k_new") = py::none(), py::arg("v_new") = py::none(), py::arg("scale") = -1.0,
           py::arg("rope_theta") = 10000.0, py::arg("rotary_dim") = -1, py::arg("advance") = false,
-          py::arg("q_rot_out") = py::none(), py::arg("workspace") = py::none());
+          py::arg("q_rot_out") = py::none(), py::arg("workspace") = py::none(), py::arg("prefetch_kv") = false);
     m.def("paged_prefill", &paged_prefill,
           "Prompts (or chunks) over a paged cache: RoPE(q,k_new) at T_b+i, append, causal attention over T_b+n_b keys",
           py::arg("q"), py::arg("k_new"), py::arg("v_new"), py::arg("k_pages"), py::arg("v_pages"), py::arg("out"),

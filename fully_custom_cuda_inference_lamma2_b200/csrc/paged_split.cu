@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
     }
     __syncthreads();
     griddep_launch_dependents();
-    griddep_wait();
+    if (!sp.early) griddep_wait();
 
     At at = line.template build<kThreads>(reinterpret_cast<int*>(red_ml));
     const int ntiles = line.ntiles;
@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
         fetch_tiles<TL, E4M3, COLS>(line, at, is_v, is_v ? &mv : &mk, is_v ? &mv16 : &mk16, tiles_sm, full, empty, scale_sm, abort_flag);
     } else {
         // ============================================================ computing warps
+        if (sp.early) griddep_wait();  // before the queries, the new rows and everything that is written
         const int w = warp, g = lane >> 2, t4 = lane & 3;
         const int rot = p.rot, half = rot >> 1;
         float m[NB][2], l[NB][2];
@@ -529,13 +530,15 @@ static int launch_split_t(TileParams& sp, const Freqs& f, int sms, int dev, cuda
     return launch_pdl(paged_split_kernel<D, NB, E4M3>, dim3(sms * per_sm), dim3(kThreads), smem, st, m[0], m[1], m[2], m[3], sp, f);
 }
 
-int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, uint8_t* ws, const WsLayout& L, cudaStream_t st) {
+int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, bool early, uint8_t* ws, const WsLayout& L,
+                 cudaStream_t st) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
     const int sms = device_sm_count(dev);
     TileParams sp;
     sp.p = p;
     sp.fused = fused;
+    sp.early = early;
     sp.stages = 0;
     sp.cut_cnt = reinterpret_cast<uint32_t*>(ws + 256);
     sp.part_lse = reinterpret_cast<float*>(ws + L.part_lse);

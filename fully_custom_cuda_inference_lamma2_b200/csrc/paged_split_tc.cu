@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
     __syncthreads();
     tc::fence_after_sync();
     griddep_launch_dependents();
-    griddep_wait();
+    if (!tp.early) griddep_wait();
     At at = line.template build<kTcThreads>(reinterpret_cast<int*>(mx_sm));
     const uint32_t tmem = *tmem_slot;
     const uint32_t tmem_o = tmem + 2 * C::STRIDE;
@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
         // ============================================================ softmax
         // A wait that fails leaves garbage behind, never a barrier that some warps skip: the loop runs on, its
         // waits return at once, and the error word says so.
+        if (tp.early) griddep_wait();  // before the queries, the new rows and everything that is written
         const uint32_t lane_row = (uint32_t)warp * 32;
         const int rot = p.rot, half = rot >> 1;
         const int box_log2 = min(p.page_log2, 7);

@@ -73,6 +73,7 @@ static int fill(const fcci_paged_desc* d, Op op, Params& p, Freqs& f, WsLayout& 
     if (d->rotary_dim > 0 && !(d->rope_theta >= 1e-6f && d->rope_theta < INFINITY))
         return bad(FCCI_EINVAL, "rope_theta must be positive (1e-6 at least)");
     if (op != Op::kAppend && !(d->scale > 0.f && d->scale < INFINITY)) return bad(FCCI_EINVAL, "scale must be positive");
+    if (d->flags & ~(op == Op::kDecode ? FCCI_PAGED_PREFETCH_KV : 0u)) return bad(FCCI_EINVAL, "unknown bits in flags");
     if (d->advance && !d->k_new) return bad(FCCI_EINVAL, "advance needs k_new");
     const int64_t elt = e4m3 ? 1 : 2;
     const void* ptrs[7] = {d->q, d->k_new, d->v_new, d->k_pages, d->v_pages, d->out, d->q_rot_out};
@@ -169,7 +170,7 @@ static int paged_step(const fcci_paged_desc* d, Op op, cudaStream_t stream) {
         if (rc) return rc;
     }
     p.advance = d->advance;
-    return launch_split(p, f, e4m3, op == Op::kDecode && p.append, ws, L, stream);
+    return launch_split(p, f, e4m3, op == Op::kDecode && p.append, d->flags & FCCI_PAGED_PREFETCH_KV, ws, L, stream);
 }
 
 }  // namespace pg

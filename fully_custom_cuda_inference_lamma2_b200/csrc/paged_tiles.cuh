@@ -28,6 +28,7 @@ constexpr int kHead = 4;  // places of a unit's head on the line
 struct TileParams {
     Params p;
     int32_t fused;   // the kernel appends row T itself (decode)
+    int32_t early;   // lengths, page table, scales and cached rows may be read before the programmatic-launch wait
     int32_t stages;
     float* part_lse;    // [2 * grid][kMaxCols]
     float* part_o;      // [2 * grid][kMaxCols][D]

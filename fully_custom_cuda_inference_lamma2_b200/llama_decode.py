@@ -148,7 +148,8 @@ class GreedyDecoder:
         s = self.s
         out = self.ctx.view(1, s.heads, s.head_dim)
         if isinstance(self.arena, PagedKVCache):
-            paged_decode(self.arena, l, q, out, k_new=k, v_new=v, advance=(l == s.layers - 1), rope_theta=s.rope_theta)
+            paged_decode(self.arena, l, q, out, k_new=k, v_new=v, advance=(l == s.layers - 1),
+                         rope_theta=s.rope_theta, prefetch_kv=True)
         else:
             decode_attention(self.arena, l, q, out, k_new=k, v_new=v, advance=(l == s.layers - 1),
                              rope_theta=s.rope_theta, prefetch_kv=True)

@@ -117,13 +117,18 @@ def paged_append(cache: PagedKVCache, layer: int, k_new: torch.Tensor, v_new: to
 def paged_decode(cache: PagedKVCache, layer: int, q: torch.Tensor, out: torch.Tensor, *,
                  k_new: Optional[torch.Tensor] = None, v_new: Optional[torch.Tensor] = None, advance: bool = False,
                  scale: Optional[float] = None, rope_theta: float = 10000.0, rotary_dim: int = -1,
-                 q_rot_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                 q_rot_out: Optional[torch.Tensor] = None, prefetch_kv: bool = False) -> torch.Tensor:
     """One decode step of `layer`: RoPE + append at T_b (when k_new is given) and split-KV attention over all keys of
-    each sequence, in one launch on the current stream, without allocation or host sync."""
+    each sequence, in one launch on the current stream, without allocation or host sync.
+
+    prefetch_kv: read the lengths, the page table and the cached rows before waiting for the previous kernel on the
+    stream (FCCI_PAGED_PREFETCH_KV). Only when no kernel that may still be running writes them, e.g. right after the
+    projection that produced q/k_new/v_new, or after another layer's step that does not advance."""
     k, v, ks, vs = cache.layer(layer)
     attn_varlen.paged_decode(q, k, v, out, cache.page_table, cache.seq_lens, k_scales=ks, v_scales=vs, k_new=k_new,
                              v_new=v_new, scale=-1.0 if scale is None else float(scale), rope_theta=rope_theta,
-                             rotary_dim=rotary_dim, advance=advance, q_rot_out=q_rot_out, workspace=cache.workspace)
+                             rotary_dim=rotary_dim, advance=advance, q_rot_out=q_rot_out, workspace=cache.workspace,
+                             prefetch_kv=prefetch_kv)
     return out
 
 

@@ -113,7 +113,14 @@ typedef struct fcci_paged_desc {
     int32_t max_kv_tokens; /* prefill: bound on the sum of T_b + n_b; negative: what the workspace has room for */
     void* workspace;       /* fcci_paged_workspace_bytes() bytes, zeroed once with _init */
     size_t workspace_bytes;
+    uint32_t flags; /* FCCI_PAGED_PREFETCH_KV (decode only) */
 } fcci_paged_desc;
+
+/* Decode: read seq_lens, the page table, scales and the cached rows below T_b before the programmatic-launch wait, so
+ * that they overlap the kernel before it on the stream; q, k_new and v_new are still read after it. Set it only when no
+ * kernel that can still be running when this one starts writes any of those: for example a decode step right after the
+ * projection that produced q/k/v, or after another layer's decode step that does not advance. */
+#define FCCI_PAGED_PREFETCH_KV 1u
 
 int fcci_paged_append(const fcci_paged_desc* desc, cudaStream_t stream);
 int fcci_paged_decode(const fcci_paged_desc* desc, cudaStream_t stream);

@@ -15,7 +15,7 @@ class PagedDesc(C.Structure):
         ("v_scales_stride_p", I64), ("v_scales_stride_h", I64), ("page_table", P), ("page_table_stride", I64),
         ("seq_lens", P), ("out", P), ("out_stride_t", I64), ("out_stride_h", I64), ("q_rot_out", P), ("scale", C.c_float),
         ("rope_theta", C.c_float), ("rotary_dim", I32), ("advance", I32), ("max_kv_tokens", I32), ("workspace", P),
-        ("workspace_bytes", C.c_size_t),
+        ("workspace_bytes", C.c_size_t), ("flags", C.c_uint32),
     ]
 
 

@@ -143,6 +143,50 @@ def test_calls_in_two_streams_with_their_own_workspaces(pkg):
         assert av.paged_read_error(ws) == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float16])
+def test_early_reads_change_nothing(pkg, dtype):
+    """A chain of layers' steps with and without prefetch_kv, over a page end, eager and replayed: the same bits."""
+    L, B, hq, hkv, D, steps = 6, 5, 8, 2, 128, 20
+    T = [0, 13, 500, 1300, 31]
+    got = []
+    for early, use_graph in ((False, False), (True, False), (True, True)):
+        cache = pkg.PagedKVCache(L, B, hkv, D, num_pages=140, page_size=16, q_heads=hq, dtype=dtype)
+        for t in (cache.k, cache.v):
+            t.view(torch.uint8 if dtype != torch.float16 else torch.int16).fill_(0x3A if dtype != torch.float16 else 0x3800)
+        if cache.k_scales is not None:
+            cache.k_scales.view(torch.uint8).fill_(124)
+            cache.v_scales.view(torch.uint8).fill_(124)
+        for b in range(B):
+            cache.reserve(b, T[b] + steps + 2)
+        cache.seq_lens.copy_(torch.tensor(T, dtype=torch.int32))
+        q, k, v = rows((L, B, hq, D), 301), rows((L, B, hkv, D), 302), rows((L, B, hkv, D), 303)
+        out = torch.zeros(L, B, hq, D).half().cuda()
+
+        def step():
+            q.mul_(1.01)  # an ordinary launch between the steps
+            for l in range(L):
+                pkg.paged_decode(cache, l, q[l], out[l], k_new=k[l], v_new=v[l], advance=(l == L - 1), prefetch_kv=early)
+
+        seen = []
+        if use_graph:
+            step()
+            seen.append(out.clone())
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                step()
+        for _ in range(steps - len(seen)):
+            graph.replay() if use_graph else step()
+            seen.append(out.clone())
+        torch.cuda.synchronize()
+        assert cache.read_error() == 0 and cache.seq_lens.tolist() == [t + steps for t in T]
+        got.append((torch.stack(seen), cache.k.view(torch.uint8).clone(), cache.v.view(torch.uint8).clone()))
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.equal(a, b)
+
+
 def test_one_workspace_serves_calls_of_other_shapes(pkg):
     """Append, decode, prompts and short chunks of different batches through one workspace, in turn, twice."""
     av = pkg.attn_varlen

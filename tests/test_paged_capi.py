@@ -76,6 +76,8 @@ def test_more_refusals(lib):
     assert rc("decode", Hq=34, Hkv=2) == EUNSUPPORTED and rc("decode", D=256, Hq=18, page=64) == EUNSUPPORTED
     assert rc("decode", D=256, page=128) == EUNSUPPORTED
     assert rc("decode", e4m3=False, k_scales=0x60000) == EINVAL
+    assert rc("decode", flags=2) == EINVAL and rc("append", flags=1) == EINVAL
+    assert rc("prefill", cu_seqlens_q=CU, flags=1) == EINVAL
     assert rc("append", q_rot_out=None) == EINVAL and rc("append", q=None) == EINVAL
     assert rc("append", k_new=None, v_new=None) == EINVAL
     assert rc("prefill") == EINVAL, "prefill needs cu_seqlens_q"
