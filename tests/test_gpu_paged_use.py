@@ -211,6 +211,143 @@ def test_one_workspace_serves_calls_of_other_shapes(pkg):
             assert av.paged_read_error(ws) == 0
 
 
+@pytest.mark.parametrize("rot", [0, 32, 96])
+def test_partial_rotation_of_every_call(pkg, rot):
+    av = pkg.attn_varlen
+    for T, new in (([40, 3, 0], [1, 1, 1]), ([40, 3, 0], [3, 1, 2]), ([40, 3, 0], [70, 1, 90])):
+        c = H.make_cache(T, new, 1, 128, 32, True, seed=310)
+        n = sum(new)
+        q, k, v = rows((n, 4, 128), 311), rows((n, 1, 128), 312), rows((n, 1, 128), 313)
+        d, out = H.to_device(c), torch.zeros(n, 4, 128).half().cuda()
+        cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32).cuda()
+        kw = dict(k_scales=d["k_scales"], v_scales=d["v_scales"], rotary_dim=rot, rope_theta=1000.0)
+        if max(new) == 1:
+            av.paged_decode(q, d["k"], d["v"], out, d["table"], d["T"], k_new=k, v_new=v, **kw)
+        else:
+            av.paged_prefill(q, k, v, d["k"], d["v"], out, d["table"], d["T"], cu, max(new), **kw)
+        pos = [T[b] + i for b, m in enumerate(new) for i in range(m)]
+        seq = [b for b, m in enumerate(new) for _ in range(m)]
+        after = H.back(d)
+        H.check_append(c, after, "k", c["T"], cu.cpu(), c["table"], exact_rotation(k.cpu(), pos, rot, 1000.0), rot > 0)
+        H.check_attention(out.cpu(), exact_rotation(q.cpu(), pos, rot, 1000.0), after, c["table"], [p + 1 for p in pos], seq,
+                          128 ** -0.5, f"rot {rot}", q_fp16=max(new) > 16)
+
+
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_strided_operands_and_a_full_cache(pkg, e4m3):
+    """q, k and v as slices of one projection, a page table and scales that are slices too, T + 1 = capacity, and
+    no workspace given, under capture: its own is zeroed at every replay."""
+    av = pkg.attn_varlen
+    B, hq, hkv, D, page = 3, 6, 2, 64, 16
+    T = [3 * page - 1, 2 * page, 7]
+    c = H.make_cache(T, [1] * B, hkv, D, page, e4m3, seed=320)
+    d = H.to_device(c)
+    wide = torch.full((B, 9), -1, dtype=torch.int32).cuda()
+    wide[:, 2:5] = d["table"][:, :3]
+    table = wide[:, 2:5]
+    if e4m3:
+        for name in ("k_scales", "v_scales"):
+            s = d[name].view(torch.uint8)
+            both = torch.full((s.shape[1], 2, s.shape[0]), 200, dtype=torch.uint8).cuda()
+            both[:, 1] = s.t()
+            d[name] = both[:, 1].t().view(torch.float8_e8m0fnu)
+    qkv = rows((B, (hq + 2 * hkv) * D), 321).view(B, hq + 2 * hkv, D)
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
+    o2 = torch.zeros(B, hq, 2, D).half().cuda()
+    out = o2[:, :, 1]
+    kw = dict(k_scales=d["k_scales"], v_scales=d["v_scales"], k_new=k, v_new=v)
+    av.paged_decode(q, d["k"], d["v"], out, table, d["T"], **kw)
+    first = out.clone()
+    out.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        av.paged_decode(q, d["k"], d["v"], out, table, d["T"], **kw)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first) and (o2[:, :, 0] == 0).all()
+    exact = torch.stack([P.rope(q[b].cpu(), T[b], D, 10000.0) for b in range(B)])
+    after = H.back({n: (t if not (e4m3 and n.endswith("scales")) else t.view(torch.uint8).contiguous().view(torch.float8_e8m0fnu))
+                    for n, t in d.items()})
+    H.check_attention(out.cpu(), exact, after, c["table"], [t + 1 for t in T], range(B), D ** -0.5, "slices")
+
+
+@pytest.mark.parametrize("page,D,e4m3", [(64, 128, True), (16, 64, False)])
+def test_offsets_past_32_bits(pkg, page, D, e4m3):
+    """Pages behind 4 GB of a pool, read, appended to, expanded."""
+    av = pkg.attn_varlen
+    T, new = [130, 5], [1, 1]
+    c = H.make_cache(T, new if D != 128 else [80, 3], 2, D, page, e4m3, seed=330)
+    small = H.to_device(c)
+    num = c["k"].shape[0]
+    total = (5 << 30) // (2 * page * D * (1 if e4m3 else 2))
+    d = dict(small)
+    for name in ("k", "v"):
+        big = torch.empty((total,) + tuple(c[name].shape[1:]), dtype=torch.uint8 if e4m3 else torch.float16, device="cuda")
+        big[-num:] = small[name].view(big.dtype)
+        d[name] = big.view(small[name].dtype)
+        if e4m3:
+            sc = torch.full((total, 2), 127, dtype=torch.uint8, device="cuda")
+            sc[-num:] = small[name + "_scales"].view(torch.uint8)
+            d[name + "_scales"] = sc.view(torch.float8_e8m0fnu)
+    table = torch.where(small["table"] >= 0, small["table"] + (total - num), small["table"])
+
+    def tail():
+        return H.back({n: (t[-num:] if n != "table" and n != "T" and t is not None else t) for n, t in d.items()})
+
+    kw = dict(k_scales=d["k_scales"], v_scales=d["v_scales"])
+    q, k, v = rows((2, 4, D), 331), rows((2, 2, D), 332), rows((2, 2, D), 333)
+    out = torch.zeros_like(q)
+    av.paged_decode(q, d["k"], d["v"], out, table, d["T"], k_new=k, v_new=v, **kw)
+    exact = torch.stack([P.rope(q[b].cpu(), T[b], D, 10000.0) for b in range(2)])
+    H.check_attention(out.cpu(), exact, tail(), c["table"], [t + 1 for t in T], range(2), D ** -0.5, "far decode")
+    if D == 128:
+        cu = torch.tensor([0, 80, 83], dtype=torch.int32).cuda()
+        q, k, v = rows((83, 4, D), 334), rows((83, 2, D), 335), rows((83, 2, D), 336)
+        out = torch.zeros_like(q)
+        av.paged_prefill(q, k, v, d["k"], d["v"], out, table, d["T"], cu, 80, max_kv_tokens=300, **kw)
+        pos = [T[0] + i for i in range(80)] + [T[1] + i for i in range(3)]
+        H.check_attention(out.cpu(), exact_rotation(q.cpu(), pos, D), tail(), c["table"], [p + 1 for p in pos], [0] * 80 + [1] * 3,
+                          D ** -0.5, "far prefill", q_fp16=True)
+
+
+def test_thousands_of_sequences_and_too_many(pkg):
+    """A batch whose bookkeeping takes a good part of shared memory, and one that it does not hold: refused."""
+    av = pkg.attn_varlen
+    for B, fits in ((3000, True), (20000, False)):
+        pool = torch.full((8, 1, 16, 128), 0x30, dtype=torch.uint8).cuda().view(torch.float8_e4m3fn)
+        vals = torch.full((8, 1, 16, 128), 0x38, dtype=torch.uint8).cuda().view(torch.float8_e4m3fn)  # 1.0
+        scales = torch.full((8, 1), 127, dtype=torch.uint8).cuda().view(torch.float8_e8m0fnu)
+        table = (torch.arange(B * 2, dtype=torch.int32) % 8).view(B, 2).cuda()  # pages shared by many: read only
+        lens = (torch.arange(B, dtype=torch.int32) % 33).cuda()
+        q, out = rows((B, 2, 128), 340), torch.full((B, 2, 128), 7.0).half().cuda()
+        call = lambda: av.paged_decode(q, pool, vals, out, table, lens, k_scales=scales, v_scales=scales)  # noqa: E731
+        if not fits:
+            with pytest.raises(RuntimeError, match="batch too large"):
+                call()
+            continue
+        call()
+        torch.cuda.synchronize()
+        want = (lens > 0).half()[:, None, None].expand_as(out)  # values are all 1: the mean is 1, or 0 of none
+        assert torch.equal(out, want)
+
+
+def test_prefill_of_rows_that_belong_to_nobody(pkg):
+    """Offsets that name no row of the batch, and ones that run backwards: nothing is written, the latter is reported."""
+    av = pkg.attn_varlen
+    c = H.make_cache([20, 0], [90, 0], 1, 128, 16, True, seed=350)
+    d = H.to_device(c)
+    q, k = rows((100, 2, 128), 351), rows((100, 1, 128), 352)
+    ws = av.make_paged_workspace(2, 2, 1, 128, 100, 90, 400)
+    for offsets, err in (([0, 0, 0], 0), ([0, -3, 2], 1), ([0, 200, 200], 1), ([60, 60, 10], 1)):
+        out = torch.full_like(q, 7.0)
+        av.paged_prefill(q, k, k, d["k"], d["v"], out, d["table"], d["T"], torch.tensor(offsets, dtype=torch.int32).cuda(), 90,
+                         k_scales=d["k_scales"], v_scales=d["v_scales"], workspace=ws)
+        torch.cuda.synchronize()
+        assert av.paged_read_error(ws) == err, offsets
+        assert (out == 7.0).all() and torch.equal(H.bits(H.back(d)["k"]), H.bits(c["k"]))
+
+
 def test_entry_points_refuse_what_does_not_fit(pkg):
     av = pkg.attn_varlen
     c = H.make_cache([5, 6], [1, 1], 2, 128, 16, True, seed=250)
