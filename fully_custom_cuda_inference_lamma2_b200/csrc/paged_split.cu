@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                             x0 = rotated(x0, y.x, cs[(i - i0) * half + k], lowhalf);
                             x1 = rotated(x1, y.y, cs[(i - i0) * half + k + 1], lowhalf);
                         }
-                        if (p.q_rot && at.j == 0)
+                        if (p.q_rot && at.j == 0 && T >= 0)
                             *reinterpret_cast<uint32_t*>(p.q_rot + ((tok0 + i) * p.Hq + hq) * D + d) = pack_half2(x0, x1);
                     }
                     // (a rotation of the largest fp16 values passes fp16's range: the low part takes the rest)

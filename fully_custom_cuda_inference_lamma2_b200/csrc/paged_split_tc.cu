@@ -298,12 +298,13 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                         }
                         amax = fmaxf(amax, fabsf(x[e]));
                     }
-                    if (p.q_rot && at.j == 0 && c < rows)
+                    if (p.q_rot && at.j == 0 && c < rows && T >= 0)
                         *reinterpret_cast<uint2*>(p.q_rot + ((tok0 + i) * p.Hq + at.h * G + (r0 + c) - i * G) * D + d) =
                             make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
-                    const int e = exponent_448(redux_max(amax), -100, 100);
+                    const float largest = redux_max(amax);
+                    const int e = exponent_448(largest, -100, 100);
                     const float up = exp2_int(-e);
-                    if (lane == 0) qs_sm[c] = exp2_int(e) * p.scale_log2;
+                    if (lane == 0) qs_sm[c] = largest < INFINITY ? exp2_int(e) * p.scale_log2 : NAN;  // codes would saturate
 #pragma unroll
                     for (int j = 0; j < 4; ++j) x[j] *= up;
 #pragma unroll
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                     if (c >= rows) continue;
                     const float sum = (l_sm[c] + l_sm[COLS + c]) + (l_sm[2 * COLS + c] + l_sm[3 * COLS + c]);
                     const float o = of_parts(a[c], a[COLS + c], a[2 * COLS + c]);
-                    const float y = sum > 0.f ? o / sum : 0.f;
+                    const float y = sum == 0.f ? 0.f : o / sum;  // no key; a NaN stays one
                     if (whole) {
                         out_row(p, at, r0, c)[tid] = __float2half_rn(y);
                     } else {

@@ -336,6 +336,45 @@ def test_decode_largest_queries(av, e4m3):
     H.check_attention(out, rotated_queries(t), H.back(d), c["table"], [34, 201], [0, 1], 1e-6, "largest")
 
 
+@pytest.mark.parametrize("D,e4m3", [(128, True), (64, True), (128, False)])
+@pytest.mark.parametrize("T", [[40, 40, 40], [3000, 40, 3000]])
+def test_decode_nan_in_live_rows(av, D, e4m3, T):
+    """A NaN among the keys that a row sees makes the row NaN, one among the values its dim, and neither anything else."""
+    c = H.make_cache(T, [1] * 3, 2, D, 16, e4m3, seed=137)
+    t = new_tokens(c, 4, seed=138)
+    nan = torch.tensor(0x7F, dtype=torch.uint8).view(H.F8) if e4m3 else torch.tensor(float("nan"), dtype=torch.float16)
+    raw = lambda x: x.view(torch.uint8) if e4m3 else x  # noqa: E731
+    raw(c["k"])[int(c["table"][0, 1]), 1, 3, 7] = raw(nan)   # sequence 0, kv head 1, row 19
+    raw(c["v"])[int(c["table"][2, 2]), 0, 5, 9] = raw(nan)   # sequence 2, kv head 0, row 37, dim 9
+    d, out, q_rot, err = run_decode(av, c, t)
+    assert err == 0
+    want = torch.zeros(out.shape, dtype=torch.bool)
+    want[0, 2:] = True
+    want[2, :2, 9] = True
+    assert torch.equal(out.isnan(), want)
+
+
+@pytest.mark.parametrize("D,e4m3", [(128, True), (64, True), (128, False)])
+def test_decode_queries_that_are_not_finite(av, D, e4m3):
+    c = H.make_cache([200, 300], [1] * 2, 2, D, 16, e4m3, seed=139)
+    t = new_tokens(c, 4, seed=140)
+    t["q"][0, 1, 5] = float("inf")
+    t["q"][1, 2, 6] = float("nan")
+    d, out, q_rot, err = run_decode(av, c, t)
+    assert err == 0
+    want = torch.zeros(out.shape, dtype=torch.bool)
+    want[0, 1] = want[1, 2] = True
+    assert torch.equal(out.isnan(), want)
+
+
+@pytest.mark.parametrize("D,e4m3", [(128, True), (64, True), (128, False)])
+def test_decode_refused_sequence_keeps_q_rot(av, D, e4m3):
+    c = H.make_cache([50, 40, 30], [1] * 3, 2, D, 16, e4m3, seed=141)
+    c["T"] = torch.tensor([50, 16 * c["table"].shape[1], -5], dtype=torch.int32)
+    d, out, q_rot, err = run_decode(av, c, new_tokens(c, 4, seed=142))
+    assert err == CAPACITY and (q_rot[0] != 0).any() and (q_rot[1:] == 0).all() and (out[1:] == 0).all()
+
+
 @pytest.mark.parametrize("theta", [0.3, 1.0, 5e5, 1e30])
 def test_append_odd_thetas(av, theta):
     c = H.make_cache([1000, 3], [1, 1], 1, 64, 16, False, seed=135)
