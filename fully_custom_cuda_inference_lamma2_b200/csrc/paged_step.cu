@@ -86,7 +86,7 @@ static int fill(const fcci_paged_desc* d, Op op, Params& p, Freqs& f, WsLayout& 
     const int64_t pool_st[6] = {d->k_stride_p, d->k_stride_h, d->k_stride_t, d->v_stride_p, d->v_stride_h, d->v_stride_t};
     for (int64_t x : pool_st)
         if (x < 0 || (x * elt & 15)) return bad(FCCI_EINVAL, "strides must be non-negative multiples of 16 bytes");
-    if (d->k_stride_t * elt < d->D || d->v_stride_t * elt < d->D) return bad(FCCI_EINVAL, "the rows of a page overlap");
+    if (d->k_stride_t < d->D || d->v_stride_t < d->D) return bad(FCCI_EINVAL, "the rows of a page overlap");
     if (d->k_scales_stride_p < 0 || d->k_scales_stride_h < 0 || d->v_scales_stride_p < 0 || d->v_scales_stride_h < 0)
         return bad(FCCI_EINVAL, "negative scale stride");
     int dev = 0;
