@@ -15,6 +15,10 @@ namespace pg {
 constexpr int kMaxRot = 256;
 constexpr int kScaleMin = -15, kScaleMax = 8;  // exponents of a page's scale
 
+// Long chunks hold their rotated queries in fp16 times this: a rotation of the largest fp16 values reaches 92637, past
+// fp16's 65504. Their scale takes it back. (Halving is exact but for elements below 2^-13, then off by 2^-24.)
+constexpr float kLongQuery = 0.5f;
+
 struct Params {
     int32_t B, Hq, Hkv, G, D;
     int32_t total_q, max_q;

@@ -266,8 +266,12 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     if (E4M3) amax = fmaxf(fmaxf(amax, fmaxf(fabsf(u.x), fabsf(u.y))), fmaxf(fabsf(w.x), fabsf(w.y)));
                 }
             }
-            auto store16 = [&](__half* row, int i) {
-                auto two = [](float2 v) { return pack_half2(v.x, v.y); };
+            auto store16 = [&](__half* row, int i, float factor) {
+                const float2 f2 = make_float2(factor, factor);
+                auto two = [&](float2 v) {
+                    v = __fmul2_rn(v, f2);
+                    return pack_half2(v.x, v.y);
+                };
                 *reinterpret_cast<uint4*>(row + dlo) = make_uint4(two(x[i][0]), two(x[i][1]), two(x[i][2]), two(x[i][3]));
                 *reinterpret_cast<uint4*>(row + dhi) = make_uint4(two(x[i][4]), two(x[i][5]), two(x[i][6]), two(x[i][7]));
             };
@@ -330,9 +334,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     const int pos = p0 + row0 + i * RP;
                     __half* row = is_q ? p.q_rot + ((src_row + i * RP) * p.Hq + h) * D
                                        : reinterpret_cast<__half*>(page + (row0 + i * RP) * st);
-                    store16(row, i);
+                    store16(row, i, is_q && p.exp_k ? kLongQuery : 1.f);
                     if (!is_q && exp_row >= 0)
-                        store16((is_v ? p.exp_v : p.exp_k) + h * p.exp_sh + (exp_row + pos) * D, i);
+                        store16((is_v ? p.exp_v : p.exp_k) + h * p.exp_sh + (exp_row + pos) * D, i, 1.f);
                 }
             }
         }

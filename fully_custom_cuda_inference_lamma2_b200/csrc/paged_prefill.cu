@@ -5,9 +5,9 @@
 // small beside its products once a chunk has some dozens of query rows per kv head (shorter
 // ones take the split-KV kernels, which read the pages in place). code * 2^e is exact in fp16 for every scale that an
 // append makes, but for 256 * 2^8, which becomes 65504 (2^-11 of itself, an fp16 rounding). The rotated queries and the
-// weights are rounded once to fp16, as in the attention over an arena: holding the queries in two parts, as the split
-// kernels do, would add half to the products of a kernel that the products bound (results are off by 3.5e-4 to
-// 5.4e-4 in the 2-norm, 2.1e-4 of it their own rounding).
+// weights are rounded once to fp16, as in the attention over an arena (the queries halved, so that none passes its range):
+// holding the queries in two parts, as the split kernels do, would add half to the products of a kernel that the
+// products bound (results are off by 3.5e-4 to 5.4e-4 in the 2-norm, 2.1e-4 of it their own rounding).
 //
 // Measured: 2 x 2048 new tokens after 12000 to 14000, 64 / 8 heads: attention 1598 us, append 61, expansion 45 (3.6 TB/s
 // in and out); 16 prompts of 256 to 4096, 32 heads: attention 722 us, append 335.
@@ -184,7 +184,7 @@ int launch_prefill(const Params& base, const Freqs& f, bool e4m3, uint8_t* ws, c
     a.k_cache = p.exp_k, a.k_sh = p.exp_sh, a.k_st = p.D;
     a.v_cache = p.exp_v, a.v_sh = p.exp_sh, a.v_st = p.D;
     a.out = p.out, a.o_st = p.o_st, a.o_sh = p.o_sh;
-    a.scale_log2 = scale_log2;
+    a.scale_log2 = scale_log2 / kLongQuery;
     a.advance = advance;
     a.err = p.err;
     uint32_t* head = reinterpret_cast<uint32_t*>(ws + 32);

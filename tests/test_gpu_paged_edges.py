@@ -1,0 +1,56 @@
+"""GPU checks of the paged operators at the edges of their ranges: the largest queries and keys, scale bytes that no append
+makes, weights far below the largest, calls that are refused in part, bounds far above what a call holds."""
+import math
+
+import pytest
+import torch
+
+import paged_helpers as H
+from helpers import randn_half
+from oracle import paged_oracle as P
+from test_gpu_paged import (CAPACITY, DEV, check_whole_append, exact_rotation, new_tokens, rotated_queries, run_append,
+                            run_decode)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def av():
+    import fully_custom_cuda_inference_lamma2_b200 as pkg
+
+    return pkg.attn_varlen
+
+
+def prefill(av, c, t, scale=None, advance=False, max_new=None, max_kv=None, d=None):
+    """paged_prefill of t over c: device cache, out (7.0 where nothing was written), error word."""
+    d = d or H.to_device(c)
+    q, k, v = t["q"].to(DEV), t["k"].to(DEV), t["v"].to(DEV)
+    out = torch.full_like(q, 7.0)
+    B, hq, D = len(c["new"]), q.shape[1], q.shape[2]
+    most = max_new or max(c["new"])
+    kv = max_kv if max_kv is not None else sum(max(n, 0) for n in c["new"]) + int(c["T"].clamp(min=0).sum())
+    ws = av.make_paged_workspace(B, hq, c["hkv"], D, q.shape[0], most, kv)
+    av.paged_prefill(q, k, v, d["k"], d["v"], out, d["table"], d["T"], t["cu"].to(DEV), most, k_scales=d["k_scales"],
+                     v_scales=d["v_scales"], scale=-1.0 if scale is None else scale, advance=advance, workspace=ws,
+                     max_kv_tokens=kv)
+    torch.cuda.synchronize()
+    return d, out.cpu(), av.paged_read_error(ws)
+
+
+def seq_of_rows(c):
+    return [b for b, n in enumerate(c["new"]) for _ in range(n)]
+
+
+# ---------------------------------------------------------------- the largest queries and keys
+
+@pytest.mark.parametrize("e4m3", [True, False])
+@pytest.mark.parametrize("new", [[130, 65], [10, 3]])
+def test_prefill_largest_queries(av, e4m3, new):
+    """Queries whose rotation passes fp16's range, in long chunks and short ones: their scores are finite."""
+    c = H.make_cache([33, 200], new, 1, 128, 32, e4m3, seed=401)
+    t = new_tokens(c, 2, seed=402)
+    t["q"] = (torch.sign(t["q"].float()) * 65504.0).half()
+    d, out, err = prefill(av, c, t, scale=1e-6)
+    assert err == 0 and rotated_queries(t).abs().max() > 70000
+    H.check_attention(out, rotated_queries(t), H.back(d), c["table"], [p + 1 for p in t["pos"]], seq_of_rows(c), 1e-6,
+                      "largest queries", q_fp16=True)
