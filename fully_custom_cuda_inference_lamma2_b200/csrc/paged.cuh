@@ -18,6 +18,9 @@ constexpr int kScaleMin = -15, kScaleMax = 8;  // exponents of a page's scale
 // Long chunks hold their rotated queries in fp16 times this: a rotation of the largest fp16 values reaches 92637, past
 // fp16's 65504. Their scale takes it back. (Halving is exact but for elements below 2^-13, then off by 2^-24.)
 constexpr float kLongQuery = 0.5f;
+// The same for the keys of e4m3 pages, as an exponent: a page of scale 2^8 may hold rotated keys up to 352 * 2^8 = 90112.
+// (Exact but for codes below 2^-6 at scale 2^-15, then off by 2^-25 before the scale takes it back.)
+constexpr int kLongKeyExp = -1;
 
 struct Params {
     int32_t B, Hq, Hkv, G, D;

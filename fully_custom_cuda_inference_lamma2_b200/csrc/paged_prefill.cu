@@ -4,9 +4,9 @@
 // Expanding costs 1 byte in and 2 bytes out for each cached value, and the attention then reads 2; that is
 // small beside its products once a chunk has some dozens of query rows per kv head (shorter
 // ones take the split-KV kernels, which read the pages in place). code * 2^e is exact in fp16 for every scale that an
-// append makes, but for 256 * 2^8, which becomes 65504 (2^-11 of itself, an fp16 rounding). The rotated queries and the
-// weights are rounded once to fp16, as in the attention over an arena (the queries halved, so that none passes its range):
-// holding the queries in two parts, as the split kernels do, would add half to the products of a kernel that the
+// append makes, but for a value's 256 * 2^8, which becomes 65504 (2^-11 of itself, an fp16 rounding); rotated keys go up to
+// 352 * 2^8 and are expanded at half their size (paged.cuh: kLongKeyExp). The rotated queries and the weights are rounded once
+// to fp16, as in the attention over an arena (the queries halved, so that none passes its range): holding the queries in two parts, as the split kernels do, would add half to the products of a kernel that the
 // products bound (results are off by 3.5e-4 to 5.4e-4 in the 2-norm, 2.1e-4 of it their own rounding).
 //
 // Measured: 2 x 2048 new tokens after 12000 to 14000, 64 / 8 heads: attention 1598 us, append 61, expansion 45 (3.6 TB/s
@@ -16,6 +16,7 @@
 // them), the expansion of the rows cached before, the attention.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -128,8 +129,9 @@ __global__ void __launch_bounds__(kExpandThreads) paged_expand_kernel(const __gr
         __half2 scale;
         bool clamp = false;
         if constexpr (E4M3) {
-            const int e = (int)(is_v ? p.v_scales[id * p.vs_sp + h * p.vs_sh] : p.k_scales[id * p.ks_sp + h * p.ks_sh]) - 127;
-            scale = __float2half2_rn(exp2_int(e));
+            const int e = is_v ? (int)p.v_scales[id * p.vs_sp + h * p.vs_sh] - 127
+                               : (int)p.k_scales[id * p.ks_sp + h * p.ks_sh] - 127 + kLongKeyExp;
+            scale = __float2half2_rn(exp2_int(max(e, -126)));  // 0 from 2^-25 down: a byte that no append makes
             clamp = e >= kScaleMax;
         }
         for (int row = r0; row < rows; row += 4 * RPS) {
@@ -184,7 +186,7 @@ int launch_prefill(const Params& base, const Freqs& f, bool e4m3, uint8_t* ws, c
     a.k_cache = p.exp_k, a.k_sh = p.exp_sh, a.k_st = p.D;
     a.v_cache = p.exp_v, a.v_sh = p.exp_sh, a.v_st = p.D;
     a.out = p.out, a.o_st = p.o_st, a.o_sh = p.o_sh;
-    a.scale_log2 = scale_log2 / kLongQuery;
+    a.scale_log2 = scale_log2 / (kLongQuery * (e4m3 ? ldexpf(1.f, kLongKeyExp) : 1.f));
     a.advance = advance;
     a.err = p.err;
     uint32_t* head = reinterpret_cast<uint32_t*>(ws + 32);

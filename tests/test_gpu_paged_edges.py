@@ -54,3 +54,23 @@ def test_prefill_largest_queries(av, e4m3, new):
     assert err == 0 and rotated_queries(t).abs().max() > 70000
     H.check_attention(out, rotated_queries(t), H.back(d), c["table"], [p + 1 for p in t["pos"]], seq_of_rows(c), 1e-6,
                       "largest queries", q_fp16=True)
+
+
+@pytest.mark.parametrize("new", [[130, 40], [9, 3], [1, 1]])
+def test_prefill_largest_keys_of_e4m3_pages(av, new):
+    """Rotated keys above fp16's range, new ones and cached ones: a chunk of any length sees what the pages hold."""
+    T = [100, 37]
+    c = H.make_cache(T, new, 2, 128, 16, True, seed=403)
+    g = torch.Generator().manual_seed(404)
+    live = c["k"].view(torch.uint8) != 0x7F
+    big = torch.tensor([288.0, 320.0, 352.0, -352.0, 256.0, -288.0])[torch.randint(0, 6, c["k"].shape, generator=g)]
+    c["k"] = torch.where(live, big.to(H.F8).view(torch.uint8), c["k"].view(torch.uint8)).view(H.F8)
+    c["k_scales"].fill_(135)
+    t = new_tokens(c, 4, seed=405)
+    t["k"] = (torch.sign(t["k"].float()) * 65504.0).half()
+    d, out, err = prefill(av, c, t, scale=1e-6)
+    assert err == 0
+    after = H.back(d)
+    assert float(after["k"].float().nan_to_num(0).abs().max()) * 256 > 80000
+    H.check_attention(out, rotated_queries(t), after, c["table"], [p + 1 for p in t["pos"]], seq_of_rows(c), 1e-6, "largest keys",
+                      q_fp16=max(new) * 2 > 64)
