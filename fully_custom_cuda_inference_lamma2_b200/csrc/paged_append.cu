@@ -19,6 +19,10 @@ namespace pg {
 constexpr int kTokenWarps = 16, kTokenThreads = kTokenWarps * 32;
 constexpr int kTokenTasks = 4;  // rows of a warp, at most
 
+// 2^(from - to), from what a page had to what it takes; at least the least normal number, which leaves a code nothing either.
+// (A page that no append has filled may have any scale byte.)
+__device__ __forceinline__ float rescale(int from, int to) { return exp2_int(max(from - to, -126)); }
+
 // One token per sequence. A warp takes `tasks` rows (query heads, or the key or value of a kv head): one when there are few
 // sequences, so that the rows spread over as many warps as there are, else up to four, whose loads are
 // under way together while the CTA gets through the chain length -> page -> scale and the angles, which all rows share.
@@ -111,7 +115,7 @@ __global__ void __launch_bounds__(kTokenThreads) paged_append_token_kernel(const
                 int ex = scale_exponent(amax);
                 if (off && ex > had[k]) {
                     // the rows before this one take the larger scale (rare: the page's largest value grew past a power of two)
-                    const float down = exp2_int(max(had[k], -126) - ex);
+                    const float down = rescale(had[k], ex);
                     for (int i = lane; i < off * (D / 4); i += 32) {
                         uint32_t* w = reinterpret_cast<uint32_t*>(page + (i / (D / 4)) * st + (i % (D / 4)) * 4);
                         const uint32_t c = *w;
@@ -122,7 +126,7 @@ __global__ void __launch_bounds__(kTokenThreads) paged_append_token_kernel(const
                     }
                 }
                 ex = max(ex, had[k]);
-                const float up = exp2_int(-ex);
+                const float up = rescale(0, ex);
                 if constexpr (E == 2) {
                     *reinterpret_cast<uint16_t*>(page + off * st + d0) = (uint16_t)e4m3x2(x[0] * up, x[1] * up);
                 } else {
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     int ex = scale_exponent(amax);
                     const bool grows = old && ex > had;
                     ex = max(ex, had);
-                    const float up = exp2_int(-ex), down = grows ? exp2_int(max(had, -126) - ex) : 1.f;
+                    const float up = rescale(0, ex), down = grows ? rescale(had, ex) : 1.f;
                     const float2 up2 = make_float2(up, up);
                     auto four = [&](float2 u, float2 w) {
                         u = __fmul2_rn(u, up2), w = __fmul2_rn(w, up2);

@@ -74,3 +74,52 @@ def test_prefill_largest_keys_of_e4m3_pages(av, new):
     assert float(after["k"].float().nan_to_num(0).abs().max()) * 256 > 80000
     H.check_attention(out, rotated_queries(t), after, c["table"], [p + 1 for p in t["pos"]], seq_of_rows(c), 1e-6, "largest keys",
                       q_fp16=max(new) * 2 > 64)
+
+
+# ---------------------------------------------------------------- scale bytes that no append makes
+
+@pytest.mark.parametrize("how", ["token", "rows", "decode"])
+@pytest.mark.parametrize("byte", [0, 1, 3, 7, 20, 90, 111])
+def test_append_to_a_page_of_a_tiny_scale(av, how, byte):
+    """Rows on a page whose scale is far below the new one are rounded to zero, never to something larger."""
+    T, page = [5, 20, 31], 32
+    new = [1, 1, 1] if how != "rows" else [2, 5, 1]
+    for factor in (3.0, 400.0, 20000.0):
+        c = H.make_cache(T, new, 2, 128, page, True, seed=411)
+        c["k_scales"].fill_(byte)
+        c["v_scales"].fill_(byte)
+        t = new_tokens(c, 2, seed=412)
+        for x in "kv":
+            t[x] = (t[x].float() * factor).clamp(-60000, 60000).half()
+        if how == "decode":
+            d, out, q_rot, err = run_decode(av, c, t)
+            assert out.isfinite().all()
+        else:
+            d, q_rot, err = run_append(av, c, t, how == "rows")
+        assert err == 0
+        check_whole_append(c, t, d, q_rot, 128)
+
+
+@pytest.mark.parametrize("how", ["token", "rows", "decode"])
+@pytest.mark.parametrize("byte", [136, 150, 200, 253, 254])
+def test_append_to_a_page_of_a_large_scale(av, how, byte):
+    """A present scale above the new rows' own is kept; the rows round to it, infinities saturate."""
+    T, page = [5, 20], 32
+    new = [1, 1] if how != "rows" else [2, 5]
+    c = H.make_cache(T, new, 1, 128, page, True, seed=413)
+    c["v_scales"].fill_(byte)
+    t = new_tokens(c, 2, seed=414)
+    t["v"] = (t["v"].float() * 20000).clamp(-60000, 60000).half()
+    first = [int(x) for x in t["cu"][:-1]]
+    t["v"][first[0], 0, 3], t["v"][first[1], 0, 4] = float("inf"), float("-inf")
+    d, q_rot, err = run_decode(av, c, t)[::2] + (0,) if how == "decode" else run_append(av, c, t, how == "rows")
+    after = H.back(d)
+    got = after["v"].view(torch.uint8)
+    for b in range(2):
+        p = int(c["table"][b, 0])
+        assert int(after["v_scales"][p, 0]) == byte
+        assert torch.equal(got[p, 0, : T[b]], c["v"].view(torch.uint8)[p, 0, : T[b]])
+        for i in range(new[b]):
+            x = t["v"][first[b] + i, 0].double() * 2.0 ** (127 - byte)
+            want = P.e4m3_grid(x.clamp(-448, 448))
+            assert torch.equal(after["v"][p, 0, T[b] + i].double(), want), (b, i)
