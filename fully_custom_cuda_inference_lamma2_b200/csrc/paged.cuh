@@ -129,6 +129,13 @@ __device__ __forceinline__ uint32_t half2_of_e4m3x2(uint32_t codes) {
     return h;
 }
 
+// fp16's 2^xe of a page with scale 2^e. A scale above those that an append makes may hold values that fp16 cannot: it is
+// reported, and cut so that zeros stay zeros. Below 2^-25 it is 0.
+__device__ __forceinline__ __half2 expansion_scale(const Params& p, int e, int xe) {
+    if (e > kScaleMax) set_error(p, FCCI_DEV_ERR_SCALE);
+    return __float2half2_rn(exp2_int(max(-126, min(xe, 15))));
+}
+
 // Eight e4m3 codes times the scale, as fp16; clamp: the product may pass 65504.
 __device__ __forceinline__ uint4 expanded(uint2 codes, __half2 scale, bool clamp) {
     uint32_t h[4] = {half2_of_e4m3x2(codes.x & 0xffffu), half2_of_e4m3x2(codes.x >> 16),

@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                             if (exp_row >= 0) {
                                 __half* er = (is_v ? p.exp_v : p.exp_k) + h * p.exp_sh + (exp_row + pos) * D;
                                 const int xe = is_k ? ex + kLongKeyExp : ex;
-                                const __half2 s2 = __float2half2_rn(exp2_int(xe));
+                                const __half2 s2 = expansion_scale(p, ex, xe);
                                 *reinterpret_cast<uint4*>(er + dlo) = expanded(u, s2, xe >= kScaleMax);
                                 *reinterpret_cast<uint4*>(er + dhi) = expanded(w, s2, xe >= kScaleMax);
                             }

@@ -129,10 +129,10 @@ __global__ void __launch_bounds__(kExpandThreads) paged_expand_kernel(const __gr
         __half2 scale;
         bool clamp = false;
         if constexpr (E4M3) {
-            const int e = is_v ? (int)p.v_scales[id * p.vs_sp + h * p.vs_sh] - 127
-                               : (int)p.k_scales[id * p.ks_sp + h * p.ks_sh] - 127 + kLongKeyExp;
-            scale = __float2half2_rn(exp2_int(max(e, -126)));  // 0 from 2^-25 down: a byte that no append makes
-            clamp = e >= kScaleMax;
+            const int e = (int)(is_v ? p.v_scales[id * p.vs_sp + h * p.vs_sh] : p.k_scales[id * p.ks_sp + h * p.ks_sh]) - 127;
+            const int xe = is_v ? e : e + kLongKeyExp;
+            scale = expansion_scale(p, e, xe);
+            clamp = xe >= kScaleMax;
         }
         for (int row = r0; row < rows; row += 4 * RPS) {
             uint4 x[4];

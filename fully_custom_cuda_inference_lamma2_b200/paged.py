@@ -98,7 +98,8 @@ class PagedKVCache:
         self.seq_lens[seq].zero_()
 
     def read_error(self, clear: bool = True) -> int:
-        """The device error word (bit 0 capacity, 1 timeout, 3 page outside the pool); synchronises."""
+        """The device error word (bit 0 capacity, 1 timeout, 3 page outside the pool, 4 a scale byte
+        that no append makes, in a long chunk); synchronises."""
         return attn_varlen.paged_read_error(self.workspace, clear)
 
 

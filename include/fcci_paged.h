@@ -18,7 +18,7 @@
  *                        sizing, zeroing and error readback of the caller-owned workspace
  *
  * Status codes, fcci_last_status and fcci_last_error_string are those of fcci_decode.h, and
- * so are the bits of the device error word, with one more:
+ * so are the bits of the device error word, with two more:
  */
 #ifndef FCCI_PAGED_H
 #define FCCI_PAGED_H
@@ -37,6 +37,9 @@ extern "C" {
 
 #define FCCI_DEV_ERR_PAGE 8u /* a page that a live row needs is not in [0, num_pages): never
                                 dereferenced; the sequence's results are not to be used */
+#define FCCI_DEV_ERR_SCALE 16u /* a prefill of long chunks read a page of scale above 2^8, which no append
+                                  makes and whose values its fp16 rows may not hold: the sequence's
+                                  results are not to be used */
 
 /* cache_type */
 #define FCCI_PAGED_F16 0
@@ -54,7 +57,10 @@ extern "C" {
  *                page = page_table[b*page_table_stride + t / page_size]; fp16, or e4m3 codes
  *                (cache_type FCCI_PAGED_E4M3, strides then in bytes)
  *   scales       e4m3 only: byte s at scales + page*stride_p + h*stride_h says 2^(s - 127); a
- *                row's values are code * 2^(s - 127)
+ *                row's values are code * 2^(s - 127). 255 is none; of a page without live rows the
+ *                byte may be anything. A prefill of more than 64 query rows of one kv head (max_seqlen_q *
+ *                Hq / Hkv) takes those that an append makes, 112 to 135: smaller ones lose what is below
+ *                2^-25, larger ones are reported (FCCI_DEV_ERR_SCALE)
  *   T_b          seq_lens[b] (device int32, read on device): rows already cached. T_b + n_b
  *                must not exceed max_pages * page_size
  *   RoPE         rotate-half on the first rotary_dim dims (a multiple of 16, 0 disables it)

@@ -123,3 +123,37 @@ def test_append_to_a_page_of_a_large_scale(av, how, byte):
             x = t["v"][first[b] + i, 0].double() * 2.0 ** (127 - byte)
             want = P.e4m3_grid(x.clamp(-448, 448))
             assert torch.equal(after["v"][p, 0, T[b] + i].double(), want), (b, i)
+
+
+@pytest.mark.parametrize("new", [[130, 40], [130, 0]])
+def test_long_chunk_over_pages_of_a_scale_past_fp16(av, new):
+    """Long chunks hold cached rows in fp16: a live page whose scale no append makes (above 2^8) is reported, and what it
+    holds becomes no NaN; one that is far below holds zeros, which are exact."""
+    T = [40, 37]
+    c = H.make_cache(T, new, 1, 128, 16, True, seed=415)
+    t = new_tokens(c, 2, seed=416)
+    page = int(c["table"][0, 1])
+    for byte, err_want in ((136, 16), (143, 16), (150, 16), (254, 16), (135, 0), (0, 0)):
+        for name in "kv":
+            e = c[name + "_scales"].clone()
+            e[page, 0] = byte
+            codes = c[name].view(torch.uint8).clone()
+            codes[page] = 0
+            cc = dict(c, **{name + "_scales": e, name: codes.view(H.F8)})
+            d, out, err = prefill(av, cc, t)
+            assert err == err_want, (byte, name)
+            assert out.isfinite().all()
+            if err == 0 or name == "v":  # zeros are zeros at any scale
+                n = len(t["pos"])
+                H.check_attention(out[:n], rotated_queries(t), H.back(d), c["table"], [p + 1 for p in t["pos"]], seq_of_rows(c),
+                                  128 ** -0.5, f"byte {byte}", q_fp16=True)
+
+
+def test_long_chunk_appends_to_a_page_of_a_scale_past_fp16(av):
+    """The same for a page that gets the chunk's first rows and keeps its scale."""
+    for byte, err_want in ((140, 16), (135, 0)):
+        c = H.make_cache([5], [130], 1, 128, 16, True, seed=417)
+        c["v"].view(torch.uint8)[int(c["table"][0, 0])] = 0
+        c["v_scales"][int(c["table"][0, 0])] = byte
+        d, out, err = prefill(av, c, new_tokens(c, 2, seed=418))
+        assert err == err_want and out.isfinite().all()
