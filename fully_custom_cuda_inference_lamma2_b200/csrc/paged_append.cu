@@ -169,7 +169,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
     const int b = blockIdx.y;
     const Seq s = seq_of(p, b);
     const int64_t first = ((int64_t)(s.T >> p.page_log2) + blockIdx.x) << p.page_log2;
-    const bool here = s.ok && s.n > 0 && first < (int64_t)s.T + s.n;
+    // a long chunk's plan has given rows to every sequence that is served
+    const bool served = !p.exp_k || (s.ok && p.cu_kv[b + 1] - p.cu_kv[b] == s.T + s.n);
+    const bool here = s.ok && served && s.n > 0 && first < (int64_t)s.T + s.n;
     const int p0 = here ? (int)first : 0;  // first position of the page
     if (!s.ok) {
         if (blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
         const int per = (heads + gridDim.z - 1) / gridDim.z;
         const int h_end = min(heads, (int)(blockIdx.z + 1) * per);
         // a long chunk's attention reads fp16 rows: write these while they are here
-        const int64_t exp_row = p.exp_k && p.cu_kv[b + 1] - p.cu_kv[b] == s.T + s.n ? p.cu_kv[b] : -1;
+        const int64_t exp_row = p.exp_k ? p.cu_kv[b] : -1;
         // passes whose row is new, and those whose row the page held before
         uint32_t is_new = 0, is_old = 0;
 #pragma unroll

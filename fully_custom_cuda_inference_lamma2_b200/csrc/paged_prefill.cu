@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
     __syncthreads();
     if (need > max_items) {
         // only offsets that run backwards, so that sequences share rows, can ask for so many: nothing is served
+        for (int b = threadIdx.x; b <= p.B; b += kPlanThreads) cu_kv[b] = 0;
         if (threadIdx.x == 0) {
             set_error(p, FCCI_DEV_ERR_CAPACITY);
             *a.n_items = 0;

@@ -157,3 +157,43 @@ def test_long_chunk_appends_to_a_page_of_a_scale_past_fp16(av):
         c["v_scales"][int(c["table"][0, 0])] = byte
         d, out, err = prefill(av, c, new_tokens(c, 2, seed=418))
         assert err == err_want and out.isfinite().all()
+
+
+# ---------------------------------------------------------------- calls that are refused in part
+
+def test_long_chunk_without_room_leaves_its_pages(av):
+    """A sequence whose expanded keys have no room is not served: its pages, scales, rows of out and length stay."""
+    T, new = [20, 30, 10], [70, 100, 66]
+    c = H.make_cache(T, new, 2, 128, 16, True, seed=421)
+    t = new_tokens(c, 4, seed=422)
+    for name in "kv":
+        t[name] = (t[name].float() * 100).clamp(-60000, 60000).half()  # would grow the scale of the page that holds row T
+    # the first and the third fit, the second does not
+    d, out, err = prefill(av, c, t, advance=True, max_kv=20 + 70 + 10 + 66 + 20)
+    assert err == CAPACITY and d["T"].cpu().tolist() == [90, 30, 76]
+    after = H.back(d)
+    mine = c["table"][1][c["table"][1] >= 0].long()
+    for name in "kv":
+        assert torch.equal(after[name].view(torch.uint8)[mine], c[name].view(torch.uint8)[mine]), "pages of the refused sequence"
+        assert torch.equal(after[name + "_scales"][mine], c[name + "_scales"][mine]), "scales of the refused sequence"
+    rows = list(range(70)) + list(range(170, 236))
+    assert (out[70:170] == 7.0).all()
+    pos = [t["pos"][r] for r in rows]
+    H.check_attention(out[rows], exact_rotation(t["q"][rows], pos, 128), after, c["table"], [p + 1 for p in pos],
+                      [0] * 70 + [2] * 66, 128 ** -0.5, "others", q_fp16=True)
+
+
+def test_long_chunk_of_offsets_that_share_rows(av):
+    """Offsets that run backwards, so that more work is asked for than the rows of the call allow: nothing is served, and
+    lengths, pages and scales stay."""
+    n, B = 2560, 5
+    c = H.make_cache([3] * B, [n, 0, n, 0, n], 1, 128, 128, True, seed=423)
+    c["new"] = [n, 0, 0, 0, 0]
+    t = new_tokens(c, 2, seed=424)
+    t["cu"] = torch.tensor([0, n, 0, n, 0, n], dtype=torch.int32)
+    d, out, err = prefill(av, c, t, advance=True, max_new=n, max_kv=3 * (n + 3))
+    assert err == CAPACITY and d["T"].cpu().tolist() == [3] * B and (out == 7.0).all()
+    after = H.back(d)
+    for name in "kv":
+        assert torch.equal(after[name].view(torch.uint8), c[name].view(torch.uint8))
+        assert torch.equal(after[name + "_scales"], c[name + "_scales"])
