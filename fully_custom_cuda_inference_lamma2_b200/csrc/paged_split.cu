@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
             ring.next();
         }
     }
-    advance_lengths(p, misc + 2);
+    if (line.N > 0) advance_lengths(p, misc + 2);  // no place on the line: no new token, or nothing is served
 }
 
 template <int D, int NB, bool E4M3>

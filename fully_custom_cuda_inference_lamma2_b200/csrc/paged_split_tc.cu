@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, C::TMEM);
     }
-    advance_lengths(p, misc + 2);
+    if (line.N > 0) advance_lengths(p, misc + 2);  // no place on the line: no new token, or nothing is served
 }
 
 template <int NB>

@@ -197,3 +197,25 @@ def test_long_chunk_of_offsets_that_share_rows(av):
     for name in "kv":
         assert torch.equal(after[name].view(torch.uint8), c[name].view(torch.uint8))
         assert torch.equal(after[name + "_scales"], c[name + "_scales"])
+
+
+@pytest.mark.parametrize("D,e4m3", [(128, True), (64, True), (128, False)])
+def test_lengths_past_what_a_line_holds(av, D, e4m3):
+    """Sequences of 2^30 rows are more tiles than the line's numbers hold: the call is reported, and neither the lengths nor
+    out nor the pages change. (No page of them is looked up.)"""
+    page, pages = 16, 1 << 26
+    B, hkv = 2, 2
+    kind = H.F8 if e4m3 else torch.float16
+    pool = torch.zeros(4, hkv, page, D, dtype=torch.uint8 if e4m3 else torch.float16, device=DEV)
+    scales = torch.full((4, hkv), 127, dtype=torch.uint8, device=DEV).view(H.E8) if e4m3 else None
+    table = torch.full((B, pages), -1, dtype=torch.int32, device=DEV)
+    lens = torch.full((B,), 1 << 29, dtype=torch.int32, device=DEV)
+    q, k = randn_half((B, 4, D), 425).to(DEV), randn_half((B, hkv, D), 426).to(DEV)
+    out = torch.full_like(q, 7.0)
+    ws = av.make_paged_workspace(B, 4, hkv, D, B)
+    before = pool.clone()
+    av.paged_decode(q, pool.view(kind), pool.view(kind), out, table, lens, k_scales=scales, v_scales=scales, k_new=k, v_new=k,
+                    advance=True, workspace=ws)
+    torch.cuda.synchronize()
+    assert av.paged_read_error(ws) == CAPACITY
+    assert lens.tolist() == [1 << 29] * B and (out == 7.0).all() and torch.equal(pool, before)
