@@ -14,7 +14,8 @@
 // the product of each 16 keys, in fp32, so no scale can leave fp16's range. The queries are
 // rotated here in fp32 and split in two fp16 parts (hi + lo): one rounding of them to fp16 would
 // be the largest error of the whole step (3.6e-4 instead of 2.4e-4 of the result, 2.1e-4 of it its own rounding).
-// P is rounded to fp16 (relative 2^-11, weights in [0, 1]).
+// P is rounded to fp16 (relative 2^-11), times 2^14, so that fp16's least numbers are 2^-38 of the largest weight: with the
+// largest at 1 the keys below 2^-25 of it were lost, a quarter of what 16384 keys of 2^-26 beside one share.
 //
 // Measured: fp16 pages, 17 sequences of 1 to 5000 keys, 8 kv heads, group 3: 40 us (4.7 TB/s).
 #include <cuda.h>
@@ -30,6 +31,7 @@ namespace fcci {
 namespace pg {
 
 constexpr int kThreads = kCompute + 64;
+constexpr float kSplitTop = 14.f;  // log2 of the weight of the largest score
 
 template <int D, int NB, bool E4M3>
 struct Cfg {
@@ -316,11 +318,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                         const float mu = mn == -INFINITY ? 0.f : mn;  // a row that has seen no key yet
                         al[c] = ex2(m[nb][c] - mu);
                         m[nb][c] = mn;
+                        const float zero = mu - kSplitTop;  // the score of weight 1
                         float sum = 0.f;
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
-                            x[mt][nb][c] = ex2(x[mt][nb][c] - mu);
-                            x[mt][nb][c + 2] = ex2(x[mt][nb][c + 2] - mu);
+                            x[mt][nb][c] = ex2(x[mt][nb][c] - zero);
+                            x[mt][nb][c + 2] = ex2(x[mt][nb][c + 2] - zero);
                             sum += x[mt][nb][c] + x[mt][nb][c + 2];
                         }
                         l[nb][c] = l[nb][c] * al[c] + sum;
@@ -474,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
                             __half* o16 = out_row(p, at, r0, c);
                             float* o32 = sp.part_o + (part * kMaxCols + c) * D;
                             if (!whole && g == 0)
-                                sp.part_lse[part * kMaxCols + c] = l[nb][k] > 0.f ? m[nb][k] + __log2f(l[nb][k]) : -INFINITY;
+                                sp.part_lse[part * kMaxCols + c] = l[nb][k] > 0.f ? m[nb][k] - kSplitTop + __log2f(l[nb][k]) : -INFINITY;
 #pragma unroll
                             for (int mb = 0; mb < KSTEPS; ++mb) {
                                 const float y0 = (k ? acc[nb][mb][0].y : acc[nb][mb][0].x) * inv;

@@ -159,6 +159,37 @@ def test_long_chunk_appends_to_a_page_of_a_scale_past_fp16(av):
         assert err == err_want and out.isfinite().all()
 
 
+# ---------------------------------------------------------------- weights far below the largest
+
+@pytest.mark.parametrize("D,e4m3", [(64, False), (128, False), (256, False), (64, True), (256, True)])
+def test_decode_many_keys_far_below_one(av, D, e4m3):
+    """One key of value 0 takes nearly all of every row, and what 16384 others of value 1 share (e^-gap each) is the
+    result. They all lie behind it in one CTA's stretch: 600 sequences name the same pages, two units a CTA.
+
+    A weight is off by 2^-11 of itself at most as fp16 (2^-12 as three parts), the sums by 16384 * 2^-24 and the result by
+    2^-12 and 2^-25. Weights below 2^-28 of the largest need not count: gap 18 is 2^-26."""
+    T, B, page = 16384, 600, 32
+    for gap, lost in ((14.0, 0.0), (18.0, 0.0)):
+        num = T // page
+        k = torch.zeros(num, 1, page, D)
+        v = torch.ones(num, 1, page, D)
+        k[0, 0, 0, 0], v[0, 0, 0] = 8.0, 0.0
+        kind = H.F8 if e4m3 else torch.float16
+        k, v = k.to(kind).to(DEV), v.to(kind).to(DEV)
+        scales = torch.full((num, 1), 127, dtype=torch.uint8, device=DEV).view(H.E8) if e4m3 else None
+        table = torch.arange(num, dtype=torch.int32, device=DEV).expand(B, num).contiguous()
+        lens = torch.full((B,), T, dtype=torch.int32, device=DEV)
+        q = torch.zeros(B, 2, D, dtype=torch.float16, device=DEV)
+        q[:, :, 0] = 8.0
+        out = torch.empty_like(q)
+        av.paged_decode(q, k, v, out, table, lens, k_scales=scales, v_scales=scales, scale=gap / 64.0)
+        rest = (T - 1) * math.exp(-gap)
+        want = rest / (1 + rest)
+        tol = want * (2.0 ** -10 + 2 * T * 2.0 ** -24) + 2.0 ** -25
+        worst = float((out.double() - want).abs().max())
+        assert worst <= tol, f"gap {gap}: {worst / want:.3g} of the result lost"
+
+
 # ---------------------------------------------------------------- calls that are refused in part
 
 def test_long_chunk_without_room_leaves_its_pages(av):
