@@ -355,8 +355,10 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 for (int ch = 0; ch < 8; ++ch)
                     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(TL::cell(v32, tid, ch)), "r"(0) : "memory");
             }
-            const float lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);
-            const float inv_vs = live ? exp2_int(127 - (int)(__float_as_uint(vs) >> 23)) : 0.f;
+            // (values of 448 * 2^-60 are 0 in the result; without that bound a zeroed cache's scales of 2^-127 make the sum infinite)
+            const int ev = max(-60, min(126, (int)(__float_as_uint(vs) >> 23) - 127));
+            const float lv = (float)ev;
+            const float inv_vs = live ? exp2_int(-ev) : 0.f;
             // ---- scores of this key, in the log2 domain, with V's exponent
             wait(&bar->s_full[it & 1], it >> 1);
             tc::fence_after_sync();

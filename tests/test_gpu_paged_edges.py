@@ -190,6 +190,25 @@ def test_decode_many_keys_far_below_one(av, D, e4m3):
         assert worst <= tol, f"gap {gap}: {worst / want:.3g} of the result lost"
 
 
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("byte", [0, 10, 100, 127])
+def test_decode_over_a_zeroed_cache(av, D, byte):
+    """Codes and scale bytes of a cache that was zeroed, also where a sequence is cut over many CTAs: zeros."""
+    T = [5000, 1, 0, 300]
+    c = H.make_cache(T, [1] * 4, 1, D, 16, True, seed=443, poison=False)
+    for name in "kv":
+        c[name].view(torch.uint8).zero_()
+        c[name + "_scales"].fill_(byte)
+    d, out, q_rot, err = run_decode(av, c, new_tokens(c, 4, seed=444), append=False)
+    assert err == 0 and (out == 0).all()
+    # a row of ones at the end of each
+    t = new_tokens(c, 4, seed=445)
+    t["v"].fill_(1.0)
+    d, out, q_rot, err = run_decode(av, c, t, scale=1e-9)
+    n = torch.tensor(T).double()[:, None, None] + 1  # scores of 1e-9 * 128 at most: equal weights, 1 / n in each dim
+    assert err == 0 and ((out.double() * n - 1).abs() <= 2.0 ** -10 + 5001 * 2.0 ** -24 + n * 2.0 ** -25).all()
+
+
 # ---------------------------------------------------------------- calls that are refused in part
 
 def test_long_chunk_without_room_leaves_its_pages(av):
