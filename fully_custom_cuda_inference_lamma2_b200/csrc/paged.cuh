@@ -109,16 +109,13 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
-__device__ __forceinline__ uint32_t e4m3x2_of_half2(uint32_t h) {
-    uint16_t c;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(h));
-    return c;
-}
-
-// 16 (a - b), exact where b is the e4m3 rounding of a
-__device__ __forceinline__ uint32_t half2_rest16(uint32_t a, uint32_t b) {
-    const __half2 r = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b)),
-                              __float2half2_rn(16.f));
+// e5m2 is fp16's upper byte. The codes of four fp16 values, cut (not rounded) to three bits each, and 8 times what that
+// leaves of two of them, which is exact.
+__device__ __forceinline__ uint32_t e5m2x4_of_half4(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7531); }
+__device__ __forceinline__ uint32_t half2_rest8(uint32_t a) {
+    const uint32_t cut = a & 0xff00ff00u;
+    const __half2 r = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&cut)),
+                              __float2half2_rn(8.f));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 

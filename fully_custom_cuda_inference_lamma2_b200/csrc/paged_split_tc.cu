@@ -4,19 +4,25 @@
 //
 // The e4m3 codes go into tcgen05 (kind::f8f6f4, fp32 sums) as they lie in shared memory. With mma.sync they would
 // have to become fp16 in registers first, and that conversion unit (16 lanes a cycle and SM, for 2 codes each)
-// bound that kernel at 59 % of the memory rate. The other operand keeps its precision as a sum of
-// three e4m3 values, p0 + p1 / 16 + p2 / 256, each the rounding of what the ones before left, times 16 (within 2^-12 of
-// the value, or 2^-18 absolute), as three rows of the same product:
-//   S^T[key, (part, row)] = K Q^T     A = the K tile (128 keys), B = 3 * COLS rows of query parts
-//   O^T[dim, (part, row)] += V^T P^T  A = the V tile read dim-major, B = the weight parts, 3 * COLS bytes of each
-//                                     key side by side (N-major), which is what the key's thread has
-// The parts are summed where S is read, and where O is read at a unit's end. (Unscaled parts would lose every weight below
-// 2^-16 of the largest: the many small ones beside a key that takes most of the attention.)
+// bound that kernel at 59 % of the memory rate. The other operand keeps its precision as a sum of 8-bit parts, rows of the
+// same product:
+// S^T[key, (part, row)] = K Q^T     A = the K tile (128 keys), B = 3 * COLS rows of query parts, e4m3
+// O^T[dim, (part, row)] += V^T P^T  A = the V tile read dim-major, B = the weight parts, e5m2, 4 * COLS bytes of each
+//                                   key side by side (N-major), which is what the key's thread has
+// The parts are summed where S is read, and where O is read at a unit's end.
+//   - A query is p0 + p1 / 16 + p2 / 256, each part the e4m3 rounding of what the ones before left, times 16: within 2^-12
+//     of it, or 2^-18 absolute (of 448, the row's largest).
+//   - A weight is rounded to fp16 and then is p0 + p1 / 8 + p2 / 64 + p3 / 512 exactly: e5m2 is fp16's upper byte, so a
+//     part is cut off, not rounded, and takes three bits. With the largest at 2^13 or more, all of fp16's 11 bits are there
+//     down to 2^-27 of the largest, and one bit down to 2^-37. (Three e4m3 parts, rounded, held 2^-24 of it and nothing
+//     below: 16384 keys of 2^-20 beside one lost 0.4 %. 32 x 4096 keys: group 8 48.6 us a layer with either, group 16
+//     63.4 with three parts, 65.3 with four, 66.8 with four that are rounded.)
 //   - A query row is rotated in fp32 and scaled by a power of two to at most 448 before it is split.
 //   - Thread t of the softmax owns key t of the tile: its scales are its own numbers. The exponent of V's scale
-//     joins the score, x = s + log2 vs, so the weight that multiplies the codes is 2^(x - m), and no
-//     scale can push it out of range; the sum l takes 2^(x - m) / vs, the weight of the value itself.
-//   - m moves only when a weight would exceed 2^8.75 (448 is the largest e4m3), to leave the largest at 2^6: O in
+//     joins the score, x = s + log2 vs, so the weight that multiplies the codes is 2^(x - m), and no scale can push it out
+//     of range (the bits that it keeps count from the largest weight times scale); the sum l takes 2^(x - m) / vs, the
+//     weight of the value itself.
+//   - m moves only when a weight would exceed 2^15.75 (e5m2 ends at 57344), to leave the largest at 2^13: O in
 //     tensor memory is scaled rarely, and four warps agree on it with one barrier a tile.
 //
 // Measured: 32 x 4096 keys, 8 kv heads 51.8 us (5.2 TB/s; 6.4 in the loop, the rest is the start: lengths, queries, first
@@ -25,7 +31,7 @@
 //
 // 224 threads: warps 0..3 softmax (TMEM lane t = key t, then dim t), warps 4 and 6 fetch K and V, warp 5 issues the
 // products.
-// TMEM: two S tiles and O, 3 * COLS columns each (24 or 48, in strides of 32 or 64).
+// TMEM: two S tiles of 3 * COLS columns and O of 4 * COLS, in strides of 32 or 64.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -40,18 +46,19 @@ namespace pg {
 
 constexpr int kTcThreads = kCompute + 96;
 constexpr int kTcD = 128, kTcKeys = 128;
-constexpr float kWeightTop = 6.f, kWeightMost = 8.75f;  // log2 of the largest weight after a move of m, and at most
+constexpr float kWeightTop = 13.f, kWeightMost = 15.75f;  // log2 of the largest weight after a move of m, and at most
 constexpr float kNoMax = -1e30f;                         // m before a row has seen a key
 
 template <int NB>
 struct TcCfg {
     using TL = Tile<kTcKeys, kTcD>;
     static constexpr int COLS = 8 * NB;
-    static constexpr int N = NB == 1 ? 32 : 48;         // rows of a B operand: 3 * COLS, a multiple of 16
+    static constexpr int N = NB == 1 ? 32 : 48;         // rows of query parts: 3 * COLS, a multiple of 16
+    static constexpr int NO = 4 * COLS;                 // rows of weight parts
     static constexpr int STRIDE = NB == 1 ? 32 : 64;    // TMEM columns of one accumulator
     static constexpr int TMEM = NB == 1 ? 128 : 256;
     static constexpr int QB = N * 128;                  // bytes of the query parts
-    static constexpr int PW = NB == 1 ? 32 : 64;        // bytes of a key's weight parts (the swizzle's width)
+    static constexpr int PW = NO;                       // bytes of a key's weight parts (the swizzle's width)
     static constexpr int PB = kTcKeys * PW;             // bytes of a weight buffer
     // shared memory behind the stages
     static constexpr int kP = QB, kSmall = QB + 2 * PB;  // queries, two weight buffers, the rest
@@ -74,8 +81,13 @@ __device__ __forceinline__ float redux_max(float x) {
     return y;
 }
 
-__device__ __forceinline__ float of_parts(uint32_t a, uint32_t b, uint32_t c) {
+__device__ __forceinline__ float of_query_parts(uint32_t a, uint32_t b, uint32_t c) {
     return fmaf(__uint_as_float(c), 1.f / 256.f, fmaf(__uint_as_float(b), 1.f / 16.f, __uint_as_float(a)));
+}
+
+__device__ __forceinline__ float of_weight_parts(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return fmaf(__uint_as_float(d), 1.f / 512.f,
+                fmaf(__uint_as_float(c), 1.f / 64.f, fmaf(__uint_as_float(b), 1.f / 8.f, __uint_as_float(a))));
 }
 
 // Whether any of the computing threads says so (all of them take part).
@@ -183,7 +195,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 return false;
             };
             constexpr uint32_t id_s = tc::idesc_e4m3_f32(128, C::N, 0, 0);
-            constexpr uint32_t id_o = tc::idesc_e4m3_f32(128, C::N, 1, 1);
+            constexpr uint32_t id_o = tc::idesc_e4m3_f32(128, C::NO, 1, 1, 1);
             const uint64_t qd = tc::smem_desc_sw128(smem_u32(q_sm), 16, 1024);
             const uint64_t kd0 = tc::smem_desc_sw128(smem_u32(sm), 16, 1024);
             const uint64_t vd0 = tc::smem_desc_sw128(smem_u32(sm) + TL::BYTES, TL::BYTES, 1024);
@@ -372,7 +384,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 if (lane == 0) mbar_arrive(&bar->s_free[it & 1]);
 #pragma unroll
                 for (int c = 0; c < COLS; ++c) {
-                    const float sum = of_parts(a[c], a[COLS + c], a[2 * COLS + c]);
+                    const float sum = of_query_parts(a[c], a[COLS + c], a[2 * COLS + c]);
                     x[c] = fmaf(sum * ks, qf[c], lv);
                 }
             }
@@ -413,7 +425,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                     wait(&bar->p_free[(it - 1) & 1], (it - 1) >> 1);
                     tc::fence_after_sync();
 #pragma unroll
-                    for (int part = 0; part < 3; ++part)
+                    for (int part = 0; part < 4; ++part)
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
                             uint32_t o[8];
@@ -429,7 +441,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
             }
             fresh = false;
             // ---- weights, their sum, and their parts (of the weight in fp16): bytes part * COLS + c of this key
-            uint32_t w[3 * COLS / 4];
+            uint32_t w[COLS];
 #pragma unroll
             for (int c = 0; c < COLS; c += 4) {
                 float u[4];
@@ -440,10 +452,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 }
                 uint32_t h0 = pack_half2(u[0], u[1]), h1 = pack_half2(u[2], u[3]);
 #pragma unroll
-                for (int part = 0; part < 3; ++part) {
-                    const uint32_t v0 = e4m3x2_of_half2(h0), v1 = e4m3x2_of_half2(h1);
-                    w[(part * COLS + c) / 4] = v0 | (v1 << 16);
-                    if (part < 2) h0 = half2_rest16(h0, half2_of_e4m3x2(v0)), h1 = half2_rest16(h1, half2_of_e4m3x2(v1));
+                for (int part = 0; part < 4; ++part) {
+                    w[(part * COLS + c) / 4] = e5m2x4_of_half4(h0, h1);
+                    if (part < 3) h0 = half2_rest8(h0), h1 = half2_rest8(h1);
                 }
             }
             if (it >= 2) wait(&bar->p_free[it & 1], (it >> 1) - 1);
@@ -452,11 +463,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 const uint32_t row = smem_u32(p_sm + (it & 1) * C::PB) + tid * C::PW;
                 const int sw = NB == 1 ? (tid >> 2) & 1 : (tid >> 1) & 3;
 #pragma unroll
-                for (int ch = 0; ch < 3 * NB / 2; ++ch)
+                for (int ch = 0; ch < 2 * NB; ++ch)
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + (ch ^ sw) * 16), "r"(w[4 * ch]),
                                  "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3]) : "memory");
-                if constexpr (NB == 1)
-                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(row + (1 ^ sw) * 16), "r"(w[4]), "r"(w[5]) : "memory");
             }
             fence_proxy_async_smem();
             tc::fence_before_sync();
@@ -478,21 +487,25 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
                 const size_t part = part_slot(blockIdx.x, first_tile == 0);
                 wait(&bar->p_free[it & 1], it >> 1);
                 tc::fence_after_sync();
-                uint32_t a[C::N];
-                tc::ld32(tc::taddr(tmem_o, lane_row, 0), *reinterpret_cast<uint32_t(*)[32]>(a));
-                if constexpr (C::N == 48) tc::ld16(tc::taddr(tmem_o, lane_row, 32), *reinterpret_cast<uint32_t(*)[16]>(a + 32));
-                tc::wait_ld();
 #pragma unroll
-                for (int c = 0; c < COLS; ++c) {
-                    if (c >= rows) continue;
-                    const float sum = (l_sm[c] + l_sm[COLS + c]) + (l_sm[2 * COLS + c] + l_sm[3 * COLS + c]);
-                    const float o = of_parts(a[c], a[COLS + c], a[2 * COLS + c]);
-                    const float y = sum == 0.f ? 0.f : o / sum;  // no key; a NaN stays one
-                    if (whole) {
-                        out_row(p, at, r0, c)[tid] = __float2half_rn(y);
-                    } else {
-                        tp.part_o[(part * kMaxCols + c) * D + tid] = y;
-                        if (tid == 0) tp.part_lse[part * kMaxCols + c] = sum > 0.f ? mm[c] + __log2f(sum) : -INFINITY;
+                for (int nb = 0; nb < NB; ++nb) {
+                    uint32_t a[4][8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tc::ld8(tc::taddr(tmem_o, lane_row, i * COLS + 8 * nb), a[i]);
+                    tc::wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int c = 8 * nb + k;
+                        if (c >= rows) continue;
+                        const float sum = (l_sm[c] + l_sm[COLS + c]) + (l_sm[2 * COLS + c] + l_sm[3 * COLS + c]);
+                        const float o = of_weight_parts(a[0][k], a[1][k], a[2][k], a[3][k]);
+                        const float y = sum == 0.f ? 0.f : o / sum;  // no key; a NaN stays one
+                        if (whole) {
+                            out_row(p, at, r0, c)[tid] = __float2half_rn(y);
+                        } else {
+                            tp.part_o[(part * kMaxCols + c) * D + tid] = y;
+                            if (tid == 0) tp.part_lse[part * kMaxCols + c] = sum > 0.f ? mm[c] + __log2f(sum) : -INFINITY;
+                        }
                     }
                 }
                 if (!whole) join_parts<D>(tp, at, r0, rows, ctas.x, ctas.y, misc + 1);

@@ -56,9 +56,9 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N, int a_mn, int
            ((uint32_t)(M >> 4) << 24);
 }
 
-// The same fields for tcgen05.mma.kind::f8f6f4 with e4m3 A and B (format 0 of both) and an fp32 accumulator.
-__host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N, int a_mn, int b_mn) {
-    return idesc_f16_f32(M, N, a_mn, b_mn);
+// The same fields for tcgen05.mma.kind::f8f6f4 with e4m3 A, e4m3 (format 0) or e5m2 (1) B and an fp32 accumulator.
+__host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N, int a_mn, int b_mn, int b_e5m2 = 0) {
+    return idesc_f16_f32(M, N, a_mn, b_mn) | ((uint32_t)b_e5m2 << 10);
 }
 
 // ------------------------------------------------------------ TMEM management

@@ -161,7 +161,7 @@ def test_long_chunk_appends_to_a_page_of_a_scale_past_fp16(av):
 
 # ---------------------------------------------------------------- weights far below the largest
 
-@pytest.mark.parametrize("D,e4m3", [(64, False), (128, False), (256, False), (64, True), (256, True)])
+@pytest.mark.parametrize("D,e4m3", [(64, False), (128, False), (256, False), (64, True), (256, True), (128, True)])
 def test_decode_many_keys_far_below_one(av, D, e4m3):
     """One key of value 0 takes nearly all of every row, and what 16384 others of value 1 share (e^-gap each) is the
     result. They all lie behind it in one CTA's stretch: 600 sequences name the same pages, two units a CTA.
@@ -188,6 +188,36 @@ def test_decode_many_keys_far_below_one(av, D, e4m3):
         tol = want * (2.0 ** -10 + 2 * T * 2.0 ** -24) + 2.0 ** -25
         worst = float((out.double() - want).abs().max())
         assert worst <= tol, f"gap {gap}: {worst / want:.3g} of the result lost"
+
+
+@pytest.mark.parametrize("D", [128, 64, 256])
+@pytest.mark.parametrize("group", [2, 16])
+def test_decode_values_of_uneven_scales(av, D, group):
+    """Pages whose V scales differ by 2^20, the large ones empty in half of the dims: there the small pages alone are the
+    result, and they lose nothing to the large ones' weights.
+
+    Tolerance: as in paged_helpers.check_attention, without a term that is relative to the largest weight."""
+    if D == 256 and group == 16:
+        group = 8
+    T = [200, 333]
+    c = H.make_cache(T, [0, 0], 1, D, 16, True, seed=441)
+    c["new"] = [1, 1]
+    c["v_scales"][:] = 127 - 12
+    large = torch.arange(c["v"].shape[0]) % 2 == 0
+    c["v_scales"][large] = 127 + 8
+    codes = c["v"].view(torch.uint8)
+    codes[large, :, :, D // 2:] = 0
+    t = new_tokens(c, group, seed=442)
+    d, out, q_rot, err = run_decode(av, c, t, append=False, scale=0.02)
+    assert err == 0
+    for b in range(2):
+        k, v = P.keys_values(c["k"], c["v"], c["k_scales"], c["v_scales"], c["table"][b], T[b], 0)
+        for h in range(group):
+            o, w, s, _ = P.attention(t["q"][b, h].double(), k, v, 0.02)
+            eps = 2 * s * (2.0 ** -12 + 2.0 ** -16 + 2.0 ** -20)
+            tol = w * (eps + 2.0 ** -11 + 2.0 ** -19 + 2 * T[b] * 2.0 ** -24) + o.abs() * 2.0 ** -11 + 2.0 ** -25
+            worst = ((out[b, h].double() - o).abs() / tol)[D // 2:].max()
+            assert worst <= 1, f"sequence {b}, row {h}: {float(worst):.3g} times the tolerance"
 
 
 @pytest.mark.parametrize("D", [128, 64])
