@@ -9,6 +9,7 @@
 //
 // Measured: 16 prompts of 256 to 4096 tokens, 32 q and 32 kv heads, 331 us (5.0 TB/s of what must move); 256 sequences
 // of one token, 64 q and 8 kv heads, 7.0 us; one sequence 2.4 us in a graph.
+#include <initializer_list>
 #include <mutex>
 
 #include "paged.cuh"
@@ -151,7 +152,9 @@ __global__ void __launch_bounds__(kTokenThreads) paged_append_token_kernel(const
 // before they round.
 constexpr int kRowsThreads = 256;
 
-template <int D, bool E4M3>
+// LONG: for a long chunk's attention, which takes halved queries and the new rows expanded to fp16 as well.
+// STRIDE: a CTA also takes every gridDim.x-th page behind its first (16 prompts: 370 us, 342 without the loop).
+template <int D, bool E4M3, bool LONG, bool STRIDE>
 __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(const __grid_constant__ Params p,
                                                                          const __grid_constant__ Freqs f) {
     constexpr int R = 2048 / D;      // rows per warp
@@ -168,14 +171,13 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int b = blockIdx.y;
     const Seq s = seq_of(p, b);
-    const int64_t first = ((int64_t)(s.T >> p.page_log2) + blockIdx.x) << p.page_log2;
     // a long chunk's plan has given rows to every sequence that is served
-    const bool served = !p.exp_k || (s.ok && p.cu_kv[b + 1] - p.cu_kv[b] == s.T + s.n);
-    const bool here = s.ok && served && s.n > 0 && first < (int64_t)s.T + s.n;
-    const int p0 = here ? (int)first : 0;  // first position of the page
-    if (!s.ok) {
-        if (blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
-    } else if (here) {
+    const bool served = s.ok && s.n > 0 && (!LONG || p.cu_kv[b + 1] - p.cu_kv[b] == s.T + s.n);
+    if (!s.ok && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) set_error(p, FCCI_DEV_ERR_CAPACITY);
+    // (a sequence that is not served may have any length, a negative one too: no page of it is looked at)
+    const int pages = served ? (s.T + s.n - 1 >> p.page_log2) + 1 : 0;
+    for (int page_i = served ? (s.T >> p.page_log2) + (int)blockIdx.x : 0; page_i < pages; page_i += gridDim.x) {
+        const int p0 = page_i << p.page_log2;  // first position of the page
         const int half = p.rot >> 1;
         for (int i = tid; i < p.page * half; i += kRowsThreads) {
             const int r = i / half, k = i - r * half;
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
         const int per = (heads + gridDim.z - 1) / gridDim.z;
         const int h_end = min(heads, (int)(blockIdx.z + 1) * per);
         // a long chunk's attention reads fp16 rows: write these while they are here
-        const int64_t exp_row = p.exp_k ? p.cu_kv[b] : -1;
+        const int64_t exp_row = LONG ? p.cu_kv[b] : 0;
         // passes whose row is new, and those whose row the page held before
         uint32_t is_new = 0, is_old = 0;
 #pragma unroll
@@ -272,10 +274,10 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     if (E4M3) amax = fmaxf(fmaxf(amax, fmaxf(fabsf(u.x), fabsf(u.y))), fmaxf(fabsf(w.x), fabsf(w.y)));
                 }
             }
-            auto store16 = [&](__half* row, int i, float factor) {
-                const float2 f2 = make_float2(factor, factor);
+            auto store16 = [&](__half* row, int i) {
+                const float factor = E4M3 || is_q ? kLongQuery : 1.f;  // (e4m3: queries alone come here)
                 auto two = [&](float2 v) {
-                    v = __fmul2_rn(v, f2);
+                    if (LONG) v = __fmul2_rn(v, make_float2(factor, factor));
                     return pack_half2(v.x, v.y);
                 };
                 *reinterpret_cast<uint4*>(row + dlo) = make_uint4(two(x[i][0]), two(x[i][1]), two(x[i][2]), two(x[i][3]));
@@ -300,6 +302,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     ex = max(ex, had);
                     const float up = rescale(0, ex), down = grows ? rescale(had, ex) : 1.f;
                     const float2 up2 = make_float2(up, up);
+                    const int xe = is_k ? ex + kLongKeyExp : ex;
+                    const __half2 s2 = LONG ? expansion_scale(p, ex, xe) : __half2();
+                    const bool clamp = xe >= kScaleMax;
                     auto four = [&](float2 u, float2 w) {
                         u = __fmul2_rn(u, up2), w = __fmul2_rn(w, up2);
                         return e4m3x2(u.x, u.y) | (e4m3x2(w.x, w.y) << 16);
@@ -313,12 +318,10 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                             const uint2 w = make_uint2(four(x[i][4], x[i][5]), four(x[i][6], x[i][7]));
                             *reinterpret_cast<uint2*>(row + dlo) = u;
                             *reinterpret_cast<uint2*>(row + dhi) = w;
-                            if (exp_row >= 0) {
+                            if (LONG) {
                                 __half* er = (is_v ? p.exp_v : p.exp_k) + h * p.exp_sh + (exp_row + pos) * D;
-                                const int xe = is_k ? ex + kLongKeyExp : ex;
-                                const __half2 s2 = expansion_scale(p, ex, xe);
-                                *reinterpret_cast<uint4*>(er + dlo) = expanded(u, s2, xe >= kScaleMax);
-                                *reinterpret_cast<uint4*>(er + dhi) = expanded(w, s2, xe >= kScaleMax);
+                                *reinterpret_cast<uint4*>(er + dlo) = expanded(u, s2, clamp);
+                                *reinterpret_cast<uint4*>(er + dhi) = expanded(w, s2, clamp);
                             }
                         } else if (grows && (is_old >> i & 1)) {
                             for (int k = 0; k < 4; ++k) {
@@ -341,49 +344,61 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     const int pos = p0 + row0 + i * RP;
                     __half* row = is_q ? p.q_rot + ((src_row + i * RP) * p.Hq + h) * D
                                        : reinterpret_cast<__half*>(page + (row0 + i * RP) * st);
-                    store16(row, i, is_q && p.exp_k ? kLongQuery : 1.f);
-                    if (!is_q && exp_row >= 0)
-                        store16((is_v ? p.exp_v : p.exp_k) + h * p.exp_sh + (exp_row + pos) * D, i, 1.f);
+                    store16(row, i);
+                    if (LONG && !is_q)
+                        store16((is_v ? p.exp_v : p.exp_k) + h * p.exp_sh + (exp_row + pos) * D, i);
                 }
             }
         }
+        if constexpr (!STRIDE) break;
+        __syncthreads();  // the angles of this page have been read
     }
     advance_lengths(p, &flag);
 }
 
-template <int D, bool E4M3>
+template <int D, bool E4M3, bool LONG = false>
 static int launch_append_t(const Params& p, const Freqs& f, cudaStream_t st) {
     const int heads = (p.q ? p.Hq : 0) + 2 * p.Hkv;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
+    if (dev < 0 || dev >= 128) return set_status(FCCI_EINVAL, "device index");
+    const int sms = device_sm_count(dev);
     if (!p.cu_q) {
         // one row a warp while that fits the GPU at once (4 CTAs an SM), else as many as it takes, up to four
         int tasks = 1;
-        while (tasks < kTokenTasks && (int64_t)p.B * ((heads + tasks * kTokenWarps - 1) / (tasks * kTokenWarps)) > 4 * 148) ++tasks;
+        while (tasks < kTokenTasks && (int64_t)p.B * ((heads + tasks * kTokenWarps - 1) / (tasks * kTokenWarps)) > 4 * sms) ++tasks;
         const int y = (heads + tasks * kTokenWarps - 1) / (tasks * kTokenWarps);
         return launch_pdl(paged_append_token_kernel<D, E4M3>, dim3(p.B, y), dim3(kTokenThreads), 0, st, p, f, tasks);
     }
     // pages that the longest run of new tokens can touch, and a head split that fills the GPU
     // when there are few pages
-    const int64_t slots = ((int64_t)p.max_q + p.page - 2) / p.page + 1;
+    int64_t slots = ((int64_t)(p.max_q < p.total_q ? p.max_q : p.total_q) + p.page - 2) / p.page + 1;
     const int64_t pages = (int64_t)p.total_q / p.page + p.B;
-    int64_t z = (8 * 148 + pages - 1) / pages;
+    int64_t z = (8 * sms + pages - 1) / pages;
     const int64_t most = (heads + 7) / 8;
     if (z > most) z = most;
     if (z < 1) z = 1;
+    // max_q is a bound on any sequence, total_q on all: where their product is far above the pages that there can be, the
+    // CTAs of a sequence take several pages each
+    const int64_t ctas = 16 * pages * z > 65536 ? 16 * pages * z : 65536;
+    const bool stride = slots > ctas / (p.B * z);
+    if (stride) slots = ctas / (p.B * z) > 1 ? ctas / (p.B * z) : 1;
+    const auto kernel = stride ? paged_append_rows_kernel<D, E4M3, LONG, true> : paged_append_rows_kernel<D, E4M3, LONG, false>;
     const size_t smem = (size_t)p.page * (p.rot / 2) * sizeof(float2);
     static std::once_flag once[128];
     static cudaError_t attr[128];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return set_cuda_status(cudaGetLastError());
     std::call_once(once[dev], [&]() {
-        attr[dev] = cudaFuncSetAttribute(paged_append_rows_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         64 * 1024);
+        for (auto k : {paged_append_rows_kernel<D, E4M3, LONG, false>, paged_append_rows_kernel<D, E4M3, LONG, true>}) {
+            attr[dev] = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
+            if (attr[dev] != cudaSuccess) return;
+        }
     });
     if (attr[dev] != cudaSuccess) return set_cuda_status(attr[dev]);
-    return launch_pdl(paged_append_rows_kernel<D, E4M3>, dim3((unsigned)slots, p.B, (unsigned)z), dim3(kRowsThreads), smem,
-                      st, p, f);
+    return launch_pdl(kernel, dim3((unsigned)slots, p.B, (unsigned)z), dim3(kRowsThreads), smem, st, p, f);
 }
 
 int launch_append(const Params& p, const Freqs& f, bool e4m3, cudaStream_t st) {
+    if (p.exp_k) return e4m3 ? launch_append_t<128, true, true>(p, f, st) : launch_append_t<128, false, true>(p, f, st);
     switch (p.D) {
         case 64: return e4m3 ? launch_append_t<64, true>(p, f, st) : launch_append_t<64, false>(p, f, st);
         case 128: return e4m3 ? launch_append_t<128, true>(p, f, st) : launch_append_t<128, false>(p, f, st);

@@ -299,3 +299,82 @@ def test_lengths_past_what_a_line_holds(av, D, e4m3):
     torch.cuda.synchronize()
     assert av.paged_read_error(ws) == CAPACITY
     assert lens.tolist() == [1 << 29] * B and (out == 7.0).all() and torch.equal(pool, before)
+
+
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_append_to_lengths_that_are_none(av, e4m3):
+    """Negative lengths and ones past the table, ragged rows: reported, nothing of theirs is written."""
+    T, new = [20, 17, 40, 0], [5, 70, 3, 33]
+    c = H.make_cache(T, new, 2, 128, 16, e4m3, seed=433)
+    t = new_tokens(c, 2, seed=434)
+    room = c["table"].shape[1] * 16
+    for bad in (-1, -5, -100, -2 ** 31, room - 69, 2 ** 31 - 1):
+        cc = dict(c, T=torch.tensor([20, bad, 40, 0], dtype=torch.int32))
+        d, q_rot, err = run_append(av, cc, t, True, advance=True)
+        assert err == CAPACITY and d["T"].cpu().tolist() == [25, bad, 43, 33]
+        after = H.back(d)
+        mine = c["table"][1][c["table"][1] >= 0].long()
+        for name in "kv":
+            assert torch.equal(H.bits(after[name])[mine], H.bits(c[name])[mine])
+        assert (q_rot[5:75] == 7.0).all()
+
+
+# ---------------------------------------------------------------- bounds far above what a call holds
+
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_append_under_a_bound_of_any_size(av, e4m3):
+    """max_seqlen_q is a bound: what a call holds decides its work, whatever the bound says."""
+    T, new = [5, 0, 63, 1000], [40, 1, 0, 130]
+    c = H.make_cache(T, new, 2, 128, 16, e4m3, seed=431)
+    t = new_tokens(c, 4, seed=432)
+    seen = []
+    for bound in (130, 1 << 20, 2 ** 31 - 1):
+        d = H.to_device(c)
+        q_rot = torch.full_like(t["q"], 7.0).to(DEV)
+        av.paged_append(t["k"].to(DEV), t["v"].to(DEV), d["k"], d["v"], d["table"], d["T"], k_scales=d["k_scales"],
+                        v_scales=d["v_scales"], q=t["q"].to(DEV), q_rot_out=q_rot, cu_seqlens_q=t["cu"].to(DEV), max_seqlen_q=bound)
+        torch.cuda.synchronize()
+        check_whole_append(c, t, d, q_rot.cpu(), 128)
+        seen.append((H.bits(H.back(d)["k"]), H.bits(H.back(d)["v"])))
+    for a, b in seen[1:]:
+        assert torch.equal(a, seen[0][0]) and torch.equal(b, seen[0][1])
+
+
+@pytest.mark.parametrize("how,e4m3,D", [("append", False, 64), ("append", True, 128), ("append", True, 256),
+                                        ("prefill", False, 128), ("prefill", True, 128)])
+def test_append_of_many_pages_by_few_blocks(av, how, e4m3, D):
+    """One long run of tokens beside thousands of short ones, under a bound that any could reach: every page of each is
+    written. (The values are exact in e4m3 at any scale of theirs.)"""
+    B = 3000
+    T = [(7 * b) % 33 for b in range(B)]
+    new = [1 + b % 3 for b in range(B)]
+    new[1234] = 5000
+    page = 16
+    cu = torch.tensor([0] + new, dtype=torch.int64).cumsum(0).to(torch.int32)
+    need = torch.tensor([-(-(a + n) // page) for a, n in zip(T, new)])
+    table = torch.full((B, int(need.max())), -1, dtype=torch.int32)
+    at = 0
+    for b in range(B):
+        table[b, : need[b]] = torch.arange(at, at + int(need[b]), dtype=torch.int32)
+        at += int(need[b])
+    kind = H.F8 if e4m3 else torch.float16
+    pools = [torch.zeros(at, 1, page, D, dtype=torch.float16, device=DEV).to(kind) for _ in range(2)]
+    scales = [torch.full((at, 1), 112, dtype=torch.uint8, device=DEV).view(H.E8) if e4m3 else None for _ in range(2)]
+    n = int(cu[-1])
+    v = ((torch.arange(n * D) * 5 // 3) % 8 + 8).view(n, 1, D).half().to(DEV)
+    lens = torch.tensor(T, dtype=torch.int32, device=DEV)
+    kw = dict(k_scales=scales[0], v_scales=scales[1], rotary_dim=0, advance=True)
+    if how == "append":
+        av.paged_append(v, v, *pools, table.to(DEV), lens, cu_seqlens_q=cu.to(DEV), max_seqlen_q=1 << 30, **kw)
+    else:
+        out = torch.zeros_like(v)
+        av.paged_prefill(v, v, v, *pools, out, table.to(DEV), lens, cu.to(DEV), 1 << 30, max_kv_tokens=n + sum(T), **kw)
+        assert out.isfinite().all() and (out >= 0).all() and (out <= 15).all() and (out[cu[:-1].long()][:1] > 0).all()
+    assert lens.tolist() == [a + b for a, b in zip(T, new)]
+    seq = torch.repeat_interleave(torch.arange(B), torch.tensor(new))
+    pos = torch.tensor(T)[seq] + torch.arange(n) - cu[:-1].long()[seq]
+    page_of = table[seq, pos // page].long()
+    for x, s in zip(pools, scales):
+        x = x.float().cpu() * (s.float().cpu()[:, :, None, None] if e4m3 else 1.0)
+        assert torch.equal(x[page_of, 0, pos % page], v.float().cpu()[:, 0])
+        assert int((x != 0).sum()) == n * D
