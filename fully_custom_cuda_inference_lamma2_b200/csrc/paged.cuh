@@ -9,6 +9,10 @@
 #include "fcci_paged.h"
 #include "ptx.cuh"
 
+// The append and the split attention let the next kernel start (griddep_launch_dependents) only after their own wait, unless
+// they read early: the next one may read lengths and rows before its wait, and must not do so while a kernel before
+// this one, a step that moves the lengths for instance, is still running. (A token append in a chain takes 2.44 us
+// instead of 2.37, a decode step over 512 keys 11.2 instead of 11.0.)
 namespace fcci {
 namespace pg {
 

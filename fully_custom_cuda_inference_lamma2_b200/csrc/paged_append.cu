@@ -35,8 +35,8 @@ __global__ void __launch_bounds__(kTokenThreads) paged_append_token_kernel(const
     __shared__ float2 cs[D / 2];
     const int half = p.rot >> 1;
     const uint64_t turn = threadIdx.x < half ? f.turn[threadIdx.x] : 0;  // a launch constant: read before the wait
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();  // behind the wait (paged.cuh)
     const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nkv = 2 * p.Hkv, all = nkv + (p.q ? p.Hq : 0);
     const int d0 = lane * E;
@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
     extern __shared__ float4 cs_table[];
     __shared__ int flag;
     __shared__ float amax_sm[2][kWarps];
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();  // behind the wait (paged.cuh)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int b = blockIdx.y;
     const Seq s = seq_of(p, b);

@@ -100,8 +100,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
         prefetch_tmap(&mv16);
     }
     __syncthreads();
-    griddep_launch_dependents();
     if (!sp.early) griddep_wait();
+    griddep_launch_dependents();  // behind the wait (paged.cuh)
 
     At at = line.template build<kThreads>(reinterpret_cast<int*>(red_ml));
     const int ntiles = line.ntiles;

@@ -164,8 +164,8 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    griddep_launch_dependents();
     if (!tp.early) griddep_wait();
+    griddep_launch_dependents();  // behind the wait (paged.cuh)
     At at = line.template build<kTcThreads>(reinterpret_cast<int*>(mx_sm));
     const uint32_t tmem = *tmem_slot;
     const uint32_t tmem_o = tmem + 2 * C::STRIDE;

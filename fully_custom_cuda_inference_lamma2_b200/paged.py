@@ -124,7 +124,8 @@ def paged_decode(cache: PagedKVCache, layer: int, q: torch.Tensor, out: torch.Te
 
     prefetch_kv: read the lengths, the page table and the cached rows before waiting for the previous kernel on the
     stream (FCCI_PAGED_PREFETCH_KV). Only when no kernel that may still be running writes them, e.g. right after the
-    projection that produced q/k_new/v_new, or after another layer's step that does not advance."""
+    projection that produced q/k_new/v_new, or in a chain of layers' steps whose first has it not set and of which only
+    the last advances."""
     k, v, ks, vs = cache.layer(layer)
     attn_varlen.paged_decode(q, k, v, out, cache.page_table, cache.seq_lens, k_scales=ks, v_scales=vs, k_new=k_new,
                              v_new=v_new, scale=-1.0 if scale is None else float(scale), rope_theta=rope_theta,

@@ -124,8 +124,10 @@ typedef struct fcci_paged_desc {
 
 /* Decode: read seq_lens, the page table, scales and the cached rows below T_b before the programmatic-launch wait, so
  * that they overlap the kernel before it on the stream; q, k_new and v_new are still read after it. Set it only when no
- * kernel that can still be running when this one starts writes any of those: for example a decode step right after the
- * projection that produced q/k/v, or after another layer's decode step that does not advance. */
+ * kernel that can still be running when this one starts writes any of those. Those are the kernel before it and, where that
+ * one was launched with this flag too, the ones before that, back to the last ordinary launch or paged call
+ * without the flag: everything before that one has ended. So it may be set for example right after the projection that
+ * produced q/k/v, or in a chain of layers' steps of which only the last advances and the first has not the flag. */
 #define FCCI_PAGED_PREFETCH_KV 1u
 
 int fcci_paged_append(const fcci_paged_desc* desc, cudaStream_t stream);
