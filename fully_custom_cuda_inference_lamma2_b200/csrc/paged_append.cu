@@ -295,6 +295,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_append_rows_kernel(cons
                     if (lane == 0) amax_sm[buf][warp] = amax;
                     named_bar_sync(1 + grp, 32 * W);
                     for (int w = 0; w < W; ++w) amax = fmaxf(amax, amax_sm[buf][grp * W + w]);
+                } else {
+                    __syncwarp();  // every lane has read the old scale
                 }
                 if (work && !is_q) {
                     int ex = scale_exponent(amax);
