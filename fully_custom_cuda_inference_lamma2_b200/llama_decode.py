@@ -206,20 +206,40 @@ class GreedyDecoder:
         self.generated.index_copy_(0, self._slot, self.token)
         self.step_idx.add_(1)
 
+    def _paged_tensors(self):
+        """What the pages of all layers hold, as bytes ([L, num_pages, ...]); nothing of an arena."""
+        if not isinstance(self.arena, PagedKVCache):
+            return []
+        c = self.arena
+        return [t.view(torch.uint8) for t in (c.k, c.v, c.k_scales, c.v_scales) if t is not None]
+
+    def _page_of_next_row(self) -> Optional[int]:
+        """The page that the next token's row goes to, if the cache has one (reads T on the host)."""
+        if not isinstance(self.arena, PagedKVCache):
+            return None
+        at, pages = int(self.arena.seq_lens[0]) // self.arena.page_size, self.arena.pages_of(0)
+        return pages[at] if 0 <= at < len(pages) else None
+
     def capture(self, warmup: int = 0):
         """Capture one token step into a CUDA graph (the arena's seq_len is read on the device, so
-        the graph is valid for every length). The caller's state (T, token) is restored."""
+        the graph is valid for every length). The caller's state (T, token, what the cache holds) is restored."""
         saved_T = self.arena.seq_lens.clone()
         saved_tok, saved_idx = self.token.clone(), self.step_idx.clone()
+        page = self._page_of_next_row()
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
+            held = [t[:, page].clone() for t in self._paged_tensors()] if page is not None else []
             for _ in range(max(1, warmup)):  # first launches set kernel attributes outside the capture
                 self._step()
+                # each warm-up step writes the one row T, behind the sequence's end
+                self.arena.seq_lens.copy_(saved_T)
+                self.token.copy_(saved_tok)
+                self.step_idx.copy_(saved_idx)
+            # ... but an e4m3 page takes that row's scale if it is larger, for the rows before it too
+            for t, was in zip(self._paged_tensors(), held):
+                t[:, page] = was
         torch.cuda.current_stream().wait_stream(side)
-        self.arena.seq_lens.copy_(saved_T)
-        self.token.copy_(saved_tok)
-        self.step_idx.copy_(saved_idx)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=side):
             self._step()
