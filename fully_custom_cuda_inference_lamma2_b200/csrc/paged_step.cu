@@ -5,6 +5,10 @@
 #include <stdint.h>
 #include <string.h>
 
+#include <algorithm>
+#include <initializer_list>
+#include <utility>
+
 #include "paged.cuh"
 
 namespace fcci {
@@ -33,6 +37,22 @@ WsLayout ws_layout(int B, int Hq, int Hkv, int D, int total_q, int max_q, int ma
 enum class Op { kAppend, kDecode, kPrefill };
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Whether blocks of `inner` elements, one for each index of all dimensions (extent, stride), may share elements: not when each
+// stride, in rising order, reaches past all that the smaller ones span.
+static bool overlapping(int64_t inner, std::initializer_list<std::pair<int64_t, int64_t>> dims) {
+    std::pair<int64_t, int64_t> d[4];
+    int n = 0;
+    for (const auto& x : dims)
+        if (x.first > 1) d[n++] = {x.second, x.first};
+    std::sort(d, d + n);
+    __int128 span = inner;
+    for (int i = 0; i < n; ++i) {
+        if (d[i].first < span) return true;
+        span += (__int128)(d[i].second - 1) * d[i].first;
+    }
+    return false;
+}
 
 // Validates a descriptor; on failure records the reason and returns its FCCI_E* code.
 static int fill(const fcci_paged_desc* d, Op op, Params& p, Freqs& f, WsLayout& L) {
@@ -89,6 +109,17 @@ static int fill(const fcci_paged_desc* d, Op op, Params& p, Freqs& f, WsLayout& 
     if (d->k_stride_t < d->D || d->v_stride_t < d->D) return bad(FCCI_EINVAL, "the rows of a page overlap");
     if (d->k_scales_stride_p < 0 || d->k_scales_stride_h < 0 || d->v_scales_stride_p < 0 || d->v_scales_stride_h < 0)
         return bad(FCCI_EINVAL, "negative scale stride");
+    if (d->k_new) {  // rows are written
+        const int64_t n = d->num_pages, h = d->Hkv, ps = d->page_size;
+        if (overlapping(d->D, {{ps, d->k_stride_t}, {h, d->k_stride_h}, {n, d->k_stride_p}}) ||
+            overlapping(d->D, {{ps, d->v_stride_t}, {h, d->v_stride_h}, {n, d->v_stride_p}}))
+            return bad(FCCI_EINVAL, "pages, heads or rows of a pool that gets rows overlap");
+        if (e4m3 && (overlapping(1, {{h, d->k_scales_stride_h}, {n, d->k_scales_stride_p}}) ||
+                     overlapping(1, {{h, d->v_scales_stride_h}, {n, d->v_scales_stride_p}})))
+            return bad(FCCI_EINVAL, "scales of a pool that gets rows overlap");
+    }
+    if (op != Op::kAppend && overlapping(d->D, {{d->Hq, d->out_stride_h}, {d->total_q, d->out_stride_t}}))
+        return bad(FCCI_EINVAL, "rows of out overlap");
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
     const int sms = device_sm_count(dev);

@@ -47,7 +47,7 @@ extern "C" {
 
 /*
  * Shapes and layouts (fp16 unless stated; strides in elements; head_dim contiguous;
- * 16-byte aligned bases, strides multiples of 16 bytes):
+ * 16-byte aligned bases, strides multiples of 16 bytes; what a call writes may not overlap itself):
  *   new tokens   cu_seqlens_q == NULL: sequence b owns row b (total_q == B, one token each);
  *                else rows cu_seqlens_q[b] .. cu_seqlens_q[b+1]-1, n_b of them, at most
  *                max_seqlen_q; rows behind cu_seqlens_q[B] are neither read nor written.
