@@ -216,14 +216,15 @@ WsLayout ws_layout(int B, int Hq, int Hkv, int D, int total_q, int max_q, int ma
 
 int launch_append(const Params& p, const Freqs& f, bool e4m3, cudaStream_t st);
 // Split-KV attention; `fused`: the launch appends the one new row of each sequence itself.
-// early: FCCI_PAGED_PREFETCH_KV.
-int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, bool early, uint8_t* ws, const WsLayout& L,
-                 cudaStream_t st);
+// early: FCCI_PAGED_PREFETCH_KV. rows: what an append launched before it writes (or NULL), once every check has passed.
+int launch_split(const Params& p, const Freqs& f, const Params* rows, bool e4m3, bool fused, bool early, uint8_t* ws,
+                 const WsLayout& L, cudaStream_t st);
+int append_before(const Params* rows, const Freqs& f, bool e4m3, cudaStream_t st);
 int launch_prefill(const Params& p, const Freqs& f, bool e4m3, uint8_t* ws, const WsLayout& L, int max_kv, float scale_log2,
                    int advance, cudaStream_t st);
 struct TileParams;
 // The same on the 5th-generation tensor cores, for e4m3 pages of head_dim 128.
-int launch_split_tc(TileParams& tp, const Freqs& f, int sms, int dev, cudaStream_t st);
+int launch_split_tc(TileParams& tp, const Freqs& f, const Params* rows, int sms, int dev, cudaStream_t st);
 
 }  // namespace pg
 }  // namespace fcci

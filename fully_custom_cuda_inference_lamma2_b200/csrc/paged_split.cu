@@ -507,8 +507,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_split_kernel(const __grid_c
     if (line.N > 0) advance_lengths(p, misc + 2);  // no place on the line: no new token, or nothing is served
 }
 
+int append_before(const Params* rows, const Freqs& f, bool e4m3, cudaStream_t st) {
+    return rows ? launch_append(*rows, f, e4m3, st) : FCCI_OK;
+}
+
 template <int D, int NB, bool E4M3>
-static int launch_split_t(TileParams& sp, const Freqs& f, int sms, int dev, cudaStream_t st) {
+static int launch_split_t(TileParams& sp, const Freqs& f, const Params* rows, int sms, int dev, cudaStream_t st) {
     using C = Cfg<D, NB, E4M3>;
     const Params& p = sp.p;
     static std::once_flag once[128];
@@ -527,14 +531,15 @@ static int launch_split_t(TileParams& sp, const Freqs& f, int sms, int dev, cuda
     if (!stages) return set_status(FCCI_EUNSUPPORTED, "paged attention: batch too large for shared memory");
     sp.stages = stages;
     CUtensorMap m[4];
-    const int rc = encode_pages<typename C::TL, E4M3>(p, m);
+    int rc = encode_pages<typename C::TL, E4M3>(p, m);
+    if (!rc) rc = append_before(rows, f, E4M3, st);
     if (rc) return rc;
     const size_t smem = C::smem(stages, p.B, rope_rows, p.rot);
     return launch_pdl(paged_split_kernel<D, NB, E4M3>, dim3(sms * per_sm), dim3(kThreads), smem, st, m[0], m[1], m[2], m[3], sp, f);
 }
 
-int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, bool early, uint8_t* ws, const WsLayout& L,
-                 cudaStream_t st) {
+int launch_split(const Params& p, const Freqs& f, const Params* rows, bool e4m3, bool fused, bool early, uint8_t* ws,
+                 const WsLayout& L, cudaStream_t st) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_status(cudaGetLastError());
     const int sms = device_sm_count(dev);
@@ -548,17 +553,17 @@ int launch_split(const Params& p, const Freqs& f, bool e4m3, bool fused, bool ea
     sp.part_o = reinterpret_cast<float*>(ws + L.part_o);
     if (sms * kMaxCtasPerSm > kMaxGrid) return set_status(FCCI_EUNSUPPORTED, "paged attention: too many SMs");
     // e4m3 pages of head_dim 128 go to the tensor memory kernel: 51 against 69 us at batch 32 x 4096 keys
-    if (e4m3 && p.D == 128) return launch_split_tc(sp, f, sms, dev, st);
+    if (e4m3 && p.D == 128) return launch_split_tc(sp, f, rows, sms, dev, st);
     const int nb = (int64_t)p.max_q * p.G <= 8 || p.D == 256 ? 1 : 2;
     switch ((p.D * 10 + nb) * 2 + (e4m3 ? 1 : 0)) {
-        case 1282: return launch_split_t<64, 1, false>(sp, f, sms, dev, st);
-        case 1283: return launch_split_t<64, 1, true>(sp, f, sms, dev, st);
-        case 1284: return launch_split_t<64, 2, false>(sp, f, sms, dev, st);
-        case 1285: return launch_split_t<64, 2, true>(sp, f, sms, dev, st);
-        case 2562: return launch_split_t<128, 1, false>(sp, f, sms, dev, st);
-        case 2564: return launch_split_t<128, 2, false>(sp, f, sms, dev, st);
-        case 5122: return launch_split_t<256, 1, false>(sp, f, sms, dev, st);
-        case 5123: return launch_split_t<256, 1, true>(sp, f, sms, dev, st);
+        case 1282: return launch_split_t<64, 1, false>(sp, f, rows, sms, dev, st);
+        case 1283: return launch_split_t<64, 1, true>(sp, f, rows, sms, dev, st);
+        case 1284: return launch_split_t<64, 2, false>(sp, f, rows, sms, dev, st);
+        case 1285: return launch_split_t<64, 2, true>(sp, f, rows, sms, dev, st);
+        case 2562: return launch_split_t<128, 1, false>(sp, f, rows, sms, dev, st);
+        case 2564: return launch_split_t<128, 2, false>(sp, f, rows, sms, dev, st);
+        case 5122: return launch_split_t<256, 1, false>(sp, f, rows, sms, dev, st);
+        case 5123: return launch_split_t<256, 1, true>(sp, f, rows, sms, dev, st);
         default: return set_status(FCCI_EUNSUPPORTED, "paged attention: unsupported head_dim");
     }
 }

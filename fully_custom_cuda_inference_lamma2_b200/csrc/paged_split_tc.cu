@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) paged_split_tc_kernel(const __g
 }
 
 template <int NB>
-static int launch_tc(TileParams& tp, const Freqs& f, int sms, int dev, cudaStream_t st) {
+static int launch_tc(TileParams& tp, const Freqs& f, const Params* rows, int sms, int dev, cudaStream_t st) {
     using C = TcCfg<NB>;
     static std::once_flag once[128];
     static cudaError_t attr[128];
@@ -542,14 +542,15 @@ static int launch_tc(TileParams& tp, const Freqs& f, int sms, int dev, cudaStrea
     if (!stages) return set_status(FCCI_EUNSUPPORTED, "paged attention: batch too large for shared memory");
     tp.stages = stages;
     CUtensorMap m[4];
-    const int rc = encode_pages<typename C::TL, true>(tp.p, m);
+    int rc = encode_pages<typename C::TL, true>(tp.p, m);
+    if (!rc) rc = append_before(rows, f, true, st);
     if (rc) return rc;
     return launch_pdl(paged_split_tc_kernel<NB>, dim3(sms * per_sm), dim3(kTcThreads), C::smem(stages, tp.p.B), st, m[0], m[1],
                       m[2], m[3], tp, f);
 }
 
-int launch_split_tc(TileParams& tp, const Freqs& f, int sms, int dev, cudaStream_t st) {
-    return tp.p.cu_q || tp.p.G <= 8 ? launch_tc<1>(tp, f, sms, dev, st) : launch_tc<2>(tp, f, sms, dev, st);
+int launch_split_tc(TileParams& tp, const Freqs& f, const Params* rows, int sms, int dev, cudaStream_t st) {
+    return tp.p.cu_q || tp.p.G <= 8 ? launch_tc<1>(tp, f, rows, sms, dev, st) : launch_tc<2>(tp, f, rows, sms, dev, st);
 }
 
 }  // namespace pg

@@ -194,14 +194,10 @@ static int paged_step(const fcci_paged_desc* d, Op op, cudaStream_t stream) {
         if (kv < 0) kv = (int64_t)((d->workspace_bytes - L.expanded) / ((size_t)p.Hkv * p.D * 4));
         return launch_prefill(p, f, e4m3, ws, L, (int)(kv < 0x7fffffff ? kv : 0x7fffffff), p.scale_log2, d->advance, stream);
     }
-    if (op == Op::kPrefill) {
-        Params rows = p;
-        rows.q = nullptr;
-        rc = launch_append(rows, f, e4m3, stream);
-        if (rc) return rc;
-    }
+    Params rows = p;  // a prefill's append of its rows
+    rows.q = nullptr;
     p.advance = d->advance;
-    return launch_split(p, f, e4m3, op == Op::kDecode && p.append, d->flags & FCCI_PAGED_PREFETCH_KV, ws, L, stream);
+    return launch_split(p, f, op == Op::kPrefill ? &rows : nullptr, e4m3, op == Op::kDecode && p.append, d->flags & FCCI_PAGED_PREFETCH_KV, ws, L, stream);
 }
 
 }  // namespace pg

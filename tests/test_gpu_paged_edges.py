@@ -319,6 +319,24 @@ def test_append_to_lengths_that_are_none(av, e4m3):
         assert (q_rot[5:75] == 7.0).all()
 
 
+def test_short_chunks_of_too_many_sequences(av):
+    """A call that is refused leaves the pages alone: the check comes before the append."""
+    B = 20000
+    pool = torch.zeros(B, 1, 16, 128, dtype=torch.uint8, device=DEV)
+    scales = torch.full((B, 1), 120, dtype=torch.uint8, device=DEV)
+    table = torch.arange(B, dtype=torch.int32, device=DEV).view(B, 1)
+    lens = torch.zeros(B, dtype=torch.int32, device=DEV)
+    q = randn_half((B, 1, 128), 435).to(DEV)
+    out = torch.full_like(q, 7.0)
+    cu = torch.arange(B + 1, dtype=torch.int32, device=DEV)
+    before = av.launch_count()
+    with pytest.raises(RuntimeError, match="batch too large"):
+        av.paged_prefill(q, q, q, pool.view(H.F8), pool.view(H.F8), out, table, lens, cu, 1, k_scales=scales, v_scales=scales, advance=True)
+    torch.cuda.synchronize()
+    assert av.launch_count() == before
+    assert (pool == 0).all() and (scales == 120).all() and (lens == 0).all() and (out == 7.0).all()
+
+
 # ---------------------------------------------------------------- bounds far above what a call holds
 
 @pytest.mark.parametrize("e4m3", [True, False])
