@@ -86,8 +86,9 @@ class PagedKVCache:
             raise RuntimeError(f"sequence {seq}: {tokens} tokens need more than {self.max_pages} pages")
         if need > len(self._free):
             raise RuntimeError(f"sequence {seq}: {need} pages needed, {len(self._free)} free")
-        new = [self._free.pop() for _ in range(need)]
+        new = self._free[:-need - 1:-1]
         self.page_table[seq, len(have):len(have) + need] = torch.tensor(new, dtype=torch.int32).to(self.device)
+        del self._free[-need:]
         have.extend(new)
 
     def release(self, seq: int) -> None:
