@@ -209,7 +209,8 @@ inline int64_t max_items(int B, int Hq, int total_q) { return ((int64_t)total_q 
 // Query rows of one kv head (new tokens x group) up to which a chunk takes the split-KV kernels. Split against expanding,
 // us, e4m3: 8 sequences of 2000 keys, 8 kv heads, 64 rows 76 against 107, 128 rows 122 against 108; one of 8000, 128
 // rows 59 against 140; 32 of 4000, 128 rows 646 against 948, 256 rows 1312 against 952; 16 of 500, 32 kv heads, 16 rows
-// 86 against 123, 32 rows 142 against 126. Where they cross depends on lengths that only the device knows.
+// 86 against 123, 32 rows 142 against 126. Where they cross depends on lengths that only the device knows; max_q is the
+// caller's bound on them, so a loose one sends short chunks the long way.
 constexpr int kSplitRows = 64;
 inline bool long_chunk(int Hq, int Hkv, int max_q) { return (int64_t)max_q * (Hq / Hkv) > kSplitRows; }
 WsLayout ws_layout(int B, int Hq, int Hkv, int D, int total_q, int max_q, int max_kv, int grid);

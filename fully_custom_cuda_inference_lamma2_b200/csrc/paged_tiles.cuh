@@ -5,9 +5,11 @@
 // A unit is (sequence b, kv head h, column group c): up to COLS query rows of the group, rows being
 // (token, query head) pairs, so a cached key is read once for all of them. A unit's keys are cut into tiles
 // of KEYS rows; all tiles of all units form one line, of which every CTA of a persistent grid takes an
-// equal stretch, whatever the lengths are. On the line a unit begins with kHead places that hold no tile: what
-// its queries and its end cost (17 sequences of 1 to 5000 keys x 8 kv heads, fp16: 56 us with none, 41 us with
-// 2, 40 us with 4; a CTA with eight units of one tile held up all). A unit that lies in one stretch is finished there; of a cut
+// equal stretch, whatever the lengths are. On the line a unit begins with kHead places that hold no tile: what its queries and
+// its end cost. With 0, 2, 4 and 8 places (us, a CTA with many short units held up all): e4m3, D 128, 64 sequences of 128 to
+// 8192 keys x 32 kv heads 529, 350, 332, 337; 17 of 1 to 5000 x 8 kv heads 40.0, 29.0, 27.5, 28.3; e4m3, D 64, the same
+// 472, 311, 295, 308 and 32.6, 23.9, 23.0, 24.4; fp16, D 128, 64 x 8 kv heads 203, 169, 167, 167 and 17 50.9, 42.6, 38.7, 37.0.
+// A unit that lies in one stretch is finished there; of a cut
 // one, every CTA leaves its part (o, log-sum-exp) in the workspace and the last to arrive joins them. No
 // CTA waits for another.
 #pragma once
@@ -183,8 +185,11 @@ struct Line {
         }
         CT = min(N, gridDim.x);
         if (uniform && N > 0) {
-            // equal units: a number of CTAs that is a multiple of the units keeps every cut at the same
-            // places of each, unless that leaves more than 15 % of the grid idle
+            // equal units: a number of CTAs that is a multiple of the units keeps every cut at the same places of each,
+            // unless that leaves more than 15 % of the grid idle. Us, with the rule and without, 8 kv heads, e4m3 D 128,
+            // e4m3 D 64, fp16 D 128: 32 x 4096 keys (14 % idle) 50.0 / 55.5, 45.1 / 45.9, 88.7 / 93.2; 35 x 2000 (5 %)
+            // 32.3 / 41.4, 26.9 / 32.6, 53.4 / 57.1; beyond it 30 x 4096 (19 %) 48.0 / 52.9, 45.1 / 43.7, 81.7 / 87.5 and
+            // 25 x 4096 (32 %) 44.3 / 46.8, 44.7 / 38.2, 75.3 / 76.4: there it depends on the kernel.
             const unsigned all = (unsigned)units[B];
             if (all <= gridDim.x) {
                 const unsigned k = min(gridDim.x / all, N / all);
