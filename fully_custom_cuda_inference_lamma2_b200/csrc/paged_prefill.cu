@@ -188,6 +188,7 @@ int launch_prefill(const Params& base, const Freqs& f, bool e4m3, uint8_t* ws, c
     a.v_cache = p.exp_v, a.v_sh = p.exp_sh, a.v_st = p.D;
     a.out = p.out, a.o_st = p.o_st, a.o_sh = p.o_sh;
     a.scale_log2 = scale_log2 / (kLongQuery * (e4m3 ? ldexpf(1.f, kLongKeyExp) : 1.f));
+    a.weight_log2 = 7.f;  // keys down to 2^-31 of a row's largest weight count (2^-24 with 0), and thousands may share it
     a.advance = advance;
     a.err = p.err;
     uint32_t* head = reinterpret_cast<uint32_t*>(ws + 32);

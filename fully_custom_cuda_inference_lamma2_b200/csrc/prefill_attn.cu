@@ -34,7 +34,7 @@
 //   S_g  = Q_g K_j^T       tcgen05.mma kind::f16, M=128 N=128, A and B K-major
 //   O_g += P_g V_j         A = P_g from TMEM, B = V_j MN-major (head_dim contiguous)
 // The row maximum is only moved when it grows by more than 2^8 (P then stays
-// below 256, exact in fp16 range), so the O correction (TMEM load, scale,
+// below 256, times 2^weight_log2, in fp16's range), so the O correction (TMEM load, scale,
 // store) is rare after the first tiles.
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     m = mx;
                     l *= alpha;
                 }
-                const float mu = (m == -INFINITY) ? 0.f : m;
+                const float mu = ((m == -INFINITY) ? 0.f : m) - p.weight_log2;
                 const float2 scl = make_float2(sl2, sl2), nmu = make_float2(-mu, -mu);
                 float2 rsa = make_float2(0.f, 0.f), rsb = make_float2(0.f, 0.f);
                 // P = 2^(s * scale * log2 e - m) as fp16 over the first 64 columns of S_g;

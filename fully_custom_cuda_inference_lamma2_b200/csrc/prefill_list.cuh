@@ -33,6 +33,7 @@ struct Params {
     __half* out;
     int64_t o_st, o_sh;
     float scale_log2;
+    float weight_log2;  // log2 of the weight of a row's maximum when that moves, at most 7 (it may then grow by 2^8)
     float rope_theta;
     int32_t rotary_dim;
     int32_t advance;

@@ -190,6 +190,35 @@ def test_decode_many_keys_far_below_one(av, D, e4m3):
         assert worst <= tol, f"gap {gap}: {worst / want:.3g} of the result lost"
 
 
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_long_chunk_many_keys_far_below_one(av, e4m3):
+    """The same for a chunk of 70 tokens behind them: there a weight is fp16 and the largest lies between 2^7 and 2^15, so
+    that each is off by 2^-32 of the largest at most, or by 2^-11 of itself."""
+    T, n, page = 16384, 70, 64
+    pages = T // page + 2
+    k = torch.zeros(pages, 1, page, 128)
+    v = torch.ones(pages, 1, page, 128)
+    k[0, 0, 0, 0], v[0, 0, 0] = 8.0, 0.0
+    kind = H.F8 if e4m3 else torch.float16
+    for gap in (14.0, 18.0):
+        kp, vp = k.to(kind).to(DEV), v.to(kind).to(DEV)
+        scales = [torch.full((pages, 1), 127, dtype=torch.uint8, device=DEV).view(H.E8) if e4m3 else None for _ in range(2)]
+        table = torch.arange(pages, dtype=torch.int32, device=DEV).view(1, pages)
+        lens = torch.tensor([T], dtype=torch.int32, device=DEV)
+        q = torch.zeros(n, 1, 128, dtype=torch.float16, device=DEV)
+        q[:, :, 0] = 8.0
+        out = torch.empty_like(q)
+        av.paged_prefill(q, torch.zeros_like(q), torch.ones_like(q), kp, vp, out, table, lens,
+                         torch.tensor([0, n], dtype=torch.int32, device=DEV), n, k_scales=scales[0], v_scales=scales[1],
+                         scale=gap / 64.0, rotary_dim=0)
+        keys = T + 1 + torch.arange(n, dtype=torch.float64)
+        rest = (keys - 1) * math.exp(-gap)
+        want = (rest / (1 + rest))[:, None, None]
+        tol = keys[:, None, None] * 2.0 ** -32 + want * (2.0 ** -10 + 2 * T * 2.0 ** -24) + 2.0 ** -25
+        worst = ((out.cpu().double() - want).abs() / tol).max()
+        assert worst <= 1, f"gap {gap}: {float(worst):.3g} times the tolerance, {float(out.max() / want.max()):.3g} of the result"
+
+
 @pytest.mark.parametrize("D", [128, 64, 256])
 @pytest.mark.parametrize("group", [2, 16])
 def test_decode_values_of_uneven_scales(av, D, group):
