@@ -9,8 +9,9 @@
 // to fp16, as in the attention over an arena (the queries halved, so that none passes its range): holding the queries in two parts, as the split kernels do, would add half to the products of a kernel that the
 // products bound (results are off by 3.5e-4 to 5.4e-4 in the 2-norm, 2.1e-4 of it their own rounding).
 //
-// Measured: 2 x 2048 new tokens after 12000 to 14000, 64 / 8 heads: attention 1598 us, append 61, expansion 45 (3.6 TB/s
-// in and out); 16 prompts of 256 to 4096, 32 heads: attention 722 us, append 335.
+// Measured: 2 x 2048 new tokens after 12000 to 14000, 64 / 8 heads: attention 1456 us, append 61, expansion 45 (3.6 TB/s
+// in and out); 16 prompts of 256 to 4096, 32 heads: attention 659 us, append 335 (one pass; in a loop, under the power cap,
+// the attention takes up to 1600 and 720).
 //
 // Launches: the plan (row ranges, work list), the append (which also writes its own rows expanded, while it has
 // them), the expansion of the rows cached before, the attention.

@@ -25,8 +25,8 @@
 //   - m moves only when a weight would exceed 2^15.75 (e5m2 ends at 57344), to leave the largest at 2^13: O in
 //     tensor memory is scaled rarely, and four warps agree on it with one barrier a tile.
 //
-// Measured: 32 x 4096 keys, 8 kv heads 51.8 us (5.2 TB/s; 6.4 in the loop, the rest is the start: lengths, queries, first
-// tiles, and the end); 64 sequences of 128 to 8192 keys, 32 kv heads 385 us (5.8 TB/s). A tile takes the softmax some 1900
+// Measured: 32 x 4096 keys, 8 kv heads 51.2 us (5.3 TB/s; 6.4 in the loop, the rest is the start: lengths, queries, first
+// tiles, and the end); 64 sequences of 128 to 8192 keys, 32 kv heads 384 us (5.8 TB/s). A tile takes the softmax some 1900
 // cycles of latency, less than the memory needs for it with two CTAs an SM.
 //
 // 224 threads: warps 0..3 softmax (TMEM lane t = key t, then dim t), warps 4 and 6 fetch K and V, warp 5 issues the
