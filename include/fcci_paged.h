@@ -68,7 +68,7 @@ extern "C" {
  *                fp32 products
  *   append       rows T_b .. T_b + n_b - 1, each value rounded once from fp32: to fp16, or to
  *                e4m3 after the exact product with 2^-e. e of a page is the smallest in
- *                [-15, 8] with max|new rows of the page| <= 448 * 2^e, or the page's present e
+ *                [-15, 8] with max|new rows of the page| (in fp32) <= 448 * 2^e, or the page's present e
  *                if that is larger and the page holds rows below T_b; if e grows, those
  *                rows are rounded to the new scale. Infinities saturate, NaN stays NaN. A page
  *                that gets rows must belong to one sequence alone.
