@@ -6,8 +6,9 @@
 // ones take the split-KV kernels, which read the pages in place). code * 2^e is exact in fp16 for every scale that an
 // append makes, but for a value's 256 * 2^8, which becomes 65504 (2^-11 of itself, an fp16 rounding); rotated keys go up to
 // 352 * 2^8 and are expanded at half their size (paged.cuh: kLongKeyExp). The rotated queries and the weights are rounded once
-// to fp16, as in the attention over an arena (the queries halved, so that none passes its range): holding the queries in two parts, as the split kernels do, would add half to the products of a kernel that the
-// products bound (results are off by 3.5e-4 to 5.4e-4 in the 2-norm, 2.1e-4 of it their own rounding).
+// to fp16, as in the attention over an arena (the queries halved, so that none passes its range): holding the queries in
+// two parts, as the split kernels do, would add half to the products of a kernel that the products bound, and take shared
+// memory for two more tiles (results are off by 3.5e-4 to 4.2e-4 in the 2-norm, 2.1e-4 of it their own rounding).
 //
 // Measured: 2 x 2048 new tokens after 12000 to 14000, 64 / 8 heads: attention 1456 us, append 61, expansion 45 (3.6 TB/s
 // in and out); 16 prompts of 256 to 4096, 32 heads: attention 659 us, append 335 (one pass; in a loop, under the power cap,
